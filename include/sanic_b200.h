@@ -89,7 +89,7 @@ int32_t sanic_sync(sanic_ctx* ctx, void* stream);
  * src/metal.rs:686-705; there is no device-side injector here): writes `code` into the context's status word exactly as a
  * kernel whose bounded wait ran out would, so the next sanic_sync returns the matching error and clears the word.
  * Codes: 1-29 mbarrier waits of the tensor-core kernels, 31-33 persistent step (grid barrier, ring full, ring empty),
- * 41+q peer flag of rank q, 51 gather index, 52 decode length clamp. No kernel is launched and nothing on the device is disturbed. */
+ * 41+q peer flag of rank q, 51 gather index, 52 decode length clamp, 53-56 the paged-cache entry points. No kernel is launched and nothing on the device is disturbed. */
 int32_t sanic_status_inject(sanic_ctx* ctx, int32_t code);
 
 /* ── carrier structure: what the emitter keys kernel choice on (src/derive.rs:519-530) ── */
@@ -551,6 +551,103 @@ int32_t sanic_machine_instantiate(sanic_schedule* s, const sanic_state_decl* sta
 int32_t sanic_machine_output(sanic_replay* m, const char* name, sanic_buffer_view* out);  /* Machine::output (src/graph.rs:343-356) */
 /* The buffer state `name` will be read from by the NEXT step (to load a prefilled cache, or to read a state back). */
 int32_t sanic_machine_state(sanic_replay* m, const char* name, sanic_buffer_view* out);
+
+/* ── serving over a paged key/value cache ──
+ * The reference decodes one sequence against one contiguous cache (src/nn.rs:208-212, src/graph.rs:127-160); these entry
+ * points are the ragged, many-request form of that step and have no counterpart there. A pool holds n_pages pages of
+ * page_size key (value) rows; page tables map request b's key j to row j % page_size of page block_table[b][j / page_size].
+ * A step is: sanic_page_table_append (lengths -> table entries, slots, positions), sanic_paged_cache_write (RoPE and the
+ * write of the new keys and values), sanic_attn_paged, and, where the new tokens were drafted, sanic_draft_verify. All
+ * lengths, tables and slots are read from the device, so a captured step replays over new lengths. What the device reads is
+ * checked there: nothing outside the given extents is read or written, and an entry out of range is reported by the next
+ * sanic_sync on the context (SANIC_ERR_INVALID, codes 53-56). Captured: the calls allocate nothing and may be captured; two
+ * graphs that may replay at the same time need workspaces of their own. */
+
+/* Page tables, slots and positions of one step, from the requests' lengths. Request b holds seq_lens[b] tokens in
+ * held_pages[b] pages (held_pages NULL: ceil(seq_lens / page_size)) and appends new_lens[b] (0 allowed). With
+ * need_b = ceil((seq_lens[b] + new_lens[b]) / page_size) it takes max(0, need_b - held_b) pages off the END of the free list, requests
+ * in order: the r-th page taken in the whole step is free_pages[*free_count - 1 - r]. Entries that a row holds already, and
+ * entries behind the ones taken, are left as they were. Outputs: query_start [n + 1] (exclusive sums of new_lens), kv_lens
+ * (seq + new), pages_out (pages the row holds now), *free_count_out, and per token row of the step its position and slot
+ * (page * page_size + row). Token rows behind the last request get slot -1 and position 0.
+ * A request that finds the list empty or its table row full keeps what it got: the missing entries are -1 (where the row has
+ * room for them), the tokens in them get slot -1, and code 53 is reported; so are a negative length (read as 0) and new
+ * tokens beyond n_tokens (query_start stops there). Outputs may not overlap inputs; block_table is updated in place. */
+typedef struct {
+    const int32_t* seq_lens; const int32_t* new_lens; const int32_t* held_pages;     /* [n_requests] */
+    const int32_t* free_pages; const int32_t* free_count;                           /* [free_capacity], device scalar */
+    int32_t* block_table; int64_t table_stride;                                     /* [n_requests, max_pages] */
+    int32_t* query_start; int32_t* kv_lens; int32_t* pages_out; int32_t* free_count_out;
+    int32_t* positions; int64_t* slots;                                             /* [n_tokens] */
+    int32_t n_requests, n_tokens, page_size, max_pages, free_capacity;              /* n_requests <= 8000 */
+} sanic_page_append_params;
+int32_t sanic_page_table_append(sanic_ctx* ctx, const sanic_page_append_params* p, void* stream);
+
+/* Rotate-half RoPE (src/nn.rs:176-194) of q and k at per-token positions, and the write of k and v into their page slots.
+ * q, k, v: token rows of heads, [n_tokens, heads, head_dim] with a stride between tokens (heads contiguous: slices of one
+ * fused projection are read in place), src_dtype f32, bf16 or f16. q_out: [n_tokens, q_heads, head_dim] at cache_dtype with a
+ * token stride; may be q itself when the types agree. q and q_out NULL: only the cache is written. table NULL (then positions
+ * may be NULL): no rotation. Arithmetic f32, one rounding at the store (f32 to f16 overflows to infinity). A token with a
+ * negative slot writes nothing, its q_out row neither. A slot or position past its extent is skipped and reported (code 56).
+ * Slots of one call must differ: which of two tokens with one slot remains is not defined. */
+typedef struct {
+    const void* q; const void* k; const void* v;
+    int64_t q_stride, k_stride, v_stride;            /* elements between tokens */
+    void* q_out; int64_t q_out_stride;
+    void* k_pages; void* v_pages;                    /* cache_dtype */
+    int64_t k_page_stride, k_row_stride, k_head_stride, v_page_stride, v_row_stride, v_head_stride;   /* elements; head_dim dense */
+    const float* table; const int32_t* positions; int32_t n_positions;   /* [n_positions][head_dim / 2][2], sanic_rope_table */
+    const int64_t* slots;
+    int32_t n_tokens, q_heads, kv_heads, head_dim;   /* head_dim a multiple of 16, at most 256 */
+    int32_t page_size, n_pages;
+    int32_t src_dtype, cache_dtype;                  /* cache_dtype SANIC_BF16 or SANIC_F16; src_dtype SANIC_F32 or the same */
+} sanic_paged_write_params;
+int32_t sanic_paged_cache_write(sanic_ctx* ctx, const sanic_paged_write_params* p, void* stream);
+
+/* Causal attention of every request's new tokens over its pages: the carrier of sanic_attn_fwd_bf16 / _decode_splitkv.
+ * Token i of request b (row query_start[b] + i of q) stands at position kv_lens[b] - len_b + i, len_b = query_start[b + 1] -
+ * query_start[b], and sees the keys at or before it, at most `window` of them when window > 0. The chunk's own keys are in
+ * the pages already. out [n_tokens, q_heads, head_dim] at dtype, dense; lse (optional) [n_tokens, q_heads] f32, the natural
+ * log of the sum of exp(scale q.k). A token that sees no key (position < 0) gets zeros and -inf. Rows of q outside every
+ * request's range, and their out and lse, are neither read for a result nor written. Keys no token of the request sees
+ * (behind kv_lens, before the window) are not read, whatever the pages hold there. Scores, maxima, sums and the output
+ * accumulator are f32; the weights exp(s - max) are rounded to dtype for the product with v. max_query_len, a bound on the
+ * chunk lengths (0: n_tokens), only selects a kernel: a longer chunk is still computed. dtype SANIC_BF16 or SANIC_F16,
+ * head_dim 64 or 128, at most 64 query heads per kv head. A table entry outside [0, n_pages) reads as zeros; it, and lengths
+ * past the table row or n_tokens (clamped), are reported (code 54). */
+typedef struct {
+    const void* q; void* out; float* lse;
+    const void* k_pages; const void* v_pages;
+    const int32_t* block_table; const int32_t* query_start; const int32_t* kv_lens;
+    void* workspace; size_t workspace_bytes;         /* sanic_attn_paged_workspace_bytes(), 16-byte aligned, any contents */
+    int64_t q_token_stride, q_head_stride;           /* elements; multiples of 8 */
+    int64_t k_page_stride, k_row_stride, k_head_stride, v_page_stride, v_row_stride, v_head_stride, table_stride;
+    int32_t dtype, n_requests, n_tokens, max_query_len, q_heads, kv_heads, head_dim, page_size, n_pages, max_pages, window;
+    float scale;
+} sanic_attn_paged_params;
+int32_t sanic_attn_paged(sanic_ctx* ctx, const sanic_attn_paged_params* p, void* stream);
+/* 0 when the parameters (pointers included, workspace excepted) are not valid. */
+size_t sanic_attn_paged_workspace_bytes(sanic_ctx* ctx, const sanic_attn_paged_params* p);
+
+/* Verification of drafted tokens: for request b, draft i (i < draft_lens[b]) with token x is accepted while
+ * u_accept[b][i] * q_i(x) < p_i(x), in order, up to the first that is not. p_i is row target_start[b] + i of target_probs
+ * (target_start NULL: b * (max_draft + 1)), q_i is draft_probs[b][i], or 1 on x and 0 elsewhere when draft_probs is NULL.
+ * One more token follows: after a rejection at i it is drawn with weights max(p_i - q_i, 0) (p_i itself if they are all 0), after
+ * draft_lens[b] acceptances with weights p of the next row. Drawn: the first j whose running sum of weights exceeds
+ * u_sample[b] times their total, in index order, sums in f64; weights that are NaN, infinite or not positive count as 0. tokens_out
+ * [n, max_draft + 1]: accepted drafts, the drawn token (-1 if no weight is positive), -1 behind it; accepted [n]: the count of drafts
+ * accepted. A draft token outside the vocabulary is rejected, draft lengths are clamped to [0, max_draft], a target row outside
+ * [0, target_rows) ends the request with -1; each is reported (code 55). */
+typedef struct {
+    const float* target_probs; int64_t target_stride; int32_t target_rows; const int32_t* target_start;
+    const float* draft_probs; int64_t draft_request_stride, draft_stride;     /* [n, max_draft, vocab] or NULL */
+    const int32_t* draft_tokens;                                              /* [n, max_draft] */
+    const int32_t* draft_lens;                                                /* [n], NULL: max_draft */
+    const float* u_accept; const float* u_sample;                             /* [n, max_draft], [n], in [0, 1) */
+    int32_t* tokens_out; int32_t* accepted;
+    int32_t n_requests, max_draft, vocab;                                     /* max_draft <= 32 */
+} sanic_draft_verify_params;
+int32_t sanic_draft_verify(sanic_ctx* ctx, const sanic_draft_verify_params* p, void* stream);
 
 /* ── planning facts, the device-level split, measured tuning ──
  * sanic_fitted_specs is the reference's DeviceSpecs (src/cost.rs:33-60: sram_bytes ... mem_latency_s, same meaning) with

@@ -164,6 +164,36 @@ class StateDecl(C.Structure):
     _fields_ = [("input_name", C.c_char_p), ("root", i32), ("pinned", i32)]
 
 
+class PageAppendParams(C.Structure):
+    _fields_ = [(n, vp) for n in ("seq_lens", "new_lens", "held_pages", "free_pages", "free_count", "block_table")] + \
+               [("table_stride", i64)] + \
+               [(n, vp) for n in ("query_start", "kv_lens", "pages_out", "free_count_out", "positions", "slots")] + \
+               [(n, i32) for n in ("n_requests", "n_tokens", "page_size", "max_pages", "free_capacity")]
+
+
+class PagedWriteParams(C.Structure):
+    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("q_stride", i64), ("k_stride", i64), ("v_stride", i64),
+                ("q_out", vp), ("q_out_stride", i64), ("k_pages", vp), ("v_pages", vp)] + \
+               [(f"{t}_{n}_stride", i64) for t in "kv" for n in ("page", "row", "head")] + \
+               [("table", vp), ("positions", vp), ("n_positions", i32), ("slots", vp)] + \
+               [(n, i32) for n in ("n_tokens", "q_heads", "kv_heads", "head_dim", "page_size", "n_pages", "src_dtype", "cache_dtype")]
+
+
+class AttnPagedParams(C.Structure):
+    _fields_ = [(n, vp) for n in ("q", "out", "lse", "k_pages", "v_pages", "block_table", "query_start", "kv_lens", "workspace")] + \
+               [("workspace_bytes", C.c_size_t), ("q_token_stride", i64), ("q_head_stride", i64)] + \
+               [(f"{t}_{n}_stride", i64) for t in "kv" for n in ("page", "row", "head")] + [("table_stride", i64)] + \
+               [(n, i32) for n in ("dtype", "n_requests", "n_tokens", "max_query_len", "q_heads", "kv_heads", "head_dim", "page_size",
+                                   "n_pages", "max_pages", "window")] + [("scale", f32)]
+
+
+class DraftVerifyParams(C.Structure):
+    _fields_ = [("target_probs", vp), ("target_stride", i64), ("target_rows", i32), ("target_start", vp), ("draft_probs", vp),
+                ("draft_request_stride", i64), ("draft_stride", i64)] + \
+               [(n, vp) for n in ("draft_tokens", "draft_lens", "u_accept", "u_sample", "tokens_out", "accepted")] + \
+               [(n, i32) for n in ("n_requests", "max_draft", "vocab")]
+
+
 class FittedSpecs(C.Structure):
     _fields_ = [(n, C.c_double) for n in ("sram_bytes", "regfile_bytes", "hbm_bandwidth", "peak_flops", "launch_overhead", "dtype_bytes")] + \
                [("compute_dtype", i32), ("boundary_dtype", i32)] + \
@@ -235,6 +265,11 @@ PROTOTYPES = {
     "sanic_generic_destroy": (i32, [vp]),
     "sanic_generic_kernel_name": (C.c_char_p, [vp]),
     "sanic_generic_cache_stats": (i32, [C.POINTER(i64), C.POINTER(i64)]),
+    "sanic_page_table_append": (i32, [vp, C.POINTER(PageAppendParams), vp]),
+    "sanic_paged_cache_write": (i32, [vp, C.POINTER(PagedWriteParams), vp]),
+    "sanic_attn_paged": (i32, [vp, C.POINTER(AttnPagedParams), vp]),
+    "sanic_attn_paged_workspace_bytes": (C.c_size_t, [vp, C.POINTER(AttnPagedParams)]),
+    "sanic_draft_verify": (i32, [vp, C.POINTER(DraftVerifyParams), vp]),
     "sanic_program_create": (i32, [vp, C.POINTER(StageDesc), i32, C.POINTER(vp)]),
     "sanic_program_destroy": (i32, [vp]),
     "sanic_program_kernel_count": (i32, [vp]),

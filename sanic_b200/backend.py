@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -28,6 +29,19 @@ _TORCH_DTYPE = {abi.F32: torch.float32, abi.BF16: torch.bfloat16, abi.F16: torch
 
 def _ptr(t):
     return C.c_void_p(t.data_ptr()) if t is not None else None
+
+
+class PageStep(NamedTuple):
+    """What page_table_append hands the rest of a step: all on the device."""
+    query_start: torch.Tensor    # [n + 1] int32
+    kv_lens: torch.Tensor        # [n] int32, new tokens included
+    held_pages: torch.Tensor     # [n] int32, the next step's held_pages
+    free_count: torch.Tensor     # [1] int32, the next step's free_count
+    positions: torch.Tensor      # [n_tokens] int32
+    slots: torch.Tensor          # [n_tokens] int64, -1 behind the last request
+
+
+_HALF = {torch.bfloat16: abi.BF16, torch.float16: abi.F16}
 
 
 class CudaDevice:
@@ -381,6 +395,169 @@ class CudaDevice:
         self._check(self.lib.sanic_rope_bf16(self.h, _ptr(x), _ptr(out), rows, seq, D, _ptr(table), pos0, self.stream()),
                     "rope_bf16")
         return out
+
+    # ── serving over a paged cache ──
+    def _paged(self, name, t, dtypes, rank):
+        """A tensor of this device with one of `dtypes`, dense along its last axis; any strides before it."""
+        if not isinstance(t, torch.Tensor) or t.get_device() != self.ordinal:
+            raise RunError(f"input `{name}` is not a tensor on {self.torch_device}")
+        if t.dtype not in dtypes:
+            raise RunError(f"input `{name}` has dtype {t.dtype}; expected {' or '.join(map(str, dtypes))}")
+        if t.dim() != rank:
+            raise RunError(f"input `{name}` has {t.dim()} axes; expected {rank}")
+        st = t.stride()
+        if st[-1] != 1 and t.shape[-1] > 1 and t.numel():
+            raise RunError(f"input `{name}` must be contiguous along its last axis")
+        return st
+
+    def _flat(self, name, t, dtype, n):
+        if not isinstance(t, torch.Tensor) or t.get_device() != self.ordinal:
+            raise RunError(f"input `{name}` is not a tensor on {self.torch_device}")
+        if t.dtype != dtype:
+            raise RunError(f"input `{name}` has dtype {t.dtype}; expected {dtype}")
+        if t.numel() != n or not t.is_contiguous():
+            raise RunError(f"input `{name}` must hold {n} contiguous elements; its shape is {tuple(t.shape)}")
+        return t.data_ptr()
+
+    def page_table_append(self, seq_lens, new_lens, block_table, free_pages, free_count, page_size, n_tokens, held_pages=None):
+        """Page tables, slots and positions of one step from the requests' lengths: request b (seq_lens[b] tokens held in
+        held_pages[b] pages, default their ceil) appends new_lens[b] tokens and takes the pages it lacks off the end of
+        free_pages[:free_count] into its row of block_table [n, max_pages], in place. seq_lens, new_lens, held_pages [n],
+        free_pages and free_count [1] are int32; n_tokens token rows are laid out (at least the sum of new_lens; rows behind it get
+        slot -1). Returns a PageStep. Nothing is read back: a pool that runs out is reported by the next sync()."""
+        n = seq_lens.shape[0]
+        st = self._paged("block_table", block_table, (torch.int32,), 2)
+        if block_table.shape[0] != n:
+            raise RunError(f"block_table has {block_table.shape[0]} rows for {n} requests")
+        i32 = torch.int32
+        n_tokens = int(n_tokens)
+        if n_tokens < 0:
+            raise RunError("n_tokens must not be negative")
+        # one allocation for the five int32 outputs, each 16-byte aligned
+        pad = lambda k: (k + 3) // 4 * 4
+        a, b, c = pad(n + 1), pad(n), pad(n_tokens)
+        ints = torch.empty(a + 2 * b + 4 + c, dtype=i32, device=self.torch_device)
+        out = PageStep(ints[:n + 1], ints[a:a + n], ints[a + b:a + b + n], ints[a + 2 * b:a + 2 * b + 1],
+                       ints[a + 2 * b + 4:a + 2 * b + 4 + n_tokens], torch.empty(n_tokens, dtype=torch.int64, device=self.torch_device))
+        base = ints.data_ptr()
+        p = abi.PageAppendParams(
+            self._flat("seq_lens", seq_lens, i32, n), self._flat("new_lens", new_lens, i32, n),
+            None if held_pages is None else self._flat("held_pages", held_pages, i32, n),
+            self._flat("free_pages", free_pages, i32, free_pages.numel()), self._flat("free_count", free_count, i32, 1),
+            block_table.data_ptr(), st[0], base, base + 4 * a, base + 4 * (a + b), base + 4 * (a + 2 * b), base + 4 * (a + 2 * b + 4),
+            out.slots.data_ptr(), n, n_tokens, int(page_size), block_table.shape[1], free_pages.numel())
+        self._check(self.lib.sanic_page_table_append(self.h, C.byref(p), self.stream()), "page_table_append")
+        return out
+
+    def _pages(self, k_pages, v_pages):
+        if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
+            raise RunError(f"k_pages {tuple(k_pages.shape)} {k_pages.dtype} and v_pages {tuple(v_pages.shape)} {v_pages.dtype} disagree")
+        return (self._paged("k_pages", k_pages, (torch.bfloat16, torch.float16), 4),
+                self._paged("v_pages", v_pages, (torch.bfloat16, torch.float16), 4))
+
+    def _token_rows(self, name, t, dtype, n_tokens, heads, dim):
+        st = self._paged(name, t, (dtype,), 3)
+        if t.shape[0] != n_tokens or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+            raise RunError(f"input `{name}` has shape {tuple(t.shape)}; expected [{n_tokens}, {heads if heads is not None else 'heads'}, {dim}]")
+        if t.shape[1] > 1 and st[1] != dim:
+            raise RunError(f"the heads of `{name}` must lie side by side")
+        return st[0]
+
+    def paged_cache_write(self, k, v, k_pages, v_pages, slots, q=None, positions=None, rope_table=None, q_out=None):
+        """k, v [n_tokens, kv_heads, D] -> rows slots[t] (page * page_size + row, int64; negative: skipped) of k_pages, v_pages
+        [n_pages, page_size, kv_heads, D] bf16 or f16 (any strides: a transposed [n_pages, kv_heads, page_size, D] pool too), in place.
+        With rope_table (of rope_table()) and positions [n_tokens] int32, k and q [n_tokens, q_heads, D] are rotated first.
+        k, v and q are slices of one projection or tensors of their own, f32 or of the pages' type. Returns q at the pages'
+        type (into q_out when given, which may be q), or None without q. Rows of q with a negative slot stay unwritten."""
+        ks, vs = self._pages(k_pages, v_pages)
+        n_pages, page_size, hkv, d = k_pages.shape
+        t = k.shape[0]
+        src = k.dtype
+        if src != torch.float32 and src != k_pages.dtype:
+            raise RunError(f"input `k` has dtype {src}; expected torch.float32 or {k_pages.dtype}")
+        kst, vst = self._token_rows("k", k, src, t, hkv, d), self._token_rows("v", v, src, t, hkv, d)
+        qst = qost = hq = 0
+        if q is not None:
+            hq = q.shape[1]
+            qst = self._token_rows("q", q, src, t, hq, d)
+            if q_out is None:
+                q_out = torch.empty((t, hq, d), dtype=k_pages.dtype, device=self.torch_device)
+            qost = self._token_rows("q_out", q_out, k_pages.dtype, t, hq, d)
+        elif q_out is not None:
+            raise RunError("q_out needs q")
+        n_pos = 0
+        if rope_table is not None:
+            if positions is None:
+                raise RunError("rope_table needs positions")
+            n_pos = rope_table.shape[0]
+            if tuple(rope_table.shape[1:]) != (d // 2, 2):
+                raise RunError(f"rope_table has shape {tuple(rope_table.shape)}; expected [positions, {d // 2}, 2]")
+            self._flat("rope_table", rope_table, torch.float32, rope_table.numel())
+        p = abi.PagedWriteParams(
+            None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), qst, kst, vst, None if q is None else q_out.data_ptr(), qost,
+            k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+            None if rope_table is None else rope_table.data_ptr(),
+            None if rope_table is None else self._flat("positions", positions, torch.int32, t), n_pos, self._flat("slots", slots, torch.int64, t),
+            t, hq, hkv, d, page_size, n_pages, abi.F32 if src == torch.float32 else _HALF[src], _HALF[k_pages.dtype])
+        self._check(self.lib.sanic_paged_cache_write(self.h, C.byref(p), self.stream()), "paged_cache_write")
+        return q_out
+
+    def attn_paged(self, q, k_pages, v_pages, block_table, query_start, kv_lens, max_query_len=0, window=0, scale=None, return_lse=False,
+                   out=None):
+        """Causal attention of every request's new tokens over its pages. q [n_tokens, Hq, D] bf16 or f16: request b's chunk is rows
+        query_start[b] .. query_start[b + 1], its last token standing at key kv_lens[b] - 1 (the chunk's own keys are in the pages
+        already). k_pages, v_pages [n_pages, page_size, Hkv, D] (any strides), block_table [n, max_pages], query_start [n + 1] and
+        kv_lens [n] int32. -> out [n_tokens, Hq, D] (or into `out`), and with return_lse the log-sum-exp [n_tokens, Hq] f32.
+        max_query_len, a bound on the chunks known on the host, selects the kernel. Rows outside every chunk stay unwritten."""
+        qs = self._paged("q", q, (torch.bfloat16, torch.float16), 3)
+        ks, vs = self._pages(k_pages, v_pages)
+        ts = self._paged("block_table", block_table, (torch.int32,), 2)
+        T, hq, d = q.shape
+        n_pages, page_size, hkv, dk = k_pages.shape
+        n, max_pages = block_table.shape
+        if dk != d or q.dtype != k_pages.dtype:
+            raise RunError(f"attention shapes disagree: q {tuple(q.shape)} {q.dtype}, pages {tuple(k_pages.shape)} {k_pages.dtype}")
+        if out is None:
+            out = torch.empty((T, hq, d), dtype=q.dtype, device=self.torch_device)
+        out_ptr = self._flat("out", out, q.dtype, T * hq * d)
+        lse = torch.empty((T, hq), dtype=torch.float32, device=self.torch_device) if return_lse else None
+        p = abi.AttnPagedParams(
+            q.data_ptr(), out_ptr, lse.data_ptr() if return_lse else None, k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
+            self._flat("query_start", query_start, torch.int32, n + 1), self._flat("kv_lens", kv_lens, torch.int32, n), None, 0,
+            qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], ts[0], _HALF[q.dtype], n, T, int(max_query_len), hq, hkv, d, page_size,
+            n_pages, max_pages, int(window), float(scale) if scale is not None else 1.0 / math.sqrt(d))
+        # a workspace per call: calls on other streams, and graphs that replay side by side, never share one
+        nbytes = self.lib.sanic_attn_paged_workspace_bytes(self.h, C.byref(p))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.torch_device)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
+        self._check(self.lib.sanic_attn_paged(self.h, C.byref(p), self.stream()), "attn_paged")
+        return (out, lse) if return_lse else out
+
+    def draft_verify(self, target_probs, draft_tokens, u_accept, u_sample, draft_probs=None, draft_lens=None, target_start=None):
+        """Rejection sampling of drafted tokens (see sanic_draft_verify). target_probs [rows, vocab] f32: request b's rows start at
+        target_start[b] (default b * (K + 1)), one per draft and one more; draft_tokens [n, K] int32, draft_probs [n, K, vocab] f32
+        (None: drafts made without probabilities), draft_lens [n] int32 (None: all K); u_accept [n, K] and u_sample [n] f32 in [0, 1).
+        -> tokens [n, K + 1] int32 (kept drafts, the drawn token, then -1) and the number of drafts kept [n] int32."""
+        ts = self._paged("target_probs", target_probs, (torch.float32,), 2)
+        rows, vocab = target_probs.shape
+        if draft_tokens.dim() != 2:
+            raise RunError(f"input `draft_tokens` has shape {tuple(draft_tokens.shape)}; expected [requests, drafts]")
+        n, k = draft_tokens.shape
+        ds = (0, 0, 1)
+        if draft_probs is not None:
+            ds = self._paged("draft_probs", draft_probs, (torch.float32,), 3)
+            if tuple(draft_probs.shape) != (n, k, vocab):
+                raise RunError(f"input `draft_probs` has shape {tuple(draft_probs.shape)}; expected {(n, k, vocab)}")
+        i32, f32 = torch.int32, torch.float32
+        out = torch.empty((n, k + 1), dtype=i32, device=self.torch_device)
+        accepted = torch.empty(n, dtype=i32, device=self.torch_device)
+        p = abi.DraftVerifyParams(
+            target_probs.data_ptr(), ts[0], rows, None if target_start is None else self._flat("target_start", target_start, i32, n),
+            None if draft_probs is None or not k else draft_probs.data_ptr(), ds[0], ds[1], self._flat("draft_tokens", draft_tokens, i32, n * k) or None,
+            None if draft_lens is None else self._flat("draft_lens", draft_lens, i32, n), self._flat("u_accept", u_accept, f32, n * k) or None,
+            self._flat("u_sample", u_sample, f32, n), out.data_ptr(), accepted.data_ptr(), n, k, vocab)
+        self._check(self.lib.sanic_draft_verify(self.h, C.byref(p), self.stream()), "draft_verify")
+        return out, accepted
 
     # ── K4 ──
     def round_to_bf16_bits(self, x):

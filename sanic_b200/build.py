@@ -32,7 +32,7 @@ def _stale(target, deps):
 
 def _compile(src, verbose):
     obj = os.path.join(BUILD, src[:-3] + ".o")
-    deps = [os.path.join(CSRC, src)] + [os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith(".cuh")]
+    deps = [os.path.join(CSRC, src)] + [os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith((".cuh", ".h"))]
     deps.append(os.path.join(HERE, "..", "include", "sanic_b200.h"))
     if not _stale(obj, deps):
         return obj, ""

@@ -1,0 +1,242 @@
+// Verification of drafted tokens by rejection sampling, from given uniform numbers, so that the tokens kept are distributed as
+// the target's: draft x_i is kept while u_i q_i(x_i) < p_i(x_i) (an exact product of two f32 in f64); the token behind the kept
+// ones is drawn from max(p - q, 0) after a rejection, else from the next row's p, as the first index whose running sum exceeds
+// u times the total.
+//
+// Only one row of p (and of q after a rejection) is read per request: which one is known after at most max_draft gathered
+// pairs, which one warp takes at once. HBM bounds a batch (4 or 8 bytes per vocabulary entry); a single request is a chain of
+// latencies: lengths and tokens, their probabilities, the row, the join. One cluster of CTAs serves a request: each CTA sums
+// its slice of the row, the slices' totals are exchanged through distributed shared memory, and the CTA that holds the drawn
+// token finds it from the sums of 128-entry chunks that it kept, so that only one chunk is read twice. No workspace, no atomics:
+// the sums have a fixed order for a given cluster size. They are f64: a running sum in f32 would put the border of about one
+// entry in a thousand on its other side at a vocabulary of 1e5.
+#include <cooperative_groups.h>
+
+#include "paged.cuh"
+
+namespace {
+using namespace sanic;
+namespace cg = cooperative_groups;
+
+constexpr int THREADS = 512, WARPS = THREADS / 32;
+constexpr int CHUNK = 128;                        // entries of a warp's step
+constexpr int STEP = WARPS * CHUNK;               // entries of a block's step
+constexpr int MAX_STEPS = 256;                    // per CTA: 2^19 entries
+constexpr int MAX_CLUSTER = 16;
+
+enum { FROM_TARGET = 0, FROM_DIFFERENCE = 1, WITHOUT_TOKEN = 2 };
+
+struct Row { const float* p; const float* q; int mode, token; bool vec; };
+
+__device__ __forceinline__ double weight(float p, float q, const Row& r, int j) {
+    double w = r.mode == FROM_DIFFERENCE ? (double)p - (double)q : (double)p;
+    if (r.mode == WITHOUT_TOKEN && j == r.token) w = 0.0;
+    return w > 0.0 && w <= 3.402823466e38 ? w : 0.0;      // NaN, infinities and negative values count as 0
+}
+
+// sum over one warp chunk of entries [c, c + 128) below `end`; all lanes receive it
+__device__ __forceinline__ double chunk_sum(const Row& r, int c, int end, int lane) {
+    float p[4], q[4];
+    const bool full = c + CHUNK <= end;
+    if (full && r.vec) {
+        const float4 a = __ldcs((const float4*)(r.p + c + lane * 4));
+        p[0] = a.x; p[1] = a.y; p[2] = a.z; p[3] = a.w;
+        if (r.mode == FROM_DIFFERENCE) {
+            const float4 b = __ldcs((const float4*)(r.q + c + lane * 4));
+            q[0] = b.x; q[1] = b.y; q[2] = b.z; q[3] = b.w;
+        } else q[0] = q[1] = q[2] = q[3] = 0.0f;
+        double s = 0.0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s += weight(p[i], q[i], r, c + lane * 4 + i);
+        return s;
+    }
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {                          // rows that start off a 16-byte boundary: lanes side by side
+        const int j = c + i * 32 + lane;
+        const bool in = j < end;
+        p[i] = in ? __ldcs(r.p + j) : 0.0f;
+        q[i] = in && r.mode == FROM_DIFFERENCE ? __ldcs(r.q + j) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s += weight(p[i], q[i], r, c + i * 32 + lane);
+    return s;
+}
+__device__ __forceinline__ double warp_sum64(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ double warp_scan64(double v, int lane) {     // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const double x = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += x; }
+    return v;
+}
+
+__global__ void __launch_bounds__(THREADS) draft_verify_kernel(const sanic_draft_verify_params p, int* err) {
+    cg::cluster_group cluster = cg::this_cluster();
+    const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int b = blockIdx.x / cs;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    __shared__ double s_sum[MAX_STEPS * WARPS];       // per warp chunk: its sum, then the sum of all chunks up to it
+    __shared__ double s_total;
+    __shared__ int s_count, s_len, s_start, s_token;
+    griddep_wait();
+    griddep_launch();
+
+    if (warp == 0) {
+        const int K = p.max_draft;
+        int len = p.draft_lens ? p.draft_lens[b] : K;
+        int start = p.target_start ? p.target_start[b] : b * (K + 1);
+        bool bad = len < 0 || len > K;
+        len = min(max(len, 0), K);
+        const bool no_rows = start < 0 || (long long)start + len >= p.target_rows;
+        bad |= no_rows;
+        bool ok = false;
+        int tok = -1;
+        if (lane < len && !no_rows) {
+            tok = p.draft_tokens[(int64_t)b * K + lane];
+            if ((unsigned)tok < (unsigned)p.vocab) {
+                const float pt = p.target_probs[(int64_t)(start + lane) * p.target_stride + tok];
+                const float qt = p.draft_probs ? p.draft_probs[(int64_t)b * p.draft_request_stride + (int64_t)lane * p.draft_stride + tok] : 1.0f;
+                ok = (double)p.u_accept[(int64_t)b * K + lane] * (double)qt < (double)pt;
+            } else bad = true;
+        }
+        const unsigned failed = ~__ballot_sync(0xffffffffu, ok);      // lanes past the drafts are among them
+        const int count = failed ? __ffs(failed) - 1 : 32;
+        const int rejected = __shfl_sync(0xffffffffu, tok, min(count, 31));
+        if (rank == 0) {
+            int32_t* out = p.tokens_out + (int64_t)b * (K + 1);
+            for (int i = lane; i <= K; i += 32) if (i != count || no_rows) out[i] = -1;      // the drawn token's place is written below
+            __syncwarp();
+            if (lane < count) out[lane] = tok;
+            if (lane == 0) p.accepted[b] = count;
+            if (__any_sync(0xffffffffu, bad) && lane == 0 && err) atomicCAS(err, 0, paged::STATUS_VERIFY);
+        }
+        if (lane == 0) { s_count = count; s_len = len; s_start = no_rows ? -1 : start; s_token = rejected; }
+    }
+    __syncthreads();
+    if (s_start < 0) return;                          // every CTA of the cluster alike
+    const int count = s_count;
+    const bool rejected = count < s_len;
+    Row row;
+    row.p = p.target_probs + (int64_t)(s_start + count) * p.target_stride;
+    row.q = p.draft_probs ? p.draft_probs + (int64_t)b * p.draft_request_stride + (int64_t)min(count, max(p.max_draft - 1, 0)) * p.draft_stride : nullptr;
+    row.token = s_token;
+    row.mode = !rejected ? FROM_TARGET : (p.draft_probs ? FROM_DIFFERENCE : WITHOUT_TOKEN);
+
+    // this CTA's slice: whole block steps
+    const int steps_all = (p.vocab + STEP - 1) / STEP;
+    const int st0 = (int)((long long)steps_all * rank / cs), st1 = (int)((long long)steps_all * (rank + 1) / cs);
+    const int n_chunks = (st1 - st0) * WARPS;
+    double total = 0.0, base = 0.0;
+    while (true) {
+        row.vec = ((uintptr_t)row.p % 16) == 0 && (row.mode != FROM_DIFFERENCE || ((uintptr_t)row.q % 16) == 0);
+#pragma unroll 4
+        for (int st = st0; st < st1; ++st) {
+            const int c = st * STEP + warp * CHUNK;
+            double v = c < p.vocab ? chunk_sum(row, c, p.vocab, lane) : 0.0;
+            v = warp_sum64(v);
+            if (lane == 0) s_sum[(st - st0) * WARPS + warp] = v;
+        }
+        __syncthreads();
+        if (warp == 0) {                              // running sums over the chunks
+            double carry = 0.0;
+            for (int i = 0; i < n_chunks; i += 32) {
+                double v = warp_scan64(i + lane < n_chunks ? s_sum[i + lane] : 0.0, lane) + carry;
+                if (i + lane < n_chunks) s_sum[i + lane] = v;
+                carry = __shfl_sync(0xffffffffu, v, 31);
+            }
+            if (lane == 0) s_total = carry;
+        }
+        cluster.sync();
+        total = 0.0;
+        for (int r = 0; r < cs; ++r) {
+            if (r == rank) base = total;
+            total += *cluster.map_shared_rank(&s_total, r);
+        }
+        const bool again = !(total > 0.0) && row.mode != FROM_TARGET;
+        if (!again) break;
+        row.mode = FROM_TARGET;                       // nothing left of p - q: p itself
+        cluster.sync();                               // the totals are read before they are written again
+    }
+    const double x = (double)p.u_sample[b] * total;
+    // the owner: the first CTA whose running sum exceeds x; the last one with any weight if rounding left none
+    int owner = -1, last = -1;
+    double run = 0.0;
+    for (int r = 0; r < cs; ++r) {
+        const double mine = *cluster.map_shared_rank(&s_total, r);
+        run += mine;
+        if (mine > 0.0) last = r;
+        if (owner < 0 && run > x) owner = r;
+    }
+    if (owner < 0) owner = last;
+    int32_t* drawn = p.tokens_out + (int64_t)b * (p.max_draft + 1) + count;
+    if (owner < 0) { if (rank == 0 && tid == 0) *drawn = -1; }
+    else if (rank == owner && warp == 0) {
+        int chunk = -1, final_chunk = 0;
+        for (int i = 0; i < n_chunks && chunk < 0; i += 32) {
+            const bool in = i + lane < n_chunks;
+            const double v = in ? s_sum[i + lane] : 0.0, before = in && i + lane > 0 ? s_sum[i + lane - 1] : 0.0;
+            const unsigned over = __ballot_sync(0xffffffffu, in && base + v > x), some = __ballot_sync(0xffffffffu, in && v > before);
+            if (over) chunk = i + __ffs(over) - 1;
+            if (some) final_chunk = i + 31 - __clz(some);
+        }
+        if (chunk < 0) chunk = final_chunk;
+        const int c = st0 * STEP + chunk * CHUNK;
+        double w[4], own = 0.0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = c + lane * 4 + i;
+            w[i] = j < p.vocab ? weight(row.p[j], row.mode == FROM_DIFFERENCE ? row.q[j] : 0.0f, row, j) : 0.0;
+            own += w[i];
+        }
+        double acc = base + (chunk > 0 ? s_sum[chunk - 1] : 0.0) + (warp_scan64(own, lane) - own);
+        int hit = -1, positive = -1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            acc += w[i];
+            if (w[i] > 0.0) { positive = c + lane * 4 + i; if (hit < 0 && acc > x) hit = positive; }
+        }
+        const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), pos = __ballot_sync(0xffffffffu, positive >= 0);
+        const int from = hits ? __ffs(hits) - 1 : (pos ? 31 - __clz(pos) : 0);
+        const int token = __shfl_sync(0xffffffffu, hits ? hit : positive, from);
+        if (lane == 0) *drawn = token;
+    }
+    cluster.sync();                                   // no CTA leaves while another may read its total
+}
+}  // namespace
+
+extern "C" int32_t sanic_draft_verify(sanic_ctx* ctx, const sanic_draft_verify_params* p, void* stream) {
+    if (!ctx || !p) return SANIC_ERR_INVALID;
+    SANIC_REQUIRE(ctx, p->n_requests >= 0 && p->max_draft >= 0 && p->vocab > 0, "draft_verify: bad counts");
+    if (p->max_draft > 32) return sanic_fail(ctx, SANIC_ERR_UNSUPPORTED, "draft_verify: at most 32 drafted tokens per request");
+    if (p->vocab > (1 << 19)) return sanic_fail(ctx, SANIC_ERR_UNSUPPORTED, "draft_verify: at most 524288 vocabulary entries");
+    if (p->n_requests == 0) return SANIC_OK;
+    SANIC_REQUIRE(ctx, p->target_probs && p->u_sample && p->tokens_out && p->accepted && p->target_rows > 0, "draft_verify: null tensor");
+    SANIC_REQUIRE(ctx, p->max_draft == 0 || (p->draft_tokens && p->u_accept), "draft_verify: drafts need tokens and u_accept");
+    SANIC_REQUIRE(ctx, p->target_stride >= p->vocab || p->target_rows == 1, "draft_verify: target rows overlap");
+    SANIC_REQUIRE(ctx, !p->draft_probs || (p->draft_stride >= p->vocab && p->draft_request_stride >= 0), "draft_verify: draft rows overlap");
+    sanic_set_device(ctx);
+    // CTAs per request: enough that the batch covers four blocks per SM, at most 16 (a cluster's limit) and never less than a
+    // block step each
+    const int steps = (p->vocab + STEP - 1) / STEP;
+    int cs = 1;
+    while (cs < MAX_CLUSTER && 2 * cs * (long long)p->n_requests <= 4ll * ctx->sm_count && 2 * cs <= steps) cs *= 2;
+    static thread_local int ready_on = -1;
+    if (ready_on != ctx->device) {
+        SANIC_CUDA_CHECK(ctx, cudaFuncSetAttribute(draft_verify_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        ready_on = ctx->device;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p->n_requests * cs); cfg.blockDim = dim3(THREADS); cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cs; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    static const bool pdl = getenv("SANIC_NO_PDL") == nullptr;
+    cfg.attrs = attr; cfg.numAttrs = pdl ? 2 : 1;
+    SANIC_CUDA_CHECK(ctx, cudaLaunchKernelEx(&cfg, draft_verify_kernel, *p, ctx->status_dev));
+    return SANIC_OK;
+}

@@ -1,0 +1,90 @@
+// Attention of ragged chunks over a paged cache: what its two kernels (paged_attn.cu, paged_attn_tc.cu) share. The lengths
+// live on the device: every CTA finds its own range of the work (paged_sched.h) from them.
+#pragma once
+#include "common.cuh"
+#include "paged_sched.h"
+
+namespace sanic {
+namespace paged {
+
+constexpr int STATUS_POOL = 53;     // page_table_append: free list, table row or token rows exhausted, or a negative length
+constexpr int STATUS_ATTN = 54;     // attn_paged: a page or a length out of range
+constexpr int STATUS_VERIFY = 55;   // draft_verify: a token, draft length or target row out of range
+constexpr int STATUS_WRITE = 56;    // paged_cache_write: a slot or position out of range
+constexpr int MAX_REQUESTS = 8000;  // prefix sums over the requests are held in shared memory
+
+// What both kernels need of sanic_attn_paged_params, plus the split of the rows and of the workspace.
+struct Params : Shape {
+    const void* q; void* out; float* lse; const void* k; const void* v;
+    const int32_t* table; const int32_t* query_start; const int32_t* kv_lens;
+    int64_t q_token_stride, q_head_stride, k_page_stride, k_row_stride, k_head_stride, v_page_stride, v_row_stride, v_head_stride,
+        table_stride;
+    int n_tokens, q_heads, group, page_size, page_shift, n_pages, max_pages;
+    float scale;
+    int rows;              // rows of a partial slot (at least block_tokens * group)
+    // workspace: float [2 * ctas][rows][head_dim], float2 (max in log2 units, sum) [2 * ctas][rows], one int4 per CTA: the item
+    // that starts in its range and is shared with the next CTAs (first token row, tokens, kv head, CTAs that hold a part; 0: none)
+    float* ws_o; float2* ws_ml; int4* ws_merge;
+};
+
+#ifdef __CUDACC__
+// Lengths come from the device and are never trusted beyond what the host vouched for: token rows inside [0, n_tokens],
+// keys inside the table's row.
+struct LoadReq {
+    const Params* p;
+    int* err;              // null: do not report
+    __device__ __forceinline__ Req operator()(int b) const {
+        const int s = __ldcg(p->query_start + b), e = __ldcg(p->query_start + b + 1), kv = __ldcg(p->kv_lens + b);
+        Req r;
+        r.q0 = min(max(s, 0), p->n_tokens);
+        r.qn = min(max(e, r.q0), p->n_tokens) - r.q0;
+        r.kv = (int)min((long long)max(kv, 0), (long long)p->max_pages * p->page_size);
+        if ((r.q0 != s || r.q0 + r.qn != e || r.kv != kv) && err) atomicCAS(err, 0, STATUS_ATTN);
+        return r;
+    }
+};
+template <int KT> using DeviceWalk = Walk<KT, LoadReq>;
+
+// Prefix sums of the requests' costs into cum[0 .. n] (shared memory), by the whole block.
+template <int KT>
+__device__ __forceinline__ void scan_costs(const Params& p, long long* cum, int* err) {
+    __shared__ long long warp_sums[32];
+    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
+    const LoadReq load{&p, blockIdx.x == 0 ? err : nullptr};
+    long long carry = 0;
+    if (tid == 0) cum[0] = 0;
+    for (int b0 = 0; b0 < p.n_requests; b0 += nt) {
+        const int b = b0 + tid;
+        long long c = b < p.n_requests ? request_cost<KT>(p, load(b)) : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const long long x = __shfl_up_sync(0xffffffffu, c, o); if (lane >= o) c += x; }
+        if (lane == 31) warp_sums[warp] = c;
+        __syncthreads();
+        long long before = carry, all = 0;
+        for (int w = 0; w < nt / 32; ++w) { const long long x = warp_sums[w]; if (w < warp) before += x; all += x; }
+        if (b < p.n_requests) cum[b + 1] = before + c;
+        carry += all;
+        __syncthreads();
+    }
+    __syncthreads();
+}
+
+// The page and row of a key, and whether the page is one of the pool's. A table entry outside the pool reads as zeros and is
+// reported; nothing is ever read through it.
+__device__ __forceinline__ bool locate(const Params& p, const int32_t* row, int key, int& page, int& in_page, int* err) {
+    const int idx = p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+    in_page = key - idx * p.page_size;
+    page = __ldcg(row + idx);
+    if ((unsigned)page < (unsigned)p.n_pages) return true;
+    if (err) atomicCAS(err, 0, STATUS_ATTN);
+    return false;
+}
+#endif
+
+// paged_attn_tc.cu: the form for many rows. Whether its loads suit this layout; its launch (`q` complete).
+bool tc_supported(const sanic_attn_paged_params* p);
+int32_t tc_launch(sanic_ctx* ctx, const Params& q, int head_dim, int dtype, int ctas, void* stream);
+constexpr int TC_ROWS = 256;
+
+}  // namespace paged
+}  // namespace sanic

@@ -1,0 +1,475 @@
+// Causal attention of ragged chunks of new tokens over a paged key/value cache: the online-softmax fold (m, l, o) of
+// out_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys j at or before token i's own position (and inside a sliding
+// window), keys and values found through a page table.
+//
+// This file: the form for few query rows per (request, kv head) (decode, drafted tokens), the merge of items that several
+// CTAs share, and the entry point. paged_attn_tc.cu: the form for many rows.
+//
+// With R = tokens * (query heads per kv head) rows the fold does 4 R flop per key element and reads it once (2 bytes for
+// each of k and v), so below about 64 rows HBM bounds it: what matters is bytes in flight and equal ranges. A CTA of four
+// warps folds 64-key tiles that arrive by 16-byte cp.async through a ring of 3 (head_dim 128) or 4 (64) stages; a tile's
+// page lookups run one tile ahead of its copies. The rows of an item are 16 MT rows of m16n8k16 MMAs: with MT = 1 each warp
+// takes 16 of the tile's keys, with MT = 2 a warp takes 16 rows and half of the keys, with MT = 4 a warp takes 16 rows and
+// all keys. Carriers stay in registers; the warps that share rows merge once per segment. P goes to the tensor core rounded
+// to the storage type (bf16: 2^-9 per weight; f16 likewise after a shift by 2^8, which keeps the weights of a long flat
+// softmax out of f16's subnormals), sums and maxima are f32.
+// Rows are spread over an exactly resident grid as one contiguous range of (item, key tile) per CTA (see paged.cuh).
+#include "paged.cuh"
+
+namespace {
+using namespace sanic;
+using namespace sanic::paged;
+
+constexpr int KT = 64;
+
+template <int D> struct Cfg {
+    static constexpr int STAGES = (D == 128) ? 3 : 4;
+    static constexpr int TILE_BYTES = KT * D * 2;
+    static constexpr int STAGE_BYTES = 2 * TILE_BYTES;
+    static constexpr int RING = STAGES * STAGE_BYTES;
+    static constexpr int PREFIX_MAX = RING;            // the prefix sums over the requests share the ring's memory
+    static_assert((MAX_REQUESTS + 1) * 8 <= PREFIX_MAX, "prefix sums fit the ring");
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <bool BF16> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool BF16> constexpr float p_shift() { return BF16 ? 0.0f : 8.0f; }
+
+// One K tile and one V tile into a stage: [D/64 halves][64 keys][128 B], chunk index xor (key & 7). `off` holds the tile's
+// element offsets of k and v per key, -1 where nothing is to be read (beyond the keys the item sees, or a bad page): zeros
+// then, so that whatever a page holds there never meets a zero weight.
+template <int D>
+__device__ __forceinline__ void load_tile(const uint16_t* k, const uint16_t* v, const longlong2* off, uint32_t stage, int tid) {
+    constexpr int CPR = D / 8;
+#pragma unroll
+    for (int i = 0; i < (KT * CPR) / 128; ++i) {
+        const int id = i * 128 + tid, key = id / CPR, c = id % CPR;
+        const longlong2 o = off[key];
+        const uint32_t dst = stage + (c >> 3) * (KT * 128) + key * 128 + (((c & 7) ^ (key & 7)) << 4);
+        cp_async16(dst, k + (o.x >= 0 ? o.x + c * 8 : 0), o.x >= 0 ? 16 : 0);
+        cp_async16(dst + Cfg<D>::TILE_BYTES, v + (o.x >= 0 ? o.y + c * 8 : 0), o.x >= 0 ? 16 : 0);
+    }
+}
+
+template <int D, int MT, bool BF16>
+__global__ void __launch_bounds__(128) paged_rows_kernel(const __grid_constant__ Params p, int* err) {
+    constexpr int R = 16 * MT, WK = 4 / MT, KW = KT / WK, NC = KW / 16;    // rows, warps along keys, keys and 16-key chunks per warp
+    constexpr int KS = D / 16, NT = D / 8, STAGES = Cfg<D>::STAGES;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ longlong2 s_off[STAGES][KT];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int wr = warp % MT, wk = warp / MT;
+    const uint32_t base = smem_u32(smem);
+
+    griddep_wait();        // q, the pages, the table and the lengths come from earlier kernels of the step
+    griddep_launch();
+    scan_costs<KT>(p, (long long*)smem, err);
+    DeviceWalk<KT> walk{LoadReq{&p, nullptr}};
+    walk.init(p, (long long*)smem, blockIdx.x, gridDim.x);
+    __syncthreads();       // the prefix sums' memory becomes the tile ring
+
+    int4 merge = make_int4(0, 0, 0, 0);
+    const float sl2 = p.scale * LOG2E;
+    Seg s;
+    while (walk.next(p, s)) {
+        const int n_tiles = s.je - s.jb;
+        const int32_t* row = p.table + (int64_t)s.b * p.table_stride;
+        const uint16_t* K = (const uint16_t*)p.k + s.hk * p.k_head_stride;
+        const uint16_t* V = (const uint16_t*)p.v + s.hk * p.v_head_stride;
+        const int block0 = s.rb * p.block_tokens;                              // first token of the item in its chunk
+        const int n_tok = min(p.block_tokens, s.r.qn - block0);
+
+        // element offsets of a tile's keys, by threads 0..63
+        auto offsets = [&](int tile, int key_in_tile) {
+            longlong2 o = make_longlong2(-1, -1);
+            const int key = (s.jb + tile) * KT + key_in_tile;
+            if (key >= s.lo && key < s.hi) {
+                int page, in_page;
+                if (locate(p, row, key, page, in_page, err))
+                    o = make_longlong2(page * p.k_page_stride + in_page * p.k_row_stride, page * p.v_page_stride + in_page * p.v_row_stride);
+            }
+            return o;
+        };
+        for (int i = tid; i < STAGES * KT; i += 128)
+            if (i / KT < n_tiles) s_off[i / KT][i % KT] = offsets(i / KT, i % KT);
+        __syncthreads();
+#pragma unroll
+        for (int st = 0; st < STAGES - 1; ++st) {
+            if (st < n_tiles) load_tile<D>(K, V, s_off[st], base + st * Cfg<D>::STAGE_BYTES, tid);
+            cp_async_commit();
+        }
+
+        // query fragments: row r of the item is head r % group of token r / group
+        const int ra = wr * 16 + g, rc = ra + 8;
+        const int ta = ra / p.group, tc = rc / p.group;
+        uint32_t qf[KS][4];
+        {
+            const uint16_t* Q = (const uint16_t*)p.q + (int64_t)(s.r.q0 + block0) * p.q_token_stride + (int64_t)s.hk * p.group * p.q_head_stride;
+            const uint16_t* qa = Q + ta * p.q_token_stride + (ra - ta * p.group) * p.q_head_stride + 2 * t;
+            const uint16_t* qc = Q + tc * p.q_token_stride + (rc - tc * p.group) * p.q_head_stride + 2 * t;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                qf[ks][0] = ta < n_tok ? *(const uint32_t*)(qa + ks * 16) : 0u;
+                qf[ks][1] = tc < n_tok ? *(const uint32_t*)(qc + ks * 16) : 0u;
+                qf[ks][2] = ta < n_tok ? *(const uint32_t*)(qa + ks * 16 + 8) : 0u;
+                qf[ks][3] = tc < n_tok ? *(const uint32_t*)(qc + ks * 16 + 8) : 0u;
+            }
+        }
+        // keys a row sees: [first, first + count)
+        const int pos_a = s.r.kv - s.r.qn + block0 + ta, pos_c = s.r.kv - s.r.qn + block0 + tc;
+        const int lo_a = p.window > 0 ? max(0, pos_a - p.window + 1) : 0, lo_c = p.window > 0 ? max(0, pos_c - p.window + 1) : 0;
+        const unsigned cnt_a = ta < n_tok ? max(0, pos_a + 1 - lo_a) : 0, cnt_c = tc < n_tok ? max(0, pos_c + 1 - lo_c) : 0;
+
+        float o[NT][4];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) { o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f; }
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;      // rows ra and rc, log2 units
+        for (int it = 0; it < n_tiles; ++it) {
+            cp_async_wait<STAGES - 2>();
+            __syncthreads();
+            const int nx = it + STAGES - 1;
+            if (nx < n_tiles) load_tile<D>(K, V, s_off[nx % STAGES], base + (nx % STAGES) * Cfg<D>::STAGE_BYTES, tid);
+            cp_async_commit();
+            longlong2 ahead;
+            const bool look = tid < KT && nx + 1 < n_tiles;
+            if (look) ahead = offsets(nx + 1, tid);
+
+            const uint32_t ks_addr = base + (it % STAGES) * Cfg<D>::STAGE_BYTES, vs_addr = ks_addr + Cfg<D>::TILE_BYTES;
+            float sc[NC][2][4];
+            {
+                const int mi = lane >> 3, r = lane & 7;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[c][0][i] = sc[c][1][i] = 0.0f;
+                    const int krow = wk * KW + c * 16 + (mi >> 1) * 8 + r;
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        const int ch = 2 * ks + (mi & 1);
+                        uint32_t r0, r1, r2, r3;
+                        ldmatrix_x4(ks_addr + (ch >> 3) * (KT * 128) + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4), r0, r1, r2, r3);
+                        mma16816<BF16>(sc[c][0], qf[ks], r0, r1);
+                        mma16816<BF16>(sc[c][1], qf[ks], r2, r3);
+                    }
+                }
+            }
+            float mx0 = -INFINITY, mx1 = -INFINITY;
+            const int key0 = (s.jb + it) * KT + wk * KW + 2 * t;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int key = key0 + c * 16 + h * 8 + i;
+                        sc[c][h][i] = (unsigned)(key - lo_a) < cnt_a ? sc[c][h][i] * sl2 : -INFINITY;
+                        sc[c][h][2 + i] = (unsigned)(key - lo_c) < cnt_c ? sc[c][h][2 + i] * sl2 : -INFINITY;
+                        mx0 = fmaxf(mx0, sc[c][h][i]); mx1 = fmaxf(mx1, sc[c][h][2 + i]);
+                    }
+            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1)); mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1)); mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+            const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
+            const float a0 = m0 > -INFINITY ? ex2(m0 - mn0) : 0.0f, a1 = m1 > -INFINITY ? ex2(m1 - mn1) : 0.0f;
+            const float sub0 = (mn0 > -INFINITY ? mn0 : 0.0f) - p_shift<BF16>(), sub1 = (mn1 > -INFINITY ? mn1 : 0.0f) - p_shift<BF16>();
+            m0 = mn0; m1 = mn1;
+            float t0 = 0.0f, t1 = 0.0f;
+            uint32_t pf[NC][4];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                float e[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    e[h][0] = ex2(sc[c][h][0] - sub0); e[h][1] = ex2(sc[c][h][1] - sub0);
+                    e[h][2] = ex2(sc[c][h][2] - sub1); e[h][3] = ex2(sc[c][h][3] - sub1);
+                    t0 += e[h][0] + e[h][1]; t1 += e[h][2] + e[h][3];
+                }
+                pf[c][0] = pack2<BF16>(e[0][0], e[0][1]); pf[c][1] = pack2<BF16>(e[0][2], e[0][3]);
+                pf[c][2] = pack2<BF16>(e[1][0], e[1][1]); pf[c][3] = pack2<BF16>(e[1][2], e[1][3]);
+            }
+            l0 = l0 * a0 + t0; l1 = l1 * a1 + t1;
+            if (__any_sync(0xffffffffu, a0 != 1.0f || a1 != 1.0f)) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) { o[i][0] *= a0; o[i][1] *= a0; o[i][2] *= a1; o[i][3] *= a1; }
+            }
+            {
+                const int mi = lane >> 3, r = lane & 7;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const int krow = wk * KW + c * 16 + (mi & 1) * 8 + r;
+#pragma unroll
+                    for (int dp = 0; dp < D / 16; ++dp) {
+                        const int ch = 2 * dp + (mi >> 1);
+                        uint32_t r0, r1, r2, r3;
+                        ldmatrix_x4_trans(vs_addr + (ch >> 3) * (KT * 128) + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4), r0, r1, r2, r3);
+                        mma16816<BF16>(o[2 * dp], pf[c], r0, r1);
+                        mma16816<BF16>(o[2 * dp + 1], pf[c], r2, r3);
+                    }
+                }
+            }
+            if (look) s_off[(nx + 1) % STAGES][tid] = ahead;
+        }
+        cp_async_wait<0>();
+        __syncthreads();      // every warp is done with the ring: it takes the warps' carriers
+
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+        float2* ml = (float2*)smem;                        // [WK][R] (max, sum)
+        float* os = (float*)(smem + WK * R * 8);           // [WK][R][D + 4]
+        constexpr int OW = D + 4;
+        if (t == 0) { ml[wk * R + ra] = make_float2(m0, l0); ml[wk * R + rc] = make_float2(m1, l1); }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            *(float2*)(os + (wk * R + ra) * OW + 8 * i + 2 * t) = make_float2(o[i][0], o[i][1]);
+            *(float2*)(os + (wk * R + rc) * OW + 8 * i + 2 * t) = make_float2(o[i][2], o[i][3]);
+        }
+        __syncthreads();
+        const bool whole = s.starts && s.finishes;
+        const size_t slot = partial_slot(s, blockIdx.x);
+        const int rows = n_tok * p.group;
+        for (int idx = tid; idx < rows * (D / 4); idx += 128) {
+            const int r = idx / (D / 4), d = (idx % (D / 4)) * 4;
+            float m = -INFINITY, l = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) m = fmaxf(m, ml[w * R + r].x);
+            float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int w = 0; w < WK; ++w) {
+                const float2 x = ml[w * R + r];
+                const float f = x.x > -INFINITY ? ex2(x.x - m) : 0.0f;       // a side that saw nothing has weight 0
+                const float4 v4 = *(const float4*)(os + (w * R + r) * OW + d);
+                l += f * x.y;
+                acc.x += f * v4.x; acc.y += f * v4.y; acc.z += f * v4.z; acc.w += f * v4.w;
+            }
+            if (whole) {
+                const int tok = r / p.group, head = s.hk * p.group + r - tok * p.group;
+                const int64_t at = (int64_t)(s.r.q0 + block0 + tok) * p.q_heads + head;
+                const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;      // no visible key: zeros, and -inf for the log-sum-exp
+                *(uint2*)((uint16_t*)p.out + at * D + d) =
+                    make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+                if (p.lse && d == 0) p.lse[at] = (m + log2f(l) - p_shift<BF16>()) * LN2;
+            } else {
+                *(float4*)(p.ws_o + (slot * p.rows + r) * D + d) = acc;
+                if (d == 0) p.ws_ml[slot * p.rows + r] = make_float2(m, l);
+            }
+        }
+        if (s.parts > 1) merge = make_int4(s.r.q0 + block0, n_tok, s.hk, s.parts);
+        __syncthreads();
+    }
+    if (tid == 0) p.ws_merge[blockIdx.x] = merge;
+}
+
+// Merge of the items that several CTAs share. Block (c, y) serves the item that starts in CTA c's range, rows y, y + gridDim.y, ..
+// groups of warps: a row's parts are split over 16 / rows warps (at least one) and joined through shared memory in a fixed order.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(512) paged_merge_kernel(const __grid_constant__ Params p) {
+    griddep_wait();
+    griddep_launch();
+    const int4 it = p.ws_merge[blockIdx.x];
+    if (it.w <= 1) return;
+    __shared__ float2 s_ml[16];
+    __shared__ float s_o[16][D];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int V = D / 32;                      // floats per lane
+    const int rows = it.y * p.group;
+    const int r0 = (int)((long long)rows * blockIdx.y / gridDim.y), r1 = (int)((long long)rows * (blockIdx.y + 1) / gridDim.y);
+    int wpr = 16;                                  // warps per row
+    while (wpr > 1 && (r1 - r0) * wpr > 16) wpr >>= 1;
+    const int rpp = 16 / wpr, sub = warp % wpr;    // rows at a time, this warp's share of the parts
+    for (int rr = r0; rr < r1; rr += rpp) {
+        const int r = rr + warp / wpr;
+        float m = -INFINITY, l = 0.0f, o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = 0.0f;
+        if (r < r1) {
+            for (int q0 = sub; q0 < it.w; q0 += wpr * 4) {
+                float2 x[4]; float a[4][V];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int q = q0 + u * wpr;
+                    x[u] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) a[u][i] = 0.0f;
+                    if (q < it.w) {
+                        const size_t at = ((size_t)(blockIdx.x + q) * 2 + (q == 0 ? 1 : 0)) * p.rows + r;
+                        x[u] = __ldcg(p.ws_ml + at);
+                        const float* po = p.ws_o + at * D + lane * V;
+                        if (V == 4) { const float4 f = __ldcg((const float4*)po); a[u][0] = f.x; a[u][1] = f.y; a[u][V - 2] = f.z; a[u][V - 1] = f.w; }
+                        else { const float2 f = __ldcg((const float2*)po); a[u][0] = f.x; a[u][1] = f.y; }
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const float mn = fmaxf(m, x[u].x);
+                    const float fa = m > -INFINITY ? ex2(m - mn) : 0.0f, fb = x[u].x > -INFINITY ? ex2(x[u].x - mn) : 0.0f;
+                    l = l * fa + x[u].y * fb;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o[i] = o[i] * fa + a[u][i] * fb;
+                    m = mn;
+                }
+            }
+        }
+        if (wpr > 1) {
+            if (lane == 0) s_ml[warp] = make_float2(m, l);
+#pragma unroll
+            for (int i = 0; i < V; ++i) s_o[warp][lane * V + i] = o[i];
+            __syncthreads();
+            if (sub == 0) {
+                for (int w = 1; w < wpr; ++w) {
+                    const float2 x = s_ml[warp + w];
+                    const float mn = fmaxf(m, x.x);
+                    const float fa = m > -INFINITY ? ex2(m - mn) : 0.0f, fb = x.x > -INFINITY ? ex2(x.x - mn) : 0.0f;
+                    l = l * fa + x.y * fb;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o[i] = o[i] * fa + s_o[warp + w][lane * V + i] * fb;
+                    m = mn;
+                }
+            }
+            __syncthreads();
+        }
+        if (r < r1 && sub == 0) {
+            const int tok = r / p.group, head = it.z * p.group + r - tok * p.group;
+            const int64_t at = (int64_t)(it.x + tok) * p.q_heads + head;
+            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            uint16_t* dst = (uint16_t*)p.out + at * D + lane * V;
+            *(uint32_t*)dst = pack2<BF16>(o[0] * inv, o[1] * inv);
+            if (V == 4) *(uint32_t*)(dst + 2) = pack2<BF16>(o[V - 2] * inv, o[V - 1] * inv);
+            if (p.lse && lane == 0) p.lse[at] = (m + log2f(l) - p_shift<BF16>()) * LN2;
+        }
+    }
+}
+
+template <int D, int MT, bool BF16>
+int32_t launch_rows(sanic_ctx* ctx, const Params& p, int ctas, cudaStream_t st) {
+    constexpr int merge_bytes = (4 / MT) * 16 * MT * (8 + (D + 4) * 4);
+    constexpr int smem = Cfg<D>::RING > merge_bytes ? Cfg<D>::RING : merge_bytes;
+    static thread_local int ready_on = -1;       // the attribute is per device
+    if (ready_on != ctx->device) {
+        SANIC_CUDA_CHECK(ctx, cudaFuncSetAttribute(paged_rows_kernel<D, MT, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        ready_on = ctx->device;
+    }
+    SANIC_CUDA_CHECK(ctx, launch_pdl(paged_rows_kernel<D, MT, BF16>, dim3(ctas), dim3(128), smem, st, p, ctx->status_dev));
+    return SANIC_OK;
+}
+template <int MT>
+int32_t launch_rows_any(sanic_ctx* ctx, const Params& p, int D, int dtype, int ctas, cudaStream_t st) {
+    if (D == 128) return dtype == SANIC_BF16 ? launch_rows<128, MT, true>(ctx, p, ctas, st) : launch_rows<128, MT, false>(ctx, p, ctas, st);
+    return dtype == SANIC_BF16 ? launch_rows<64, MT, true>(ctx, p, ctas, st) : launch_rows<64, MT, false>(ctx, p, ctas, st);
+}
+
+// Resident CTAs of the rows kernel: two or three per SM, what its shared memory leaves (96 or 64 KB each).
+int rows_ctas(const sanic_ctx* ctx, int D) { return ctx->sm_count * (D == 128 ? 2 : 3); }
+
+// Which form serves a call, and the rows of an item.
+struct Plan { bool tc; int rows, ctas; };
+Plan make_plan(const sanic_ctx* ctx, const sanic_attn_paged_params* p) {
+    const int group = p->q_heads / p->kv_heads;
+    const long long want = (long long)(p->max_query_len > 0 ? p->max_query_len : p->n_tokens) * group;
+    Plan pl{};
+    pl.rows = 16;
+    while (pl.rows < 64 && pl.rows < want) pl.rows *= 2;
+    pl.ctas = rows_ctas(ctx, p->head_dim);
+    return pl;
+}
+
+size_t workspace_bytes(const Plan& pl, int D) {
+    const size_t slots = 2 * (size_t)pl.ctas * pl.rows;
+    return slots * D * 4 + slots * 8 + (size_t)pl.ctas * 16;
+}
+
+int32_t validate(sanic_ctx* ctx, const sanic_attn_paged_params* p) {
+    SANIC_REQUIRE(ctx, p->n_requests >= 0 && p->n_tokens >= 0 && p->max_query_len >= 0, "attn_paged: negative count");
+    // an empty call has tensors without elements
+    SANIC_REQUIRE(ctx, p->n_requests == 0 || p->n_tokens == 0 || (p->q && p->out && p->k_pages && p->v_pages && p->block_table && p->query_start && p->kv_lens),
+                  "attn_paged: null tensor");
+    SANIC_REQUIRE(ctx, p->dtype == SANIC_BF16 || p->dtype == SANIC_F16, "attn_paged: q, the pages and out are bf16 or f16");
+    if (p->head_dim != 64 && p->head_dim != 128) return sanic_fail(ctx, SANIC_ERR_UNSUPPORTED, "attn_paged: head_dim must be 64 or 128");
+    SANIC_REQUIRE(ctx, p->kv_heads > 0 && p->q_heads > 0 && p->q_heads % p->kv_heads == 0, "attn_paged: query heads must be a multiple of key/value heads");
+    if (p->q_heads / p->kv_heads > 64) return sanic_fail(ctx, SANIC_ERR_UNSUPPORTED, "attn_paged: at most 64 query heads per key/value head");
+    SANIC_REQUIRE(ctx, p->n_requests <= MAX_REQUESTS, "attn_paged: at most 8000 requests per call");
+    SANIC_REQUIRE(ctx, p->page_size > 0 && p->n_pages > 0 && p->max_pages > 0, "attn_paged: empty page pool or table");
+    SANIC_REQUIRE(ctx, (long long)p->max_pages * p->page_size < (1ll << 31) - 256, "attn_paged: a table row spans 2^31 keys or more");
+    SANIC_REQUIRE(ctx, (long long)p->n_tokens * p->q_heads < (1ll << 31), "attn_paged: too many rows");
+    SANIC_REQUIRE(ctx, p->window >= 0, "attn_paged: negative window");
+    SANIC_REQUIRE(ctx, p->scale > 0.0f && p->scale < INFINITY, "attn_paged: scale must be positive and finite");
+    SANIC_REQUIRE(ctx, p->q_token_stride % 8 == 0 && p->q_head_stride % 8 == 0 && p->k_page_stride % 8 == 0 && p->k_row_stride % 8 == 0 &&
+                  p->k_head_stride % 8 == 0 && p->v_page_stride % 8 == 0 && p->v_row_stride % 8 == 0 && p->v_head_stride % 8 == 0 &&
+                  ((uintptr_t)p->q % 16) == 0 && ((uintptr_t)p->k_pages % 16) == 0 && ((uintptr_t)p->v_pages % 16) == 0 && ((uintptr_t)p->out % 16) == 0,
+                  "attn_paged: rows of q, k, v and out must be 16-byte aligned");
+    SANIC_REQUIRE(ctx, p->q_token_stride >= 0 && p->q_head_stride >= 0 && p->k_page_stride >= 0 && p->k_row_stride >= 0 && p->k_head_stride >= 0 &&
+                  p->v_page_stride >= 0 && p->v_row_stride >= 0 && p->v_head_stride >= 0, "attn_paged: negative stride");
+    SANIC_REQUIRE(ctx, p->n_requests <= 1 || p->table_stride >= p->max_pages, "attn_paged: table rows overlap");
+    return SANIC_OK;
+}
+}  // namespace
+
+namespace {
+// One block column per CTA of the fold; `row_split` blocks share an item's rows.
+void launch_merge(const Params& p, int D, int dtype, int ctas, int row_split, cudaStream_t st, cudaError_t* e) {
+    const dim3 grid(ctas, row_split), block(512);
+    if (D == 128) *e = dtype == SANIC_BF16 ? launch_pdl(paged_merge_kernel<128, true>, grid, block, 0, st, p) : launch_pdl(paged_merge_kernel<128, false>, grid, block, 0, st, p);
+    else *e = dtype == SANIC_BF16 ? launch_pdl(paged_merge_kernel<64, true>, grid, block, 0, st, p) : launch_pdl(paged_merge_kernel<64, false>, grid, block, 0, st, p);
+}
+}  // namespace
+
+extern "C" {
+
+size_t sanic_attn_paged_workspace_bytes(sanic_ctx* ctx, const sanic_attn_paged_params* p) {
+    if (!ctx || !p || validate(ctx, p) != SANIC_OK) return 0;
+    return workspace_bytes(make_plan(ctx, p), p->head_dim);
+}
+
+int32_t sanic_attn_paged(sanic_ctx* ctx, const sanic_attn_paged_params* p, void* stream) {
+    if (!ctx || !p) return SANIC_ERR_INVALID;
+    int32_t rc = validate(ctx, p);
+    if (rc != SANIC_OK) return rc;
+    if (p->n_requests == 0 || p->n_tokens == 0) return SANIC_OK;
+    const Plan pl = make_plan(ctx, p);
+    SANIC_REQUIRE(ctx, p->workspace && ((uintptr_t)p->workspace % 16) == 0 && p->workspace_bytes >= workspace_bytes(pl, p->head_dim),
+                  "attn_paged: the workspace must be 16-byte aligned and of sanic_attn_paged_workspace_bytes()");
+    sanic_set_device(ctx);
+    Params q{};
+    q.q = p->q; q.out = p->out; q.lse = p->lse; q.k = p->k_pages; q.v = p->v_pages;
+    q.table = p->block_table; q.query_start = p->query_start; q.kv_lens = p->kv_lens;
+    q.q_token_stride = p->q_token_stride; q.q_head_stride = p->q_head_stride;
+    q.k_page_stride = p->k_page_stride; q.k_row_stride = p->k_row_stride; q.k_head_stride = p->k_head_stride;
+    q.v_page_stride = p->v_page_stride; q.v_row_stride = p->v_row_stride; q.v_head_stride = p->v_head_stride;
+    q.table_stride = p->table_stride;
+    q.n_requests = p->n_requests; q.n_tokens = p->n_tokens; q.q_heads = p->q_heads; q.kv_heads = p->kv_heads; q.group = p->q_heads / p->kv_heads;
+    q.page_size = p->page_size; q.n_pages = p->n_pages; q.max_pages = p->max_pages; q.window = p->window; q.scale = p->scale;
+    q.page_shift = -1;
+    for (int i = 0; i < 31; ++i) if ((1 << i) == p->page_size) q.page_shift = i;
+    q.rows = pl.rows;
+    q.block_tokens = pl.rows / q.group;
+    const size_t slots = 2 * (size_t)pl.ctas * pl.rows;
+    q.ws_o = (float*)p->workspace;
+    q.ws_ml = (float2*)(q.ws_o + slots * p->head_dim);
+    q.ws_merge = (int4*)(q.ws_ml + slots);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (pl.rows == 16) rc = launch_rows_any<1>(ctx, q, p->head_dim, p->dtype, pl.ctas, st);
+    else if (pl.rows == 32) rc = launch_rows_any<2>(ctx, q, p->head_dim, p->dtype, pl.ctas, st);
+    else rc = launch_rows_any<4>(ctx, q, p->head_dim, p->dtype, pl.ctas, st);
+    if (rc != SANIC_OK) return rc;
+    cudaError_t e = cudaSuccess;
+    launch_merge(q, p->head_dim, p->dtype, pl.ctas, 1, st, &e);
+    SANIC_CUDA_CHECK(ctx, e);
+    return SANIC_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,281 @@
+// The two bookkeeping operators of a paged cache: page tables and slots from request lengths, and the write of a step's keys
+// and values (with RoPE of q and k) into their slots.
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace {
+using namespace sanic;
+using namespace sanic::paged;
+
+// ── page_table_append ──
+// Two running sums over the requests (pages taken, tokens) place everything: page j of request b's taken ones is
+// free[F - 1 - (taken before b) - j], token i of b is row (tokens before b) + i. Up to 8000 requests fit one block's shared
+// memory, so every block takes the sums itself and then fills its own slice of the token rows, the table entries and the
+// per-request outputs: one launch, no hand-over between blocks, and the time of a decode step is the latency of two
+// dependent loads and a scan. Bytes only start to matter for the slots and positions of whole prompts (12 per token).
+constexpr int AT = 512;      // threads of a block
+
+struct AppendShared { int warp_pages[AT / 32], warp_tokens[AT / 32]; };
+
+__device__ __forceinline__ int held_of(const sanic_page_append_params& p, int b, int seq) {
+    const int h = p.held_pages ? p.held_pages[b] : (int)(((long long)seq + p.page_size - 1) / p.page_size);
+    return min(max(h, 0), p.max_pages);
+}
+
+__global__ void __launch_bounds__(AT) page_append_kernel(const sanic_page_append_params p, int* err) {
+    extern __shared__ int s_dyn[];
+    int* s_tok = s_dyn;                          // [n + 1] token rows before request b, clamped to n_tokens
+    int* s_pg = s_dyn + p.n_requests + 1;        // [n + 1] pages taken before request b
+    __shared__ AppendShared sh;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = p.n_requests;
+    griddep_wait();
+    griddep_launch();
+    const int free_n = min(max(*p.free_count, 0), p.free_capacity);
+    long long tok_carry = 0, pg_carry = 0;
+    bool bad = false;
+    if (tid == 0) { s_tok[0] = 0; s_pg[0] = 0; }
+    for (int b0 = 0; b0 < n; b0 += AT) {
+        const int b = b0 + tid;
+        int tok = 0, pg = 0;
+        if (b < n) {
+            const int seq = p.seq_lens[b], add = p.new_lens[b];
+            bad |= seq < 0 || add < 0;
+            tok = min(max(add, 0), p.n_tokens + 1);      // more than the token rows there are: reported below, and the sums stay small
+            const long long need = ((long long)max(seq, 0) + max(add, 0) + p.page_size - 1) / p.page_size;
+            bad |= need > p.max_pages;
+            pg = max(0, (int)min(need, (long long)p.max_pages) - held_of(p, b, max(seq, 0)));
+        }
+        int ct = tok, cp = pg;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, ct, o), y = __shfl_up_sync(0xffffffffu, cp, o);
+            if (lane >= o) { ct = (int)min((long long)ct + x, 1ll << 30); cp = (int)min((long long)cp + y, 1ll << 30); }
+        }
+        if (lane == 31) { sh.warp_tokens[warp] = ct; sh.warp_pages[warp] = cp; }
+        __syncthreads();
+        long long bt = tok_carry, bp = pg_carry, at = 0, ap = 0;
+        for (int w = 0; w < AT / 32; ++w) {
+            if (w < warp) { bt += sh.warp_tokens[w]; bp += sh.warp_pages[w]; }
+            at += sh.warp_tokens[w]; ap += sh.warp_pages[w];
+        }
+        if (b < n) {
+            s_tok[b + 1] = (int)min(bt + ct, (long long)p.n_tokens);
+            s_pg[b + 1] = (int)min(bp + cp, (long long)INT32_MAX);
+            bad |= bt + ct > p.n_tokens || bp + cp > free_n;
+        }
+        tok_carry += at; pg_carry += ap;
+        __syncthreads();
+    }
+    __syncthreads();
+
+    const int stride = gridDim.x * AT, first = blockIdx.x * AT + tid;
+    for (int b = first; b < n; b += stride) {
+        const int seq = max(p.seq_lens[b], 0), add = max(p.new_lens[b], 0), held = held_of(p, b, seq);
+        const int got = min(max(free_n - s_pg[b], 0), s_pg[b + 1] - s_pg[b]);
+        p.query_start[b + 1] = s_tok[b + 1];
+        p.kv_lens[b] = (int)min((long long)seq + add, (long long)INT32_MAX);
+        p.pages_out[b] = held + got;
+    }
+    if (first == 0) {
+        p.query_start[0] = 0;
+        *p.free_count_out = (int)max(0ll, (long long)free_n - pg_carry);
+    }
+    if (bad && blockIdx.x == 0 && err) atomicCAS(err, 0, STATUS_POOL);
+    // table entries: the taken pages of all requests, in order
+    const int taken = s_pg[n];
+    for (int r = first; r < taken; r += stride) {
+        int lo = 0, hi = n - 1;                  // the last request with s_pg[b] <= r
+        while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (s_pg[mid] <= r) lo = mid; else hi = mid - 1; }
+        const int col = held_of(p, lo, max(p.seq_lens[lo], 0)) + r - s_pg[lo];
+        p.block_table[(int64_t)lo * p.table_stride + col] = r < free_n ? p.free_pages[free_n - 1 - r] : -1;
+    }
+    // token rows
+    const int used = s_tok[n];
+    for (int t = first; t < p.n_tokens; t += stride) {
+        int pos = 0;
+        long long slot = -1;
+        if (t < used) {
+            int lo = 0, hi = n - 1;              // the last request with s_tok[b] <= t
+            while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (s_tok[mid] <= t) lo = mid; else hi = mid - 1; }
+            const int seq = max(p.seq_lens[lo], 0), held = held_of(p, lo, seq);
+            pos = seq + t - s_tok[lo];
+            const int idx = pos / p.page_size;
+            int page = -1;
+            if (idx < held) page = p.block_table[(int64_t)lo * p.table_stride + idx];      // entries of earlier steps: nobody writes them here
+            else if (idx < p.max_pages) {
+                const int r = s_pg[lo] + idx - held;
+                if (r < free_n) page = p.free_pages[free_n - 1 - r];
+            }
+            if (page >= 0) slot = (long long)page * p.page_size + pos - idx * p.page_size;
+        }
+        p.positions[t] = pos;
+        p.slots[t] = slot;
+    }
+}
+
+// ── paged_cache_write ──
+// Bytes: every source element read once, every rotated or copied one written once. A thread takes 8 neighbouring elements of
+// the first half of a head's row and their 8 partners of the second half (16-byte loads and stores on both sides); a row of
+// head_dim / 16 threads serves one head, and the grid runs over (token, head) with the heads of q, k and v side by side.
+template <typename T> __device__ __forceinline__ void load8(const void* base, int64_t at, float (&x)[8]);
+template <> __device__ __forceinline__ void load8<float>(const void* base, int64_t at, float (&x)[8]) {
+    const float4 a = *(const float4*)((const float*)base + at), b = *(const float4*)((const float*)base + at + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+struct Bf16 {};
+struct F16 {};
+template <> __device__ __forceinline__ void load8<Bf16>(const void* base, int64_t at, float (&x)[8]) {
+    const uint4 a = *(const uint4*)((const uint16_t*)base + at);
+    x[0] = bf16lo(a.x); x[1] = bf16hi(a.x); x[2] = bf16lo(a.y); x[3] = bf16hi(a.y);
+    x[4] = bf16lo(a.z); x[5] = bf16hi(a.z); x[6] = bf16lo(a.w); x[7] = bf16hi(a.w);
+}
+__device__ __forceinline__ float f16_to_f32(uint16_t h) { float f; asm("cvt.f32.f16 %0, %1;" : "=f"(f) : "h"(h)); return f; }
+template <> __device__ __forceinline__ void load8<F16>(const void* base, int64_t at, float (&x)[8]) {
+    const uint4 a = *(const uint4*)((const uint16_t*)base + at);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[2 * i] = f16_to_f32((uint16_t)(w[i] & 0xffffu)); x[2 * i + 1] = f16_to_f32((uint16_t)(w[i] >> 16)); }
+}
+template <bool BF16> __device__ __forceinline__ void store8(void* base, int64_t at, const float (&x)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (BF16) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+        else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
+    }
+    *(uint4*)((uint16_t*)base + at) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename S, bool BF16>
+__global__ void __launch_bounds__(256) paged_write_kernel(const sanic_paged_write_params p, int* err) {
+    const int per_head = p.head_dim / 16, heads = (p.q ? p.q_heads : 0) + 2 * p.kv_heads, half = p.head_dim / 2;
+    const long long total = (long long)p.n_tokens * heads * per_head;
+    griddep_wait();
+    griddep_launch();
+    const long long id = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (id >= total) return;
+    const int per_token = heads * per_head;
+    const int t = (int)(id / per_token), rem = (int)(id - (long long)t * per_token);
+    const int hh = rem / per_head, c = (rem - hh * per_head) * 8;
+    const int64_t slot = p.slots[t];
+    if (slot < 0) return;
+    const int nq = p.q ? p.q_heads : 0;
+    const bool is_q = hh < nq, is_k = !is_q && hh < nq + p.kv_heads;
+    const int pos = p.table ? p.positions[t] : 0;
+    if (slot >= (int64_t)p.n_pages * p.page_size || (p.table && (unsigned)pos >= (unsigned)p.n_positions)) {
+        if (rem == 0 && err) atomicCAS(err, 0, STATUS_WRITE);
+        return;
+    }
+    float a[8], b[8];
+    if (is_q) {
+        const int64_t at = t * p.q_stride + (int64_t)hh * p.head_dim + c;
+        load8<S>(p.q, at, a); load8<S>(p.q, at + half, b);
+    } else {
+        const int h = hh - nq - (is_k ? 0 : p.kv_heads);
+        const int64_t at = t * (is_k ? p.k_stride : p.v_stride) + (int64_t)h * p.head_dim + c;
+        load8<S>(is_k ? p.k : p.v, at, a); load8<S>(is_k ? p.k : p.v, at + half, b);
+    }
+    if (p.table && (is_q || is_k)) {
+        const float4* cs = (const float4*)(p.table + ((int64_t)pos * half + c) * 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 w = __ldg(cs + i);      // (cos, sin) of two neighbouring frequencies
+            const float x0 = a[2 * i], y0 = b[2 * i], x1 = a[2 * i + 1], y1 = b[2 * i + 1];
+            a[2 * i] = x0 * w.x - y0 * w.y; b[2 * i] = y0 * w.x + x0 * w.y;
+            a[2 * i + 1] = x1 * w.z - y1 * w.w; b[2 * i + 1] = y1 * w.z + x1 * w.w;
+        }
+    }
+    if (is_q) {
+        const int64_t at = t * p.q_out_stride + (int64_t)hh * p.head_dim + c;
+        store8<BF16>(p.q_out, at, a); store8<BF16>(p.q_out, at + half, b);
+        return;
+    }
+    const int64_t page = slot / p.page_size, row = slot - page * p.page_size;
+    const int h = hh - nq - (is_k ? 0 : p.kv_heads);
+    const int64_t at = is_k ? page * p.k_page_stride + row * p.k_row_stride + h * p.k_head_stride + c
+                            : page * p.v_page_stride + row * p.v_row_stride + h * p.v_head_stride + c;
+    store8<BF16>(is_k ? p.k_pages : p.v_pages, at, a); store8<BF16>(is_k ? p.k_pages : p.v_pages, at + half, b);
+}
+
+bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a && b && x < y + nb && y < x + na;
+}
+}  // namespace
+
+extern "C" {
+
+int32_t sanic_page_table_append(sanic_ctx* ctx, const sanic_page_append_params* p, void* stream) {
+    if (!ctx || !p) return SANIC_ERR_INVALID;
+    SANIC_REQUIRE(ctx, p->n_requests >= 0 && p->n_tokens >= 0 && p->free_capacity >= 0, "page_table_append: negative count");
+    SANIC_REQUIRE(ctx, p->n_requests <= MAX_REQUESTS, "page_table_append: at most 8000 requests per call");
+    SANIC_REQUIRE(ctx, p->n_tokens < (1 << 30), "page_table_append: too many token rows");
+    SANIC_REQUIRE(ctx, p->page_size > 0 && p->max_pages > 0, "page_table_append: empty pages or table rows");
+    SANIC_REQUIRE(ctx, p->free_count && p->query_start && p->free_count_out, "page_table_append: null scalar or query_start");
+    SANIC_REQUIRE(ctx, p->n_requests == 0 || (p->seq_lens && p->new_lens && p->block_table && p->kv_lens && p->pages_out),
+                  "page_table_append: null tensor");
+    SANIC_REQUIRE(ctx, p->n_tokens == 0 || (p->positions && p->slots), "page_table_append: null token rows");
+    SANIC_REQUIRE(ctx, p->free_capacity == 0 || p->free_pages, "page_table_append: null free list");
+    SANIC_REQUIRE(ctx, p->n_requests <= 1 || p->table_stride >= p->max_pages, "page_table_append: table rows overlap");
+    // every block reads the inputs while others write the outputs
+    const size_t nb = (size_t)p->n_requests * 4;
+    const struct { const void* ptr; size_t n; } in[] = {{p->seq_lens, nb}, {p->new_lens, nb}, {p->held_pages, nb}, {p->free_pages, (size_t)p->free_capacity * 4},
+                                                        {p->free_count, 4}, {p->block_table, p->n_requests ? ((size_t)(p->n_requests - 1) * p->table_stride + p->max_pages) * 4 : 0}},
+                   out[] = {{p->query_start, nb + 4}, {p->kv_lens, nb}, {p->pages_out, nb}, {p->free_count_out, 4}, {p->positions, (size_t)p->n_tokens * 4},
+                            {p->slots, (size_t)p->n_tokens * 8}};
+    for (const auto& o : out)
+        for (const auto& i : in) SANIC_REQUIRE(ctx, !overlaps(o.ptr, o.n, i.ptr, i.n), "page_table_append: an output overlaps an input");
+    for (int i = 0; i < 5; ++i)
+        SANIC_REQUIRE(ctx, !overlaps(in[5].ptr, in[5].n, in[i].ptr, in[i].n), "page_table_append: the table overlaps an input");
+    sanic_set_device(ctx);
+    const int smem = (2 * p->n_requests + 2) * 4;
+    if (smem > 48 * 1024) SANIC_CUDA_CHECK(ctx, cudaFuncSetAttribute(page_append_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    // a block's slice: about four token rows or requests per thread, at most two blocks per SM
+    const long long rows = std::max<long long>(p->n_tokens, p->n_requests);
+    const int blocks = (int)std::min<long long>(std::max<long long>(1, (rows + 4 * AT - 1) / (4 * AT)), 2 * ctx->sm_count);
+    SANIC_CUDA_CHECK(ctx, launch_pdl(page_append_kernel, dim3(blocks), dim3(AT), smem, (cudaStream_t)stream, *p, ctx->status_dev));
+    return SANIC_OK;
+}
+
+int32_t sanic_paged_cache_write(sanic_ctx* ctx, const sanic_paged_write_params* p, void* stream) {
+    if (!ctx || !p) return SANIC_ERR_INVALID;
+    SANIC_REQUIRE(ctx, p->n_tokens >= 0 && p->kv_heads > 0 && p->q_heads >= 0, "paged_cache_write: bad counts");
+    if (p->head_dim <= 0 || p->head_dim % 16 || p->head_dim > 256)
+        return sanic_fail(ctx, SANIC_ERR_UNSUPPORTED, "paged_cache_write: head_dim must be a multiple of 16, at most 256");
+    SANIC_REQUIRE(ctx, p->cache_dtype == SANIC_BF16 || p->cache_dtype == SANIC_F16, "paged_cache_write: the pages are bf16 or f16");
+    SANIC_REQUIRE(ctx, p->src_dtype == SANIC_F32 || p->src_dtype == p->cache_dtype, "paged_cache_write: the source is f32 or of the pages' type");
+    SANIC_REQUIRE(ctx, p->page_size > 0 && p->n_pages > 0, "paged_cache_write: empty page pool");
+    if (p->n_tokens == 0) return SANIC_OK;
+    SANIC_REQUIRE(ctx, p->k && p->v && p->k_pages && p->v_pages && p->slots, "paged_cache_write: null tensor");
+    SANIC_REQUIRE(ctx, !p->q == !p->q_out && (!p->q || p->q_heads > 0), "paged_cache_write: q and q_out go together");
+    SANIC_REQUIRE(ctx, !p->table || (p->positions && p->n_positions > 0), "paged_cache_write: a table needs positions");
+    const int src = p->src_dtype == SANIC_F32 ? 4 : 2;
+    // 16-byte accesses on every side
+    auto aligned = [](const void* ptr, int64_t stride, int bytes) { return ((uintptr_t)ptr % 16) == 0 && (stride * bytes) % 16 == 0 && stride >= 0; };
+    SANIC_REQUIRE(ctx, aligned(p->q, p->q ? p->q_stride : 0, src) && aligned(p->k, p->k_stride, src) && aligned(p->v, p->v_stride, src) &&
+                  aligned(p->q_out, p->q ? p->q_out_stride : 0, 2) && aligned(p->table, 0, 4) &&
+                  aligned(p->k_pages, p->k_page_stride, 2) && aligned(p->v_pages, p->v_page_stride, 2) &&
+                  p->k_row_stride % 8 == 0 && p->k_head_stride % 8 == 0 && p->v_row_stride % 8 == 0 && p->v_head_stride % 8 == 0 &&
+                  p->k_row_stride >= 0 && p->k_head_stride >= 0 && p->v_row_stride >= 0 && p->v_head_stride >= 0,
+                  "paged_cache_write: rows must be 16-byte aligned");
+    SANIC_REQUIRE(ctx, !p->q || p->q_out_stride >= (int64_t)p->q_heads * p->head_dim || p->n_tokens == 1, "paged_cache_write: q_out rows overlap");
+    SANIC_REQUIRE(ctx, p->q != p->q_out || !p->q || (src == 2 && p->q_stride == p->q_out_stride), "paged_cache_write: in place needs one type and one stride");
+    sanic_set_device(ctx);
+    const long long threads = (long long)p->n_tokens * ((p->q ? p->q_heads : 0) + 2 * p->kv_heads) * (p->head_dim / 16);
+    const long long blocks = (threads + 255) / 256;
+    SANIC_REQUIRE(ctx, blocks < (1ll << 31), "paged_cache_write: too many rows");
+    const dim3 grid((unsigned)blocks), block(256);
+    cudaStream_t st = (cudaStream_t)stream;
+    cudaError_t e;
+    if (p->cache_dtype == SANIC_BF16)
+        e = src == 4 ? launch_pdl(paged_write_kernel<float, true>, grid, block, 0, st, *p, ctx->status_dev)
+                     : launch_pdl(paged_write_kernel<Bf16, true>, grid, block, 0, st, *p, ctx->status_dev);
+    else
+        e = src == 4 ? launch_pdl(paged_write_kernel<float, false>, grid, block, 0, st, *p, ctx->status_dev)
+                     : launch_pdl(paged_write_kernel<F16, false>, grid, block, 0, st, *p, ctx->status_dev);
+    SANIC_CUDA_CHECK(ctx, e);
+    return SANIC_OK;
+}
+
+}  // extern "C"

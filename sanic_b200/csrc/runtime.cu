@@ -111,6 +111,15 @@ int32_t sanic_sync(sanic_ctx* ctx, void* stream) {
         if (code == 52)
             return sanic_fail(ctx, SANIC_ERR_INVALID, "a device-side key length was outside [1, kv_cap] and was clamped: the decode "
                                                       "position ran past the cache extent (code 52)");
+        if (code == 53)
+            return sanic_fail(ctx, SANIC_ERR_INVALID, "page_table_append: the free list, a table row or the token rows ran out, or a length "
+                                                      "was negative (code 53)");
+        if (code == 54)
+            return sanic_fail(ctx, SANIC_ERR_INVALID, "attn_paged: a table entry was outside the page pool, or a length past its extent (code 54)");
+        if (code == 55)
+            return sanic_fail(ctx, SANIC_ERR_INVALID, "draft_verify: a draft token, draft length or target row was out of range (code 55)");
+        if (code == 56)
+            return sanic_fail(ctx, SANIC_ERR_INVALID, "paged_cache_write: a slot or position was out of range (code 56)");
         return sanic_fail(ctx, SANIC_ERR_TIMEOUT, "a bounded device-side wait ran out (code " + std::to_string(code) + ")");
     }
     return SANIC_OK;

@@ -1,0 +1,794 @@
+"""The paged-cache serving operators against plain 64-bit implementations.
+
+Tolerances, from the arithmetic (u = eps / 2 of the storage type, the largest relative error of one rounding):
+  * attention: the output is rounded once (u |out|) and every weight once before the product with v (u A with
+    A = sum_j w_j |v_j|); scores are f32 sums of D products, |error| <= D 2^-24 sum |q k| scale <= 1e-4 for the inputs here
+    (D <= 128, unit-normal k, q of deviation 1.5: sum |q k| scale stays below 14), which moves a weight by at most that share on
+    each side of the quotient, 2e-4 A; f32 sums over at most a few hundred steps stay below 3e-5. So
+    |got - want| <= u |want| + (u + 2.5e-4) A.
+  * log-sum-exp: 1e-4 from the scores, 3e-5 from the sum and 2^-22 from the exponentials: 1.5e-4 absolute.
+  * RoPE: three f32 roundings of terms bounded by |a| + |b| (cos, sin <= 1), then one to storage: u |want| + 2^-22 (|a| + |b|),
+    plus the smallest subnormal step of f16 (2^-25).
+  * page tables, slots, positions, counts and tokens: exact.
+"""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "f16": torch.float16}
+
+
+@pytest.fixture(scope="module")
+def dev():
+    from sanic_b200 import CudaDevice
+    return CudaDevice(0)
+
+
+def ints(dev, xs, dtype=torch.int32):
+    return torch.tensor(xs, dtype=dtype, device=dev.torch_device)
+
+
+def gen(dev, seed):
+    g = torch.Generator(device=dev.torch_device)
+    g.manual_seed(seed)
+    return g
+
+
+# ───────────────────────── attention ─────────────────────────
+def make_problem(dev, new, ctx, hq, hkv, d, dtype, page, heads_first=False, window=0, seed=0, poison=True, extra_pages=3, table_pad=1):
+    """Ragged chunks `new` over caches of `ctx` held tokens. Every pool row that no token may see holds NaN."""
+    g = gen(dev, seed)
+    td = dev.torch_device
+    kv = [c + n for c, n in zip(ctx, new)]
+    need = [-(-x // page) for x in kv]
+    n_pages = sum(need) + extra_pages
+    order = torch.randperm(n_pages, generator=g, device=td)
+    shape = (n_pages, hkv, page, d) if heads_first else (n_pages, page, hkv, d)
+    pools = []
+    for _ in range(2):
+        x = torch.full(shape, float("nan") if poison else 3.0, device=td, dtype=DT[dtype])
+        pools.append(x.transpose(1, 2) if heads_first else x)
+    table = torch.full((len(new), max(need + [1]) + table_pad), n_pages + 77, dtype=torch.int32, device=td)   # entries past the need are never read
+    at = 0
+    keys, values = [], []
+    for b, (n, x) in enumerate(zip(need, kv)):
+        pages = order[at:at + n]
+        at += n
+        table[b, :n] = pages.to(torch.int32)
+        first = max(0, ctx[b] - window + 1) if window else 0
+        if n == 0:
+            keys.append(torch.zeros(0, hkv, d, device=td)); values.append(torch.zeros(0, hkv, d, device=td))
+            continue
+        k = torch.randn(x, hkv, d, generator=g, device=td).to(DT[dtype])
+        v = torch.randn(x, hkv, d, generator=g, device=td).to(DT[dtype])
+        keys.append(k); values.append(v)
+        if new[b]:
+            pos = torch.arange(first, x, device=td)
+            pools[0][pages[pos // page], pos % page] = k[first:]
+            pools[1][pages[pos // page], pos % page] = v[first:]
+    starts = np.concatenate([[0], np.cumsum(new)]).tolist()
+    q = (1.5 * torch.randn(starts[-1], hq, d, generator=g, device=td)).to(DT[dtype])
+    return dict(q=q, k_pages=pools[0], v_pages=pools[1], block_table=table, query_start=ints(dev, starts), kv_lens=ints(dev, kv)), keys, values
+
+
+def plain_attention(q, keys, values, new, kv, window, scale):
+    """f64; also A = sum_j w_j |v_j|."""
+    hq, d = q.shape[1:]
+    outs, bounds, lses = [], [], []
+    at = 0
+    for b, n in enumerate(new):
+        k, v = keys[b].double(), values[b].double()
+        group = hq // k.shape[1]
+        qb = q[at:at + n].double()
+        at += n
+        out = torch.zeros(n, hq, d, dtype=torch.float64, device=q.device)
+        amp = torch.zeros_like(out)
+        lse = torch.full((n, hq), -math.inf, dtype=torch.float64, device=q.device)
+        for i in range(n):
+            pos = kv[b] - n + i
+            lo = max(0, pos - window + 1) if window else 0
+            if pos < 0:
+                continue
+            kk, vv = (x[lo:pos + 1].repeat_interleave(group, 1) for x in (k, v))
+            s = torch.einsum("hd,jhd->hj", qb[i], kk) * scale
+            lse[i] = torch.logsumexp(s, 1)
+            w = torch.exp(s - lse[i][:, None])
+            out[i] = torch.einsum("hj,jhd->hd", w, vv)
+            amp[i] = torch.einsum("hj,jhd->hd", w, vv.abs())
+        outs.append(out); bounds.append(amp); lses.append(lse)
+    return torch.cat(outs), torch.cat(bounds), torch.cat(lses)
+
+
+def check_attention(got, lse, want, amp, want_lse):
+    u = torch.finfo(got.dtype).eps / 2
+    assert torch.isfinite(got).all()
+    err = (got.double() - want).abs()
+    over = err - (u * want.abs() + (u + 2.5e-4) * amp)
+    assert (over <= 0).all(), f"worst excess {over.max().item():.3e} at {np.unravel_index(int(over.argmax()), over.shape)}; err {err.max().item():.3e}"
+    empty = torch.isinf(want_lse)
+    assert torch.equal(torch.isinf(lse), empty) and (lse[empty] < 0).all()
+    assert ((lse.double() - want_lse)[~empty].abs() <= 1.5e-4).all(), (lse.double() - want_lse)[~empty].abs().max()
+
+
+def run_case(dev, new, ctx, hq, hkv, d, dtype, page, heads_first=False, window=0, seed=0, max_query_len=None, scale=None):
+    args, keys, values = make_problem(dev, new, ctx, hq, hkv, d, dtype, page, heads_first, window, seed)
+    got, lse = dev.attn_paged(**args, max_query_len=max(new) if max_query_len is None else max_query_len, window=window, scale=scale, return_lse=True)
+    dev.sync()
+    kv = [c + n for c, n in zip(ctx, new)]
+    check_attention(got, lse, *plain_attention(args["q"], keys, values, new, kv, window, scale if scale is not None else 1.0 / math.sqrt(d)))
+
+
+HEADS = [(4, 1), (8, 2), (3, 3), (7, 1), (10, 2), (16, 1)]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("page", [1, 16, 24, 64, 256])
+def test_attn_single_tokens(dev, d, dtype, page):
+    ctx = [0, 1, 14, 15, 16, 63, 64, 65, 127, 128, 200, 700]
+    hq, hkv = HEADS[(page + d) % len(HEADS)]
+    run_case(dev, [1] * len(ctx), ctx, hq, hkv, d, dtype, page, heads_first=page == 64, seed=page)
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (32, 8), (5, 1), (33, 1), (64, 1), (12, 4)])
+@pytest.mark.parametrize("window", [0, 1, 70])
+def test_attn_heads_and_windows(dev, hq, hkv, window):
+    run_case(dev, [1, 3, 2, 1], [90, 300, 0, 517], hq, hkv, 64, "bf16", 16, window=window, seed=hq + window)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("new,ctx", [([5, 3, 6, 1], [33, 250, 0, 100]), ([0, 4, 0, 0, 2, 0], [10, 70, 0, 5, 64, 9]), ([13], [129]), ([40, 1, 17], [3, 400, 0])])
+@pytest.mark.parametrize("window", [0, 37])
+def test_attn_short_chunks(dev, d, dtype, new, ctx, window):
+    run_case(dev, new, ctx, 8, 2, d, dtype, 16, window=window, seed=len(new))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("page,heads_first", [(8, False), (16, True), (24, False), (32, False), (128, True), (256, False)])
+def test_attn_long_chunks(dev, d, dtype, page, heads_first):
+    run_case(dev, [129, 1, 300, 65], [0, 500, 77, 640], 8, 2, d, dtype, page, heads_first=heads_first, seed=page)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hkv", [(2, 2), (7, 1), (12, 4), (64, 1), (33, 1)])
+@pytest.mark.parametrize("window", [0, 1, 100, 300])
+def test_attn_long_chunks_heads_and_windows(dev, d, hq, hkv, window):
+    run_case(dev, [257, 70, 1, 0, 128], [5, 600, 900, 40, 0], hq, hkv, d, "bf16", 16, window=window, seed=hq + window)
+
+
+@pytest.mark.parametrize("d,dtype", [(64, "bf16"), (128, "f16")])
+def test_attn_splits_a_long_cache(dev, d, dtype):
+    # few items over a long key axis: every CTA of the device holds a part, and the parts are merged
+    run_case(dev, [1], [40000], 8, 1, d, dtype, 64, seed=3)
+    run_case(dev, [2, 1], [20011, 9], 4, 2, d, dtype, 32, seed=4)
+    run_case(dev, [60], [12000], 8, 1, d, dtype, 64, seed=5)
+
+
+@pytest.mark.parametrize("maxq", [1, 300])
+def test_attn_chunk_longer_than_the_hint_and_more_tokens_than_keys(dev, maxq):
+    # the hint only selects a kernel; tokens before key 0 (a chunk longer than its keys) see nothing: zeros and -inf
+    args, keys, values = make_problem(dev, [90, 30, 7], [20, 0, 0], 8, 2, 64, "bf16", 16, seed=9)
+    args["kv_lens"] = ints(dev, [110, 12, 0])
+    got, lse = dev.attn_paged(**args, max_query_len=maxq, return_lse=True)
+    dev.sync()
+    check_attention(got, lse, *plain_attention(args["q"], [keys[0], keys[1][:12], keys[2][:0]], [values[0], values[1][:12], values[2][:0]],
+                                               [90, 30, 7], [110, 12, 0], 0, 0.125))
+    assert (got[90:108] == 0).all() and (got[120:] == 0).all() and torch.isinf(lse[120:]).all()
+
+
+@pytest.mark.parametrize("maxq", [4, 200])
+def test_attn_leaves_rows_outside_the_chunks_alone(dev, maxq):
+    args, keys, values = make_problem(dev, [3, 2], [40, 7], 4, 2, 64, "f16", 16, seed=2)
+    q = torch.full((11, 4, 64), float("nan"), dtype=torch.float16, device=dev.torch_device)
+    q[4:9] = args["q"]
+    args.update(q=q, query_start=args["query_start"] + 4)
+    out = torch.full((11, 4, 64), 5.0, dtype=torch.float16, device=dev.torch_device)
+    dev.attn_paged(**args, max_query_len=maxq, out=out)
+    dev.sync()
+    assert (out[:4] == 5.0).all() and (out[9:] == 5.0).all()
+    want, amp, _ = plain_attention(q[4:9], keys, values, [3, 2], [43, 9], 0, 0.125)
+    assert ((out[4:9].double() - want).abs() <= 2.0 ** -11 * want.abs() + (2.0 ** -11 + 2.5e-4) * amp).all()
+
+
+@pytest.mark.parametrize("maxq", [2, 100])
+def test_attn_strided_queries_and_a_view_of_the_pool(dev, maxq):
+    # q cut from a fused projection; pages that are every other page of a larger pool, keys and values interleaved in one tensor
+    args, keys, values = make_problem(dev, [2, 70], [100, 30], 8, 2, 128, "bf16", 16, seed=6)
+    T = args["q"].shape[0]
+    rows = torch.randn(T, 20, 128, device=dev.torch_device).to(torch.bfloat16)
+    rows[:, 3:11] = args["q"]
+    n = args["k_pages"].shape[0]
+    pool = torch.full((2 * n, 16, 2, 2, 128), float("nan"), dtype=torch.bfloat16, device=dev.torch_device)
+    pool[::2, :, 0], pool[::2, :, 1] = args["k_pages"], args["v_pages"]
+    args.update(q=rows[:, 3:11], k_pages=pool[::2, :, 0], v_pages=pool[::2, :, 1])
+    got, lse = dev.attn_paged(**args, max_query_len=maxq, return_lse=True)
+    dev.sync()
+    check_attention(got, lse, *plain_attention(args["q"], keys, values, [2, 70], [102, 100], 0, 128 ** -0.5))
+
+
+@pytest.mark.parametrize("maxq", [1, 64])
+def test_attn_pool_past_32_bit_offsets(dev, maxq):
+    # more than 2^31 elements of keys: the pages used are the last ones
+    page, hkv, d = 128, 8, 128
+    n_pages = (1 << 31) // (page * hkv * d) + 40
+    small, keys, values = make_problem(dev, [1, 33], [700, 100], 8, 8, d, "bf16", page, seed=8)
+    used = small["k_pages"].shape[0]
+    k = torch.zeros(n_pages, page, hkv, d, dtype=torch.bfloat16, device=dev.torch_device)
+    v = torch.zeros_like(k)
+    k[-used:], v[-used:] = small["k_pages"], small["v_pages"]
+    table = torch.where(small["block_table"] < used, small["block_table"] + (n_pages - used), n_pages + 5).to(torch.int32)
+    got, lse = dev.attn_paged(small["q"], k, v, table, small["query_start"], small["kv_lens"], max_query_len=maxq, return_lse=True)
+    dev.sync()
+    check_attention(got, lse, *plain_attention(small["q"], keys, values, [1, 33], [701, 133], 0, d ** -0.5))
+
+
+def test_attn_large_scores(dev):
+    # scores of some hundreds: the running maximum moves by more than any slack, weights underflow
+    args, keys, values = make_problem(dev, [1, 200], [300, 50], 4, 1, 64, "bf16", 16, seed=11)
+    for maxq in (1, 200):
+        got, lse = dev.attn_paged(**args, max_query_len=maxq, scale=20.0, return_lse=True)
+        dev.sync()
+        want, amp, wl = plain_attention(args["q"], keys, values, [1, 200], [301, 250], 0, 20.0)
+        # the f32 scores are now up to 160 times larger: |error| <= 1e-4 * 160 on each
+        err = (got.double() - want).abs()
+        assert (err <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 3.3e-2) * amp).all()
+        assert ((lse.double() - wl).abs() <= 2e-2).all()
+
+
+@pytest.mark.parametrize("maxq", [1, 64])
+def test_attn_bad_pages_and_lengths_are_reported(dev, maxq):
+    from sanic_b200 import RunError
+    args, keys, values = make_problem(dev, [1, 40], [100, 30], 4, 2, 64, "bf16", 16, seed=12)
+    good = dev.attn_paged(**args, max_query_len=maxq)
+    dev.sync()
+    for entry in (-1, args["k_pages"].shape[0], 1 << 30):
+        bad = args["block_table"].clone()
+        bad[0, 2] = entry
+        got = dev.attn_paged(**dict(args, block_table=bad), max_query_len=maxq)
+        with pytest.raises(RunError, match="code 54"):
+            dev.sync()
+        assert torch.equal(got[1:], good[1:]) and torch.isfinite(got[0]).all()       # the other request is untouched; zeros are read instead
+    for name, val in (("kv_lens", [101, 1 << 30]), ("kv_lens", [-5, 70]), ("query_start", [0, 1, 500]), ("query_start", [-3, 1, 41])):
+        dev.attn_paged(**dict(args, **{name: ints(dev, val)}), max_query_len=maxq)
+        with pytest.raises(RunError, match="code 54"):
+            dev.sync()
+    assert torch.equal(dev.attn_paged(**args, max_query_len=maxq), good)
+    dev.sync()
+
+
+def test_attn_refusals(dev):
+    from sanic_b200 import CompileError, RunError
+    args, _, _ = make_problem(dev, [2], [20], 4, 2, 64, "bf16", 16)
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=dev.torch_device)
+    with pytest.raises(CompileError, match="head_dim"):
+        dev.attn_paged(z(2, 4, 96), z(3, 16, 2, 96), z(3, 16, 2, 96), args["block_table"], args["query_start"], args["kv_lens"])
+    with pytest.raises(RunError, match="multiple"):
+        dev.attn_paged(z(2, 3, 64), args["k_pages"], args["v_pages"], args["block_table"], args["query_start"], args["kv_lens"])
+    with pytest.raises(CompileError, match="64 query heads"):
+        dev.attn_paged(z(2, 130, 64), args["k_pages"], args["v_pages"], args["block_table"], args["query_start"], args["kv_lens"])
+    with pytest.raises(RunError, match="scale"):
+        dev.attn_paged(**args, scale=0.0)
+    with pytest.raises(RunError, match="window"):
+        dev.attn_paged(**args, window=-1)
+    with pytest.raises(RunError, match="16-byte"):
+        dev.attn_paged(**dict(args, q=z(2 * 4 * 64 + 1)[1:].view(2, 4, 64)))
+    with pytest.raises(RunError, match="not a tensor on"):
+        dev.attn_paged(**dict(args, q=args["q"].cpu()))
+    from sanic_b200 import abi
+    p = abi.AttnPagedParams()
+    assert dev.lib.sanic_attn_paged_workspace_bytes(dev.h, C.byref(p)) == 0
+
+
+def test_attn_nothing_to_do(dev):
+    args, _, _ = make_problem(dev, [0, 0], [20, 0], 4, 2, 64, "bf16", 16)
+    assert dev.attn_paged(**args).shape == (0, 4, 64)
+    args["q"] = torch.zeros(3, 4, 64, dtype=torch.bfloat16, device=dev.torch_device)
+    out = torch.full((3, 4, 64), 2.0, dtype=torch.bfloat16, device=dev.torch_device)
+    dev.attn_paged(**args, out=out)
+    dev.sync()
+    assert (out == 2.0).all()
+
+
+@pytest.mark.parametrize("maxq", [1, 200])
+def test_attn_is_deterministic_and_runs_on_other_streams(dev, maxq):
+    args, _, _ = make_problem(dev, [1, 200, 3], [3000, 10, 40], 8, 2, 128, "bf16", 16, seed=13)
+    first = dev.attn_paged(**args, max_query_len=maxq, return_lse=True)
+    dev.sync()
+    side = [torch.cuda.Stream() for _ in range(3)]
+    results = []
+    for i in range(12):
+        with torch.cuda.stream(side[i % 3]):
+            results.append(dev.attn_paged(**args, max_query_len=maxq, return_lse=True))
+    torch.cuda.synchronize()
+    for r in results:
+        assert torch.equal(r[0], first[0]) and torch.equal(r[1], first[1])
+
+
+@pytest.mark.parametrize("maxq", [1, 40])
+def test_attn_captured_twice_replays_side_by_side_over_new_lengths(dev, maxq):
+    sets = [make_problem(dev, [1, 40, 1], [900, 5, 60], 8, 2, 64, "f16", 16, seed=20 + i) for i in range(2)]
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    for args, _, _ in sets:
+        dev.attn_paged(**args, max_query_len=maxq)
+    torch.cuda.synchronize()
+    for i, (args, _, _) in enumerate(sets):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[i]):
+            outs.append(dev.attn_paged(**args, max_query_len=maxq, return_lse=True))
+        graphs.append(g)
+    for kv in ([901, 45, 61], [350, 45, 17], [1, 45, 61]):
+        for args, _, _ in sets:
+            args["kv_lens"].copy_(ints(dev, kv))
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for i in range(2):
+                with torch.cuda.stream(streams[i]):
+                    graphs[i].replay()
+        torch.cuda.synchronize()
+        for (args, keys, values), (got, lse) in zip(sets, outs):
+            check_attention(got, lse, *plain_attention(args["q"], [k[:n] for k, n in zip(keys, kv)], [v[:n] for v, n in zip(values, kv)],
+                                                       [1, 40, 1], kv, 0, 0.125))
+
+
+# ───────────────────────── page tables ─────────────────────────
+def plain_append(seq, new, held, table, free, count, page, n_tokens):
+    table = table.copy()
+    max_pages = table.shape[1]
+    start, kv, pages, pos, slots, bad = [0], [], [], [], [], False
+    left = count
+    for b, (s, n) in enumerate(zip(seq, new)):
+        s, n, h = max(s, 0), max(n, 0), held[b]
+        need = -(-(s + n) // page)
+        bad |= need > max_pages or seq[b] < 0 or new[b] < 0
+        got = h
+        for col in range(h, min(need, max_pages)):
+            if left > 0:
+                left -= 1
+                table[b, col] = free[left]
+                got += 1
+            else:
+                table[b, col] = -1
+                bad = True
+        pages.append(got)
+        kv.append(s + n)
+        for i in range(n):
+            if len(pos) >= n_tokens:
+                bad = True
+                break
+            p = s + i
+            e = table[b, p // page] if p // page < max_pages else -1
+            pos.append(p)
+            slots.append(-1 if e < 0 else int(e) * page + p % page)
+        start.append(len(pos))
+    rest = n_tokens - len(pos)
+    return table, start, kv, pages, left, pos + [0] * rest, slots + [-1] * rest, bad
+
+
+def check_append(dev, seq, new, page, max_pages, count, n_tokens, held=None, capacity=None, seed=0):
+    from sanic_b200 import RunError
+    r = np.random.default_rng(seed)
+    h = held if held is not None else [min(-(-max(s, 0) // page), max_pages) for s in seq]
+    ids = r.permutation(sum(h) + (capacity or count) + 5).astype(np.int32)
+    table = np.full((len(seq), max_pages), -7, np.int32)
+    at = 0
+    for b, n in enumerate(h):
+        table[b, :n] = ids[at:at + n]
+        at += n
+    free = ids[at:at + (capacity or count)]
+    want = plain_append(seq, new, h, table, free, count, page, n_tokens)
+    t = ints(dev, table.tolist()) if len(seq) else torch.zeros(0, max_pages, dtype=torch.int32, device=dev.torch_device)
+    got = dev.page_table_append(ints(dev, seq), ints(dev, new), t, ints(dev, free.tolist()), ints(dev, [count]), page, n_tokens,
+                                held_pages=None if held is None else ints(dev, held))
+    if want[-1]:
+        with pytest.raises(RunError, match="code 53"):
+            dev.sync()
+    else:
+        dev.sync()
+    assert t.cpu().numpy().tolist() == want[0].tolist()
+    for g, w in zip(got, (want[1], want[2], want[3], [want[4]], want[5], want[6])):
+        assert g.tolist() == list(w)
+    return t, got
+
+
+@pytest.mark.parametrize("page", [1, 16, 24, 256])
+@pytest.mark.parametrize("n", [1, 3, 300, 1100])
+def test_append_random(dev, page, n):
+    r = np.random.default_rng(page * 1000 + n)
+    seq = r.integers(0, 5 * page + 20, n)
+    new = r.integers(0, 3 * page + 3, n) * (r.random(n) < 0.7)
+    seq[r.random(n) < 0.2] = 0
+    need = sum(-(-int(s + x) // page) - -(-int(s) // page) for s, x in zip(seq, new))
+    check_append(dev, seq.tolist(), new.tolist(), page, 9 + 24 // page + (20 if page == 1 else 0), need + 5, int(new.sum()) + 13, seed=n)
+
+
+def test_append_edges(dev):
+    check_append(dev, [], [], 16, 4, 3, 0)                                       # no requests at all
+    check_append(dev, [], [], 16, 4, 3, 5)
+    check_append(dev, [0, 0, 0], [0, 0, 0], 16, 4, 0, 4, capacity=0 or 2)         # nothing appended: every row is padding
+    check_append(dev, [15, 16, 17], [1, 1, 1], 16, 4, 1, 3)                       # the last row of a page, the first of a new one, inside one
+    check_append(dev, [31, 5], [1, 4], 16, 6, 4, 5, held=[4, 3])                  # more pages held than the tokens need: a rolled-back draft keeps them
+    check_append(dev, [20], [60], 16, 5, 3, 60, held=[2])
+    check_append(dev, [8000 * 16 - 3], [5], 16, 8001, 4, 5)
+
+
+def test_append_shortages_are_reported(dev):
+    check_append(dev, [16, 30, 0], [40, 10, 33], 16, 6, 4, 83)                    # the free list ends inside the last request
+    check_append(dev, [16, 30], [40, 10], 16, 6, 0, 50, capacity=3)               # an empty one
+    check_append(dev, [60, 10], [30, 3], 16, 4, 8, 33)                            # a table row too short
+    check_append(dev, [3, 3, 3], [10, 10, 10], 16, 4, 8, 17)                      # more new tokens than token rows
+    check_append(dev, [-4, 9], [3, -2], 16, 4, 8, 6)                              # negative lengths read as 0
+    check_append(dev, [5], [2], 16, 4, 8, 2)                                      # and the next call is clean again
+
+
+def test_append_refusals(dev):
+    from sanic_b200 import RunError
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev.torch_device)
+    args = dict(seq_lens=z(2), new_lens=z(2), block_table=z(2, 4), free_pages=z(5), free_count=z(1), page_size=16, n_tokens=4)
+    with pytest.raises(RunError, match="empty pages"):
+        dev.page_table_append(**dict(args, page_size=0))
+    with pytest.raises(RunError, match="8000"):
+        dev.page_table_append(**dict(args, seq_lens=z(8001), new_lens=z(8001), block_table=z(8001, 4)))
+    t = z(12)
+    with pytest.raises(RunError, match="overlaps"):
+        dev.page_table_append(**dict(args, block_table=t[:8].view(2, 4), seq_lens=t[6:8]))
+
+
+# ───────────────────────── cache writes ─────────────────────────
+def check_write(dev, t, hq, hkv, d, src, cache, page, heads_first=False, fused=False, rope=True, with_q=True, in_place=False, seed=0):
+    g = gen(dev, seed)
+    td = dev.torch_device
+    S = torch.float32 if src == "f32" else DT[src]
+    n_pages = -(-t // page) + 2
+    rows = torch.randn(t, hq + 2 * hkv, d, generator=g, device=td).to(S)
+    q, k, v = rows.split([hq, hkv, hkv], 1)
+    if not fused:
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    q0, k0, v0 = q.clone(), k.clone(), v.clone()
+    shape = (n_pages, hkv, page, d) if heads_first else (n_pages, page, hkv, d)
+    kp, vp = (torch.randn(shape, generator=g, device=td).to(DT[cache]) for _ in range(2))
+    if heads_first:
+        kp, vp = kp.transpose(1, 2), vp.transpose(1, 2)
+    kp0, vp0 = kp.clone(), vp.clone()
+    slots = torch.randperm(n_pages * page, generator=g, device=td)[:t]
+    skip = torch.rand(t, generator=g, device=td) < 0.2
+    slots[skip] = -1
+    table = dev.rope_table([500000.0 ** (-i / (d // 2)) for i in range(d // 2)], 97)
+    pos = torch.randint(0, 97, (t,), generator=g, device=td, dtype=torch.int32)
+    out = q if in_place else torch.full((t, hq, d), 9.0, dtype=DT[cache], device=td)
+    got = dev.paged_cache_write(k, v, kp, vp, slots, q=q if with_q else None, positions=pos if rope else None,
+                                rope_table=table if rope else None, q_out=out if with_q else None)
+    dev.sync()
+    cs = table.double()[pos.long()][:, None]
+    u, tiny = torch.finfo(DT[cache]).eps / 2, 2.0 ** -25
+
+    def want(x):
+        a, b = x.double().chunk(2, -1)
+        if not rope:
+            return x.double(), torch.zeros_like(x, dtype=torch.float64)
+        w = torch.cat([a * cs[..., 0] - b * cs[..., 1], b * cs[..., 0] + a * cs[..., 1]], -1)
+        return w, (a.abs() + b.abs()).repeat(1, 1, 2)
+
+    def close(x, w, size):
+        return ((x.double() - w).abs() <= u * w.abs() + 2.0 ** -22 * size + tiny).all()
+
+    keep = ~skip
+    pg, row = slots // page, slots % page
+    wk, sk = want(k0)
+    assert close(kp[pg[keep], row[keep]], wk[keep], sk[keep])
+    assert torch.equal(vp[pg[keep], row[keep]], v0[keep].to(DT[cache]))
+    touched = torch.zeros(n_pages * page, dtype=torch.bool, device=td)
+    touched[slots[keep]] = True
+    left = ~touched.view(n_pages, page)
+    assert torch.equal(kp[left], kp0[left]) and torch.equal(vp[left], vp0[left])
+    if with_q:
+        assert got.data_ptr() == out.data_ptr()
+        wq, sq = want(q0)
+        assert close(got[keep], wq[keep], sq[keep])
+        assert torch.equal(got[skip], q0[skip] if in_place else torch.full_like(got[skip], 9.0))
+    else:
+        assert got is None
+
+
+@pytest.mark.parametrize("d", [16, 64, 128, 256])
+@pytest.mark.parametrize("src,cache", [("bf16", "bf16"), ("f16", "f16"), ("f32", "bf16"), ("f32", "f16")])
+@pytest.mark.parametrize("t", [1, 7, 300])
+def test_write(dev, d, src, cache, t):
+    check_write(dev, t, 5, 2, d, src, cache, 16, heads_first=t == 7, fused=d == 64, seed=t + d)
+
+
+def test_write_forms(dev):
+    check_write(dev, 33, 4, 4, 64, "bf16", "bf16", 1)
+    check_write(dev, 33, 4, 1, 128, "f16", "f16", 24, rope=False)
+    check_write(dev, 33, 4, 2, 128, "f32", "f16", 64, with_q=False)
+    check_write(dev, 33, 4, 2, 128, "bf16", "bf16", 64, in_place=True)
+    check_write(dev, 33, 4, 2, 64, "bf16", "bf16", 16, in_place=True, fused=True)
+    check_write(dev, 2500, 32, 8, 64, "bf16", "bf16", 16)
+
+
+def test_write_out_of_range_is_reported_and_skipped(dev):
+    from sanic_b200 import RunError
+    td = dev.torch_device
+    k = torch.ones(3, 2, 64, dtype=torch.bfloat16, device=td)
+    kp, vp = (torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16, device=td) for _ in range(2))
+    table = dev.rope_table([1.0] * 32, 10)
+    for slots, pos in (([0, 64, 1], [0, 1, 2]), ([0, 1 << 40, 1], [0, 1, 2]), ([0, 5, 1], [0, 10, 2]), ([0, 5, 1], [0, -1, 2])):
+        kp.zero_(); vp.zero_()
+        dev.paged_cache_write(k, k, kp, vp, ints(dev, slots, torch.int64), positions=ints(dev, pos), rope_table=table)
+        with pytest.raises(RunError, match="code 56"):
+            dev.sync()
+        assert (vp.flatten(0, 1)[[0, 1]] == 1).all() and vp.sum() == 2 * 128
+
+
+def test_write_refusals(dev):
+    from sanic_b200 import CompileError, RunError
+    td = dev.torch_device
+    z = lambda *s, t=torch.bfloat16: torch.zeros(*s, dtype=t, device=td)
+    slots = z(2, t=torch.int64)
+    with pytest.raises(CompileError, match="head_dim"):
+        dev.paged_cache_write(z(2, 1, 24), z(2, 1, 24), z(3, 16, 1, 24), z(3, 16, 1, 24), slots)
+    with pytest.raises(RunError, match="16-byte"):
+        dev.paged_cache_write(z(2 * 64 + 4)[4:].view(2, 1, 64), z(2, 1, 64), z(3, 16, 1, 64), z(3, 16, 1, 64), slots)
+    dev.paged_cache_write(z(0, 1, 64), z(0, 1, 64), z(3, 16, 1, 64), z(3, 16, 1, 64), z(0, t=torch.int64))
+
+
+# ───────────────────────── draft verification ─────────────────────────
+def plain_verify(target, tokens, ua, us, draft, lens, start):
+    n, k = tokens.shape
+    out, counts, margin = [], [], math.inf
+    for b in range(n):
+        row, c = [], 0
+        while c < lens[b]:
+            x = int(tokens[b, c])
+            p = float(target[start[b] + c, x])
+            q = 1.0 if draft is None else float(draft[b, c, x])
+            if not float(ua[b, c]) * q < p:
+                break
+            row.append(x)
+            c += 1
+        valid = lambda w: np.where(np.isfinite(w) & (w > 0), w, 0.0)      # NaN, infinite and non-positive weights count as 0
+        w = target[start[b] + c].astype(np.float64)
+        if c < lens[b]:
+            r = w.copy()
+            if draft is None:
+                r[int(tokens[b, c])] = 0.0
+            else:
+                r = w - draft[b, c].astype(np.float64)
+            if valid(r).any():
+                w = r
+        w = valid(w)
+        cum = np.cumsum(w)
+        if cum[-1] > 0:
+            x = float(us[b]) * cum[-1]
+            j = min(int(np.searchsorted(cum, x, side="right")), int(np.flatnonzero(w)[-1]))
+            margin = min(margin, np.min(np.abs(cum - x)) / cum[-1])
+            row.append(j)
+        else:
+            row.append(-1)
+        out.append(row + [-1] * (k + 1 - len(row)))
+        counts.append(c)
+    return out, counts, margin
+
+
+def check_verify(dev, n, k, vocab, probs=True, ragged=False, packed=False, seed=0, tweak=None):
+    r = np.random.default_rng(seed)
+    soft = lambda x: (np.exp(x) / np.exp(x).sum(-1, keepdims=True)).astype(np.float32)
+    lens = r.integers(0, k + 1, n).tolist() if ragged else [k] * n
+    if packed:
+        start = np.concatenate([[0], np.cumsum([x + 1 for x in lens])])
+        start, rows = start[:-1].tolist(), int(start[-1])
+    else:
+        start, rows = [b * (k + 1) for b in range(n)], n * (k + 1)
+    logits = r.normal(size=(rows, vocab)) * 2
+    target = soft(logits)
+    draft = np.zeros((n, k, vocab), np.float32)
+    tokens = np.zeros((n, k), np.int32)
+    for b in range(n):
+        for i in range(k):
+            draft[b, i] = soft(logits[min(start[b] + i, rows - 1)] + 0.8 * r.normal(size=vocab))
+            tokens[b, i] = r.choice(vocab, p=draft[b, i].astype(np.float64) / draft[b, i].astype(np.float64).sum())
+    ua, us = r.random((n, k)).astype(np.float32), r.random(n).astype(np.float32)
+    ua, us = np.minimum(ua, np.float32(1 - 2 ** -24)), np.minimum(us, np.float32(1 - 2 ** -24))
+    if tweak:
+        tweak(target, draft, tokens, ua, us)
+    want, counts, margin = plain_verify(target, tokens, ua, us, draft if probs else None, lens, start)
+    up = lambda a: torch.tensor(a, device=dev.torch_device)
+    got, acc = dev.draft_verify(up(target), up(tokens), up(ua), up(us), draft_probs=up(draft) if probs else None,
+                                draft_lens=ints(dev, lens) if ragged else None, target_start=ints(dev, start) if packed else None)
+    dev.sync()
+    assert acc.tolist() == counts
+    assert got.tolist() == want, (got.tolist(), want, margin)
+    return got, acc
+
+
+@pytest.mark.parametrize("probs", [True, False])
+@pytest.mark.parametrize("n,k,vocab", [(1, 4, 1), (1, 4, 2), (3, 1, 127), (5, 3, 129), (2, 8, 2048), (2, 5, 2049), (7, 2, 10007), (1, 6, 128256),
+                                       (40, 3, 5000), (300, 2, 333), (3, 0, 500), (2, 32, 700)])
+def test_verify(dev, n, k, vocab, probs):
+    check_verify(dev, n, k, vocab, probs, seed=n + k)
+    check_verify(dev, n, k, vocab, probs, ragged=True, packed=True, seed=n + k + 1)
+
+
+def test_verify_takes_every_branch_and_the_exact_borders(dev):
+    # dyadic probabilities: products and sums are exact, so borders are hit on the nose
+    def tweak(target, draft, tokens, ua, us):
+        target[:] = 0.0
+        target[:, 1], target[:, 3], target[:, 6] = 0.25, 0.5, 0.25
+        draft[:] = 0.0
+        draft[:, :, 3], draft[:, :, 5] = 0.5, 0.5
+        tokens[:] = 3
+        ua[:] = 0.5
+        us[:] = [0.0, 0.25, 0.75, np.float32(1 - 2 ** -24)] * 2
+        tokens[4:, 1] = 5                    # p = 0: rejected; left over: 1 and 6 at 0.25 each
+        tokens[7, 0], ua[7, 0] = 1, 0.0      # q = 0, u = 0: 0 < 0.25 holds
+    got, acc = check_verify(dev, 8, 2, 8, tweak=tweak)
+    assert acc.tolist() == [2, 2, 2, 2, 1, 1, 1, 1]
+    assert [row[c] for row, c in zip(got.tolist(), acc.tolist())] == [1, 3, 6, 6, 1, 1, 6, 6]
+
+    def equal(target, draft, tokens, ua, us):          # u q = p is a rejection; p - q leaves nothing: p itself is drawn from
+        target[:] = 1.0 / 8
+        draft[:] = 1.0 / 4
+        ua[:] = 0.5
+    check_verify(dev, 3, 2, 8, tweak=equal)
+
+
+def test_verify_odd_weights(dev):
+    def tweak(target, draft, tokens, ua, us):
+        target[:, 5] = np.nan
+        target[:, 7] = np.inf
+        target[:, 9] = -1.0
+        target[-1] = 0.0                               # nothing to draw from: -1
+        tokens[0, 0], tokens[1, 0] = 5, 9              # NaN and negative: rejected
+    got, acc = check_verify(dev, 4, 2, 600, probs=False, tweak=tweak)
+    assert acc.tolist()[:2] == [0, 0]
+    check_verify(dev, 4, 2, 600, tweak=tweak)
+
+
+def test_verify_unaligned_rows(dev):
+    r = np.random.default_rng(5)
+    flat = torch.rand(4 * 1003 + 1, device=dev.torch_device)
+    target = flat[1:].view(4, 1003)
+    tokens = ints(dev, r.integers(0, 1003, (1, 3)).tolist())
+    ua, us = torch.zeros(1, 3, device=dev.torch_device), torch.full((1,), 0.37, device=dev.torch_device)
+    got, acc = dev.draft_verify(target, tokens, ua, us)
+    dev.sync()
+    want, counts, _ = plain_verify(target.cpu().numpy(), tokens.cpu().numpy(), ua.cpu().numpy(), us.cpu().numpy(), None, [3], [0])
+    assert got.tolist() == want and acc.tolist() == counts
+
+
+def test_verify_out_of_range_is_reported(dev):
+    from sanic_b200 import CompileError, RunError
+    td = dev.torch_device
+    target = torch.full((6, 40), 1 / 40, device=td)
+    ua, us = torch.zeros(2, 2, device=td), torch.full((2,), 0.5, device=td)
+    ok = ints(dev, [[1, 2], [3, 4]])
+    for tokens in ([[1, 40], [3, 4]], [[1, -1], [3, 4]]):
+        got, acc = dev.draft_verify(target, ints(dev, tokens), ua, us)
+        with pytest.raises(RunError, match="code 55"):
+            dev.sync()
+        assert acc.tolist() == [1, 2] and got[0].tolist() == [1, 20, -1] and got[1, :2].tolist() == [3, 4]
+    got, acc = dev.draft_verify(target, ok, ua, us, draft_lens=ints(dev, [7, -2]))
+    with pytest.raises(RunError, match="code 55"):
+        dev.sync()
+    assert acc.tolist() == [2, 0]
+    for start in ([0, 4], [-1, 3]):
+        got, acc = dev.draft_verify(target, ok, ua, us, target_start=ints(dev, start))
+        with pytest.raises(RunError, match="code 55"):
+            dev.sync()
+        bad = 1 if start[0] == 0 else 0
+        assert acc[bad] == 0 and got[bad].tolist() == [-1, -1, -1] and acc[1 - bad] == 2
+    with pytest.raises(CompileError, match="32 drafted"):
+        dev.draft_verify(torch.zeros(34, 8, device=td), torch.zeros(1, 33, dtype=torch.int32, device=td), torch.zeros(1, 33, device=td), us[:1])
+    got, acc = dev.draft_verify(target, ok, ua, us)
+    dev.sync()
+    assert acc.tolist() == [2, 2]
+
+
+# ───────────────────────── the operators together ─────────────────────────
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_speculative_serving_loop(dev, captured):
+    """Admission of prompts, then steps of up to three drafted tokens per request with rejections, over one page pool: lengths
+    go from verification straight into the next step's page tables, on the device. Checked each step against plain attention
+    over caches kept contiguously on the side, and the table against every other request's pages."""
+    td = dev.torch_device
+    n, hq, hkv, d, page, vocab, K = 5, 8, 2, 64, 16, 200, 3
+    g = gen(dev, 77)
+    dt = torch.bfloat16
+    emb = {x: torch.randn(vocab, h, d, generator=g, device=td).to(dt) for x, h in (("q", hq), ("k", hkv), ("v", hkv))}
+    head = torch.randn(hq * d, vocab, generator=g, device=td) * 0.3
+    n_pages = 60
+    kp, vp = (torch.full((n_pages, page, hkv, d), float("nan"), dtype=dt, device=td) for _ in range(2))
+    table = torch.full((n, 12), -1, dtype=torch.int32, device=td)
+    free = torch.randperm(n_pages, generator=g, device=td).to(torch.int32)
+    rope = dev.rope_table([10000.0 ** (-i / (d // 2)) for i in range(d // 2)], 12 * page)
+    state = dict(seq=torch.zeros(n, dtype=torch.int32, device=td), held=torch.zeros(n, dtype=torch.int32, device=td), count=ints(dev, [n_pages]))
+    caches = [[torch.zeros(0, hkv, d, device=td) for _ in range(2)] for _ in range(n)]
+
+    def forward(tokens, new, n_tokens, maxq):
+        step = dev.page_table_append(state["seq"], new, table, free, state["count"], page, n_tokens, held_pages=state["held"])
+        q = dev.paged_cache_write(emb["k"][tokens], emb["v"][tokens], kp, vp, step.slots, q=emb["q"][tokens], positions=step.positions, rope_table=rope)
+        return step, q, *dev.attn_paged(q, kp, vp, table, step.query_start, step.kv_lens, max_query_len=maxq, return_lse=True)
+
+    def check(step, tokens, new, seq, q, out, lse):
+        starts = step.query_start.tolist()
+        for b in range(n):
+            t = tokens[starts[b]:starts[b + 1]]
+            cs = rope.double()[step.positions[starts[b]:starts[b + 1]].long()][:, None]
+            a, c = emb["k"][t].double().chunk(2, -1)
+            turned = torch.cat([a * cs[..., 0] - c * cs[..., 1], c * cs[..., 0] + a * cs[..., 1]], -1)
+            # the written keys are within one rounding of these; the kernel's own values go on
+            mine = kp[step.slots[starts[b]:starts[b + 1]] // page, step.slots[starts[b]:starts[b + 1]] % page]
+            assert ((mine.double() - turned).abs() <= 2.0 ** -8 * turned.abs() + 2.0 ** -19).all()
+            caches[b][0] = torch.cat([caches[b][0][:seq[b]], mine.float()])
+            caches[b][1] = torch.cat([caches[b][1][:seq[b]], emb["v"][t].float()])
+        total = starts[-1]
+        want, amp, wl = plain_attention(q[:total], [c[0] for c in caches], [c[1] for c in caches], new, step.kv_lens.tolist(), 0, d ** -0.5)
+        check_attention(out[:total], lse[:total], want, amp, wl)
+        owned = [table[b, :h].tolist() for b, h in enumerate(step.held_pages.tolist())]
+        flat = sum(owned, []) + free[:int(step.free_count)].tolist()
+        assert sorted(flat) == list(range(n_pages))          # every page in one place
+
+    prompt = [30, 1, 16, 47, 5]
+    tokens = torch.randint(0, vocab, (sum(prompt),), generator=g, device=td)
+    step, q, out, lse = forward(tokens, ints(dev, prompt), sum(prompt), max(prompt))
+    dev.sync()
+    check(step, tokens, prompt, [0] * n, q, out, lse)
+    state = dict(seq=step.kv_lens.clone(), held=step.held_pages.clone(), count=step.free_count.clone())
+    last = torch.randint(0, vocab, (n,), generator=g, device=td)
+
+    # every step: the last kept token and up to K drafts of each request (request 3 stops drafting, request 1 pauses)
+    buf = dict(tokens=torch.zeros(n * (K + 1), dtype=torch.int64, device=td), new=torch.zeros(n, dtype=torch.int32, device=td),
+               draft=torch.zeros(n, K, dtype=torch.int32, device=td), lens=torch.zeros(n, dtype=torch.int32, device=td),
+               ua=torch.zeros(n, K, device=td), us=torch.zeros(n, device=td), dp=torch.full((n, K, vocab), 1.0 / vocab, device=td))
+
+    def whole():
+        step, q, out, lse = forward(buf["tokens"], buf["new"], n * (K + 1), K + 1)
+        probs = torch.softmax(torch.where(torch.isfinite(out), out, 0).float().flatten(1) @ head, -1)
+        kept, acc = dev.draft_verify(probs, buf["draft"], buf["ua"], buf["us"], draft_probs=buf["dp"], draft_lens=buf["lens"],
+                                     target_start=step.query_start[:n].contiguous())
+        return step, q, out, lse, probs, kept, acc
+
+    graph = None
+    accepted = 0
+    for it in range(12):
+        lens = [int(x) for x in torch.randint(0, K + 1, (n,), generator=g, device=td)]
+        lens[3] = 0
+        new = [x + 1 for x in lens]
+        drafts = torch.randint(0, vocab, (n, K), generator=g, device=td)
+        flat = torch.cat([torch.cat([last[b:b + 1], drafts[b, :lens[b]]]) for b in range(n)])
+        buf["tokens"].zero_(); buf["tokens"][:len(flat)] = flat
+        buf["new"].copy_(ints(dev, new)); buf["draft"].copy_(drafts); buf["lens"].copy_(ints(dev, lens))
+        buf["ua"].copy_(torch.rand(n, K, generator=g, device=td) * (0.02 if it % 2 else 1.0)); buf["us"].copy_(torch.rand(n, generator=g, device=td))
+        seq = state["seq"].tolist()
+        if captured:
+            if graph is None:
+                keep = {k: v.clone() for k, v in state.items()}
+                t0, k0, v0 = table.clone(), kp.clone(), vp.clone()
+                whole(); torch.cuda.synchronize()
+                table.copy_(t0); kp.copy_(k0); vp.copy_(v0)
+                for k in state: state[k].copy_(keep[k])
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    result = whole()
+            graph.replay()
+        else:
+            result = whole()
+        step, q, out, lse, probs, kept, acc = result
+        dev.sync()
+        check(step, buf["tokens"][:sum(new)], new, seq, q, out, lse)
+        want, counts, _ = plain_verify(probs.cpu().numpy(), buf["draft"].cpu().numpy(), buf["ua"].cpu().numpy(), buf["us"].cpu().numpy(),
+                                       buf["dp"].cpu().numpy(), lens, step.query_start.tolist()[:n])
+        assert acc.tolist() == counts and kept.tolist() == want
+        accepted += sum(counts)
+        # the next step's lengths: what was kept; pages taken for rejected drafts stay with their rows
+        state["seq"].copy_(state["seq"] + acc + 1)
+        state["held"].copy_(step.held_pages)
+        state["count"].copy_(step.free_count)
+        last = kept.gather(1, acc[:, None].long())[:, 0].long()
+    assert accepted > 0
