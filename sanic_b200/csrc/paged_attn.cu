@@ -382,6 +382,8 @@ Plan make_plan(const sanic_ctx* ctx, const sanic_attn_paged_params* p) {
     const int group = p->q_heads / p->kv_heads;
     const long long want = (long long)(p->max_query_len > 0 ? p->max_query_len : p->n_tokens) * group;
     Plan pl{};
+    pl.tc = want > 64 && tc_supported(p);
+    if (pl.tc) { pl.rows = TC_ROWS; pl.ctas = ctx->sm_count; return pl; }
     pl.rows = 16;
     while (pl.rows < 64 && pl.rows < want) pl.rows *= 2;
     pl.ctas = rows_ctas(ctx, p->head_dim);
@@ -456,18 +458,19 @@ int32_t sanic_attn_paged(sanic_ctx* ctx, const sanic_attn_paged_params* p, void*
     q.page_shift = -1;
     for (int i = 0; i < 31; ++i) if ((1 << i) == p->page_size) q.page_shift = i;
     q.rows = pl.rows;
-    q.block_tokens = pl.rows / q.group;
+    q.block_tokens = pl.tc ? 2 * (128 / q.group) : pl.rows / q.group;
     const size_t slots = 2 * (size_t)pl.ctas * pl.rows;
     q.ws_o = (float*)p->workspace;
     q.ws_ml = (float2*)(q.ws_o + slots * p->head_dim);
     q.ws_merge = (int4*)(q.ws_ml + slots);
     cudaStream_t st = (cudaStream_t)stream;
-    if (pl.rows == 16) rc = launch_rows_any<1>(ctx, q, p->head_dim, p->dtype, pl.ctas, st);
+    if (pl.tc) rc = tc_launch(ctx, q, p->head_dim, p->dtype, pl.ctas, st);
+    else if (pl.rows == 16) rc = launch_rows_any<1>(ctx, q, p->head_dim, p->dtype, pl.ctas, st);
     else if (pl.rows == 32) rc = launch_rows_any<2>(ctx, q, p->head_dim, p->dtype, pl.ctas, st);
     else rc = launch_rows_any<4>(ctx, q, p->head_dim, p->dtype, pl.ctas, st);
     if (rc != SANIC_OK) return rc;
     cudaError_t e = cudaSuccess;
-    launch_merge(q, p->head_dim, p->dtype, pl.ctas, 1, st, &e);
+    launch_merge(q, p->head_dim, p->dtype, pl.ctas, pl.tc ? 8 : 1, st, &e);
     SANIC_CUDA_CHECK(ctx, e);
     return SANIC_OK;
 }

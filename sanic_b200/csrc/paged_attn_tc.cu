@@ -1,0 +1,583 @@
+// Attention of ragged chunks over a paged cache, the form for many query rows per (request, kv head): S = Q K^T and O += P V are
+// tcgen05 MMAs with accumulators in tensor memory; Q, K and V arrive by TMA, keys and values one page at a time.
+//
+// An item (paged_sched.h) is up to 256 query rows of one (request, kv head): the heads of a group are packed next to their
+// token (row = token * group + head), so a chunk of 64 tokens of a 4-head group fills both 128-row tiles and reads its keys
+// once. The two tiles ping-pong on the tensor core: while one tile's softmax warpgroup turns S into P, the other tile's MMAs run.
+//   warp 0       producer: page ids of a 128-key tile one tile ahead (a lane per page), then one TMA box per page and 64
+//                columns; K and V tiles share one ring
+//   warps 1, 3   MMA issuers, one per query tile
+//   warp 2       tensor-memory allocator
+//   warps 4-7    softmax, correction and epilogue of tile 0, one thread per row;   warps 8-11 the same for tile 1
+// Tensor memory, 512 columns. head_dim 64: S0 S1 | P0 P1 | O0 O1 with P in columns of its own, so the next S is computed while
+// the exponentials of this one run. head_dim 128: S0 S1 | O0 O1, P over the S it came from: S(j+1) follows PV(j) in the
+// tensor core's own order, and the other tile's products fill the time in between.
+// Rows of V outside the keys the item sees (the tail of the last page, pages before the window) are zeroed in shared memory
+// before the product, since 0 times what a page holds there may be NaN; scores of such keys are replaced, not added to.
+// The rescale of O waits until a row's maximum has moved by more than 2^8 (f16: 2^4, since its weights are shifted up by 2^8
+// against subnormals and must stay below 65504); after the first tile of a segment the maximum is taken inside the first
+// half of the exponentials, which are redone in the rare case that it moved.
+//
+// Bound: 4 rows keys head_dim flop on the tensor pipe (8192 per clock and SM) against one exponential per score on the SFU (16
+// per clock and SM): equal at head_dim 128, SFU-bound at 64.
+#include <algorithm>
+
+#include "paged.cuh"
+#include "tc_common.cuh"
+
+namespace {
+using namespace sanic;
+using namespace sanic::tc;
+using namespace sanic::paged;
+
+constexpr int BM = 128, BN = 128, NTHREADS = 384;
+
+template <int D> struct Tc {
+    static constexpr bool ALIAS = D == 128;            // P shares S's columns
+    static constexpr int SLABS = D / 64, SLAB = BN * 128;      // 64-column slabs of 128-byte rows
+    static constexpr int TILE = BN * D * 2;
+    static constexpr int QBUF = D == 64 ? 2 : 1;       // query buffers across items
+    static constexpr int NS = D == 64 ? 10 : 5;        // ring slots, one K or V tile each
+    static constexpr int TM_S = 0, TM_P = ALIAS ? 0 : 256, P_STEP = ALIAS ? 128 : 64, TM_O = ALIAS ? 256 : 384;
+    static constexpr int DATA = (2 * QBUF + NS) * TILE;
+};
+template <int D> struct Shared {
+    uint64_t q_full[2], q_empty[2], full[Tc<D>::NS], empty[Tc<D>::NS];
+    uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], o_free[2];      // per query tile
+    uint32_t tmem_base;
+    volatile int abort_flag;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void ffma2(float& d0, float& d1, float a0, float a1, float b, float c) {
+    asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %4};\n\tmov.b64 rc, {%5, %5};\n\t"
+        "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b), "f"(c));
+}
+__device__ __forceinline__ void fadd2(float& d0, float& d1, float a0, float a1) {   // d += a
+    asm("{\n\t.reg .b64 ra, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rd, {%0, %1};\n\tadd.rn.f32x2 rd, rd, ra;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "+f"(d0), "+f"(d1) : "f"(a0), "f"(a1));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t pred;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
+    return pred != 0;
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(dst), "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                 ::"r"(dst), "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__host__ __device__ constexpr uint32_t idesc_of(int M, int N, bool b_mn_major, bool bf16) {     // f16 operands: format fields 0
+    return make_idesc(M, N, b_mn_major) & (bf16 ? ~0u : ~((1u << 7) | (1u << 10)));
+}
+
+struct TcArgs { int tile_tokens, box_rows, k_heads_inner, v_heads_inner; };
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(NTHREADS, 1)
+paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                const __grid_constant__ Params p, const TcArgs a, int* err) {
+    using C = Tc<D>;
+    constexpr float P_SHIFT = BF16 ? 0.0f : 8.0f, SLACK = BF16 ? 8.0f : 4.0f;
+    extern __shared__ unsigned char smem_dyn[];
+    const uint32_t raw = smem_u32(smem_dyn);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    unsigned char* aligned = smem_dyn + (base - raw);
+    const uint32_t q_addr = base, ring_addr = base + 2 * C::QBUF * C::TILE;
+    Shared<D>* sh = (Shared<D>*)(aligned + C::DATA);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) { mbar_init(&sh->q_full[i], 1); mbar_init(&sh->q_empty[i], 2); }
+        for (int s = 0; s < C::NS; ++s) { mbar_init(&sh->full[s], 1); mbar_init(&sh->empty[s], 2); }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&sh->s_full[t], 1); mbar_init(&sh->s_free[t], 4); mbar_init(&sh->p_full[t], 4);
+            mbar_init(&sh->pv_done[t], 1); mbar_init(&sh->o_free[t], 4);
+        }
+        sh->abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == 2) tmem_alloc(&sh->tmem_base, 512);
+    griddep_wait();          // lengths, table, q and pages come from earlier kernels of the step
+    griddep_launch();
+    long long* cum = (long long*)(aligned + 2 * C::QBUF * C::TILE);      // the prefix sums share the ring's memory
+    scan_costs<BN>(p, cum, err);
+    DeviceWalk<BN> walk{LoadReq{&p, nullptr}};
+    walk.init(p, cum, blockIdx.x, gridDim.x);
+    fence_async_smem();      // generic accesses to the ring end before TMA writes it
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = sh->tmem_base;
+    volatile int* abortp = &sh->abort_flag;
+    const int tile_rows = a.tile_tokens * p.group;
+    Seg s;
+
+    // Every role walks the same segments. The first warpgroup gives registers to the softmax warpgroups: 128 x 72 + 256 x 216 =
+    // the 64,512 the launch was given.
+    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+        int slot = 0; uint32_t phase = 1;
+        bool ok = true;
+        int n = 0;
+        const int boxes = BN / a.box_rows;
+        while (ok && walk.next(p, s)) {
+            if (s.je <= s.jb) continue;
+            const int32_t* row = p.table + (int64_t)s.b * p.table_stride;
+            const int block0 = s.rb * p.block_tokens;
+            const int tiles = min(p.block_tokens, s.r.qn - block0) > a.tile_tokens ? 2 : 1;
+            // a lane's page of key tile j: -1 where no visible key lies in its box, n_pages (read as zeros) for a bad entry
+            auto page_of = [&](int j) {
+                const int key = j * BN + lane * a.box_rows;
+                if (lane >= boxes || key >= s.hi || key + a.box_rows <= s.lo) return -1;
+                int page, in_page;
+                return locate(p, row, key, page, in_page, err) ? page : p.n_pages;
+            };
+            int page = page_of(s.jb);
+            for (int j = s.jb; j < s.je && ok; ++j) {
+                const int ahead = j + 1 < s.je ? page_of(j + 1) : -1;
+                const int key = j * BN + lane * a.box_rows;
+                const int in_page = p.page_shift >= 0 ? key & (p.page_size - 1) : key % p.page_size;
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, page >= 0)) * a.box_rows * 128 * C::SLABS;
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh->empty[slot], phase, abortp, err, 11));
+                    if (!ok) break;
+                    if (lane == 0) mbar_expect_tx(&sh->full[slot], bytes);
+                    __syncwarp();
+                    if (page >= 0) {
+                        const uint32_t dst = ring_addr + slot * C::TILE + lane * a.box_rows * 128;
+                        const bool inner = kv ? a.v_heads_inner : a.k_heads_inner;
+                        const int y = inner ? s.hk : in_page, z = inner ? in_page : s.hk;
+#pragma unroll
+                        for (int c = 0; c < C::SLABS; ++c)
+                            tma_load_4d(dst + c * C::SLAB, kv ? &map_v : &map_k, &sh->full[slot], c * 64, y, z, page);
+                    }
+                    if (++slot == C::NS) { slot = 0; phase ^= 1; }
+                }
+                if (ok && j == s.jb) {       // the query tiles, behind the first keys: those need not wait for the last item's last product
+                    const int qb = C::QBUF == 2 ? n & 1 : 0;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh->q_empty[qb], ((C::QBUF == 2 ? n >> 1 : n) & 1) ^ 1, abortp, err, 10));
+                    if (!ok) break;
+                    if (lane == 0) {
+                        mbar_expect_tx(&sh->q_full[qb], tiles * tile_rows * 128 * C::SLABS);
+                        for (int t = 0; t < tiles; ++t)
+                            for (int c = 0; c < C::SLABS; ++c)
+                                tma_load_3d(q_addr + (qb * 2 + t) * C::TILE + c * C::SLAB, &map_q, &sh->q_full[qb], c * 64, s.hk * p.group,
+                                            s.r.q0 + block0 + t * a.tile_tokens);
+                    }
+                    __syncwarp();
+                }
+                page = ahead;
+            }
+            ++n;
+        }
+    } else if (warp == 1 || warp == 3) {
+        const bool leader = elect_one();
+        const int t = __shfl_sync(0xffffffffu, warp == 3 ? 1 : 0, 0);
+        constexpr uint32_t idesc_qk = idesc_of(BM, BN, false, BF16), idesc_pv = idesc_of(BM, D, true, BF16);
+        bool ok = true;
+        int n = 0;
+        uint32_t u_base = 0;                 // ring position of the segment's first key tile
+        uint32_t n_qk = 0, n_pv = 0;         // QK / PV issues so far
+        uint32_t n_act = 0;                  // earlier segments in which this tile had rows
+        while (ok && walk.next(p, s)) {
+            if (s.je <= s.jb) continue;
+            const int block0 = s.rb * p.block_tokens;
+            const bool both = min(p.block_tokens, s.r.qn - block0) > a.tile_tokens;
+            const int qb = C::QBUF == 2 ? n & 1 : 0;
+            const uint32_t q_phase = (C::QBUF == 2 ? n >> 1 : n) & 1;
+            ++n;
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh->q_full[qb], q_phase, abortp, err, 12));
+            if (!ok) break;
+            fence_after();
+            if (t == 1 && !both) {
+                // No rows for this tile: everything goes back untouched, but in step with the producer, so that no barrier is
+                // ever asked for a phase more than one ahead of its own.
+                if (leader) mbar_arrive(&sh->q_empty[qb]);
+                for (int i = 0; i < 2 * (s.je - s.jb) && ok; ++i, ++u_base) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh->full[u_base % C::NS], (u_base / C::NS) & 1, abortp, err, 14));
+                    if (ok && leader) mbar_arrive(&sh->empty[u_base % C::NS]);
+                }
+                continue;
+            }
+            int jq = s.jb, jp = s.jb;        // next key tile whose QK / PV is to be issued
+            uint32_t idle = 0;
+            while (ok && jp < s.je) {
+                bool progressed = false;
+                if (jq < s.je) {
+                    const uint32_t u = u_base + 2 * (uint32_t)(jq - s.jb);
+                    const int slot = u % C::NS;
+                    const bool free_s = C::ALIAS ? jq == jp : n_qk == 0 || mbar_test(&sh->s_free[t], (n_qk - 1) & 1);
+                    if (__all_sync(0xffffffffu, free_s && mbar_test(&sh->full[slot], (u / C::NS) & 1))) {
+                        fence_after();
+                        const uint64_t ad = make_desc(q_addr + (qb * 2 + t) * C::TILE, 16, 1024);
+                        const uint64_t bd = make_desc(ring_addr + slot * C::TILE, 16, 1024);
+                        if (leader) {
+#pragma unroll
+                            for (int kk = 0; kk < D / 16; ++kk) {
+                                const uint32_t o = (kk >> 2) * (C::SLAB >> 4) + (kk & 3) * 2;
+                                umma_f16(tmem + C::TM_S + t * BN, ad + o, bd + o, idesc_qk, kk > 0 ? 1u : 0u);
+                            }
+                            umma_commit(&sh->s_full[t]);
+                            umma_commit(&sh->empty[slot]);
+                            if (jq + 1 == s.je) umma_commit(&sh->q_empty[qb]);
+                        }
+                        __syncwarp();
+                        ++jq; ++n_qk; progressed = true;
+                    }
+                }
+                if (jp < jq) {
+                    const uint32_t u = u_base + 2 * (uint32_t)(jp - s.jb) + 1;
+                    const int slot = u % C::NS;
+                    const bool first = jp == s.jb;
+                    // the first PV of a segment overwrites O: the epilogue of the tile's previous segment must have read it
+                    if (__all_sync(0xffffffffu, mbar_test(&sh->p_full[t], n_pv & 1) && mbar_test(&sh->full[slot], (u / C::NS) & 1) &&
+                                                 (!first || n_act == 0 || mbar_test(&sh->o_free[t], (n_act - 1) & 1)))) {
+                        const int za = max(0, s.lo - jp * BN), zb = min(BN, s.hi - jp * BN);
+                        if (za > 0 || zb < BN) {       // rows [0, za) and [zb, 128) of V hold nothing of the item's
+                            const int n_rows = za + BN - zb;
+                            for (int i = lane; i < n_rows * 8 * C::SLABS; i += 32) {
+                                const int r = i / (8 * C::SLABS), c = i % (8 * C::SLABS);
+                                const int rr = r < za ? r : zb + r - za;
+                                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(ring_addr + slot * C::TILE + (c >> 3) * C::SLAB + rr * 128 + (c & 7) * 16), "r"(0) : "memory");
+                            }
+                            fence_async_smem();
+                            __syncwarp();
+                        }
+                        fence_after();
+                        const uint64_t vd = make_desc(ring_addr + slot * C::TILE, C::SLAB, 1024);
+                        if (leader) {
+#pragma unroll
+                            for (int kk = 0; kk < BN / 16; ++kk)       // A = P from tensor memory: 16 keys = 8 columns per step
+                                umma_f16_ts(tmem + C::TM_O + t * D, tmem + C::TM_P + t * C::P_STEP + 8 * kk, vd + 128 * kk, idesc_pv,
+                                            (!first || kk > 0) ? 1u : 0u);
+                            if (!C::ALIAS || jp + 1 == s.je) umma_commit(&sh->pv_done[t]);
+                            umma_commit(&sh->empty[slot]);
+                        }
+                        __syncwarp();
+                        ++jp; ++n_pv; progressed = true;
+                    }
+                }
+                if (progressed) idle = 0;
+                else {
+                    __nanosleep(32);
+                    if (++idle > (SPIN_LIMIT >> 4) || ((idle & 1023u) == 0 && __any_sync(0xffffffffu, *abortp != 0))) {
+                        if (idle > (SPIN_LIMIT >> 4) && leader) { *abortp = 1; atomicCAS(err, 0, 13); }
+                        ok = false;
+                    }
+                }
+            }
+            u_base += 2 * (uint32_t)(s.je - s.jb);
+            ++n_act;
+        }
+    } else if (warp >= 4) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int t = (warp - 4) >> 2, q4 = warp & 3, row = q4 * 32 + lane;
+        const uint32_t lane_base = (uint32_t)(q4 * 32) << 16;
+        const uint32_t s_tmem = tmem + lane_base + C::TM_S + t * BN;
+        const uint32_t p_tmem = tmem + lane_base + C::TM_P + t * C::P_STEP;
+        const uint32_t o_tmem = tmem + lane_base + C::TM_O + t * D;
+        const float sl2 = p.scale * LOG2E;
+        const int row_tok = row / p.group, row_head = row - row_tok * p.group;
+        uint32_t n_it = 0, n_act = 0;        // key tiles folded, segments served by this tile so far
+        bool ok = true, scores_ready = false;
+        int4 merge = make_int4(0, 0, 0, 0);
+        while (ok && walk.next(p, s)) {
+            const int block0 = s.rb * p.block_tokens;
+            const int n_tok = min(p.block_tokens, s.r.qn - block0);
+            if (t == 0 && s.parts > 1) merge = make_int4(s.r.q0 + block0, n_tok, s.hk, s.parts);
+            const int tok = t * a.tile_tokens + row_tok;
+            const bool valid = row < tile_rows && tok < n_tok;
+            if (t == 1 && n_tok <= a.tile_tokens) continue;
+            const bool empty = s.je <= s.jb;
+            const int64_t at = ((int64_t)(s.r.q0 + block0 + tok)) * p.q_heads + s.hk * p.group + row_head;
+            float m = -INFINITY, l = 0.0f;
+            const int pos = s.r.kv - s.r.qn + block0 + tok;
+            const int khi = valid ? max(0, pos + 1) : 0, klo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+            // key tiles from inner_lo to inner_hi are seen whole by every row of the tile
+            const int tile_pos = s.r.kv - s.r.qn + block0 + t * a.tile_tokens;
+            const int inner_hi = tile_pos + 1;
+            const int inner_lo = p.window > 0 ? tile_pos + a.tile_tokens - p.window : 0;
+            const bool busy = __any_sync(0xffffffffu, valid);      // a warp without rows only keeps the barriers' count
+            for (int j = s.jb; j < s.je && ok; ++j, ++n_it) {
+                const bool first = j == s.jb;
+                if (!scores_ready) ok = mbar_wait_spin(&sh->s_full[t], n_it & 1, abortp, err, 21);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                scores_ready = false;
+                fence_after();
+                if (!busy) {
+                    fence_before();
+                    __syncwarp();
+                    if (!C::ALIAS) {
+                        if (lane == 0) mbar_arrive(&sh->s_free[t]);
+                        // P(j)'s arrival may not count for P(j - 1), which the other warps may still be writing: in step with them
+                        ok = __all_sync(0xffffffffu, n_it == 0 || mbar_wait(&sh->pv_done[t], (n_it - 1) & 1, abortp, err, 24));
+                        if (!ok) break;
+                    }
+                    if (lane == 0) mbar_arrive(&sh->p_full[t]);
+                    continue;
+                }
+                const int k0 = j * BN;
+                const bool edge = k0 + BN > inner_hi || k0 < inner_lo;
+                uint32_t r[BN];
+#pragma unroll
+                for (int c = 0; c < BN / 32; ++c) tmem_ld32_nowait(s_tmem + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
+                tmem_ld_wait();
+                if (!C::ALIAS) {
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh->s_free[t]);        // S is in registers
+                }
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < BN; ++i) { const int kk = k0 + i; if (!(kk >= klo && kk < khi)) r[i] = 0xFF800000u; }  // -inf
+                }
+                const bool spec = !first;
+                float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                float alpha = 1.0f;
+                bool need = false;
+                auto new_reference = [&]() {
+                    const float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
+                    const float m_cand = fmaxf(m, mx * sl2);
+                    need = valid && ((m_cand - m > SLACK) || (!(m > -INFINITY) && m_cand > -INFINITY));
+                    if (need) { alpha = (m > -INFINITY) ? ex2(m - m_cand) : 0.0f; m = m_cand; }
+                };
+                if (!spec) {
+#pragma unroll
+                    for (int i = 0; i < BN; i += 8) {
+                        mxs[0] = max3(mxs[0], __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+                        mxs[1] = max3(mxs[1], __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
+                        mxs[2] = max3(mxs[2], __uint_as_float(r[i + 4]), __uint_as_float(r[i + 5]));
+                        mxs[3] = max3(mxs[3], __uint_as_float(r[i + 6]), __uint_as_float(r[i + 7]));
+                    }
+                    new_reference();
+                }
+                float msub = ((m > -INFINITY) ? m : 0.0f) - P_SHIFT;
+                const bool pv_ready = !C::ALIAS && n_it > 0 && mbar_test(&sh->pv_done[t], (n_it - 1) & 1);
+                float sums[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                uint32_t pk[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    if (spec) {     // the row maximum of all 128 scores, four per step
+                        mxs[0] = max3(mxs[0], __uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]));
+                        mxs[1] = max3(mxs[1], __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
+                    }
+                    float x0, x1;
+                    ffma2(x0, x1, __uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), sl2, -msub);
+                    const float p0 = ex2(x0), p1 = ex2(x1);
+                    fadd2(sums[(2 * i) & 7], sums[(2 * i + 1) & 7], p0, p1);
+                    pk[i] = pack2<BF16>(p0, p1);
+                }
+                if (spec) {
+                    new_reference();
+                    if (__any_sync(0xffffffffu, need)) {       // some row's reference moved: the half is taken again
+                        msub = ((m > -INFINITY) ? m : 0.0f) - P_SHIFT;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) sums[i] = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            float x0, x1;
+                            ffma2(x0, x1, __uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), sl2, -msub);
+                            const float p0 = ex2(x0), p1 = ex2(x1);
+                            fadd2(sums[(2 * i) & 7], sums[(2 * i + 1) & 7], p0, p1);
+                            pk[i] = pack2<BF16>(p0, p1);
+                        }
+                    }
+                }
+                // Before P or O is written the previous PV of this tile must be done. With P over S it is: S(j) was computed
+                // behind it, and its commit covered both.
+                if (!C::ALIAS && n_it > 0) {
+                    if (!pv_ready) ok = mbar_wait_spin(&sh->pv_done[t], (n_it - 1) & 1, abortp, err, 22);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    fence_after();
+                }
+                if (!first && __any_sync(0xffffffffu, need)) {
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32(o_tmem + c * 32, o);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        tmem_st32(o_tmem + c * 32, o);
+                    }
+                }
+                tmem_st32(p_tmem, pk);
+                if (!C::ALIAS) scores_ready = (j + 1 < s.je) && mbar_test(&sh->s_full[t], (n_it + 1) & 1);
+#pragma unroll
+                for (int i = 32; i < 64; ++i) {
+                    float x0, x1;
+                    ffma2(x0, x1, __uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), sl2, -msub);
+                    const float p0 = ex2(x0), p1 = ex2(x1);
+                    fadd2(sums[(2 * i) & 7], sums[(2 * i + 1) & 7], p0, p1);
+                    r[i] = pack2<BF16>(p0, p1);
+                }
+                tmem_st32(p_tmem + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+                l = l * alpha + (((sums[0] + sums[1]) + (sums[2] + sums[3])) + ((sums[4] + sums[5]) + (sums[6] + sums[7])));
+                tmem_st_wait();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->p_full[t]);
+            }
+            if (!ok) break;
+            uint32_t o[D];
+            if (!empty) {
+                ok = __all_sync(0xffffffffu, mbar_wait_spin(&sh->pv_done[t], ((C::ALIAS ? n_act : n_it - 1)) & 1, abortp, err, 23));
+                if (!ok) break;
+                ++n_act;
+                fence_after();
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) tmem_ld32_nowait(o_tmem + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&o[c * 32]));
+                tmem_ld_wait();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->o_free[t]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < D; ++i) o[i] = 0u;
+            }
+            if (!valid) continue;
+            if (s.starts && s.finishes) {
+                const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;      // no visible key: zeros, and -inf for the log-sum-exp
+                uint16_t* dst = (uint16_t*)p.out + at * D;
+                if (!(l != 0.0f)) {
+#pragma unroll
+                    for (int i = 0; i < D; ++i) o[i] = 0u;                   // every weight of the row was 0: V's zero rows and NaN alike
+                }
+#pragma unroll
+                for (int q = 0; q < D / 8; ++q) {
+                    uint32_t wv[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        wv[j] = pack2<BF16>(__uint_as_float(o[8 * q + 2 * j]) * inv, __uint_as_float(o[8 * q + 2 * j + 1]) * inv);
+                    *(uint4*)(dst + q * 8) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
+                }
+                if (p.lse) p.lse[at] = (m + log2f(l) - P_SHIFT) * LN2;
+            } else {
+                const size_t r = (size_t)partial_slot(s, blockIdx.x) * p.rows + t * tile_rows + row;
+                float4* dst = (float4*)(p.ws_o + r * D);
+#pragma unroll
+                for (int q = 0; q < D / 4; ++q)
+                    dst[q] = make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]), __uint_as_float(o[4 * q + 2]), __uint_as_float(o[4 * q + 3]));
+                p.ws_ml[r] = make_float2(m, l);
+            }
+        }
+        if (warp == 4 && lane == 0) p.ws_merge[blockIdx.x] = merge;
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 2) { fence_after(); tmem_dealloc(tmem, 512); }
+}
+
+// Row-major view of rank 3 or 4, 128-byte swizzle, zero fill out of bounds; strides in elements of 2 bytes, dims innermost first.
+int32_t encode(sanic_ctx* ctx, CUtensorMap* map, bool bf16, const void* ptr, int rank, const cuuint64_t* dims, const int64_t* strides,
+               const cuuint32_t* box) {
+    if (!ctx->encode_tiled) {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
+        if (e != cudaSuccess || !fn) return sanic_fail(ctx, SANIC_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+        ctx->encode_tiled = fn;
+    }
+    cuuint64_t st[3];
+    for (int i = 0; i + 1 < rank; ++i) st[i] = (cuuint64_t)strides[i] * 2;
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    const CUresult r = ((encode_tiled_fn)ctx->encode_tiled)(
+        map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank, const_cast<void*>(ptr), dims, st, box, ones,
+        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return sanic_fail(ctx, SANIC_ERR_CUDA, "attn_paged: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+    return SANIC_OK;
+}
+
+// Strides of a pool as the tensor map wants them: (heads, rows) ordered by stride, every stride a multiple of the one before.
+struct Pool { int64_t inner, outer; bool heads_inner; };
+bool pool_of(int64_t page, int64_t row, int64_t head, int n_pages, int page_size, int heads, int d, Pool* out) {
+    if (heads == 1) head = d;              // a single head's stride is never used
+    if (page_size == 1) row = d;
+    const bool hi = head <= row;
+    const int64_t in = hi ? head : row, o = hi ? row : head;
+    if (n_pages == 1) page = o * (hi ? page_size : heads);
+    *out = Pool{in, o, hi};
+    return in >= d && o % in == 0 && page % o == 0 && page >= o && page < (1ll << 38);
+}
+
+template <int D, bool BF16>
+int32_t launch(sanic_ctx* ctx, const Params& p, int ctas, cudaStream_t st) {
+    using C = Tc<D>;
+    TcArgs a{};
+    a.tile_tokens = p.block_tokens / 2;
+    a.box_rows = std::min(p.page_size, BN);
+    CUtensorMap mq, mk, mv;
+    {
+        const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)p.q_heads, (cuuint64_t)p.n_tokens};
+        const int64_t strides[2] = {p.q_heads == 1 ? D : p.q_head_stride, p.q_token_stride};
+        const cuuint32_t box[3] = {64, (cuuint32_t)p.group, (cuuint32_t)a.tile_tokens};
+        const int32_t rc = encode(ctx, &mq, BF16, p.q, 3, dims, strides, box);
+        if (rc != SANIC_OK) return rc;
+    }
+    for (int kv = 0; kv < 2; ++kv) {
+        Pool pool;
+        pool_of(kv ? p.v_page_stride : p.k_page_stride, kv ? p.v_row_stride : p.k_row_stride, kv ? p.v_head_stride : p.k_head_stride, p.n_pages,
+                p.page_size, p.kv_heads, D, &pool);
+        const cuuint64_t hd = p.kv_heads, rd = p.page_size;
+        const cuuint64_t dims[4] = {(cuuint64_t)D, pool.heads_inner ? hd : rd, pool.heads_inner ? rd : hd, (cuuint64_t)p.n_pages};
+        const int64_t strides[3] = {pool.inner, pool.outer, p.n_pages == 1 ? pool.outer * (int64_t)dims[2] : (kv ? p.v_page_stride : p.k_page_stride)};
+        const cuuint32_t br = a.box_rows;
+        const cuuint32_t box[4] = {64, pool.heads_inner ? 1u : br, pool.heads_inner ? br : 1u, 1};
+        const int32_t rc = encode(ctx, kv ? &mv : &mk, BF16, kv ? p.v : p.k, 4, dims, strides, box);
+        if (rc != SANIC_OK) return rc;
+        (kv ? a.v_heads_inner : a.k_heads_inner) = pool.heads_inner;
+    }
+    const int smem = C::DATA + (int)sizeof(Shared<D>) + 1024;
+    static_assert(C::NS * C::TILE >= (MAX_REQUESTS + 1) * 8, "prefix sums fit the ring");
+    static thread_local int ready_on = -1;
+    if (ready_on != ctx->device) {
+        SANIC_CUDA_CHECK(ctx, cudaFuncSetAttribute(paged_tc_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        ready_on = ctx->device;
+    }
+    SANIC_CUDA_CHECK(ctx, launch_pdl(paged_tc_kernel<D, BF16>, dim3(ctas), dim3(NTHREADS), smem, st, mq, mk, mv, p, a, ctx->status_dev));
+    return SANIC_OK;
+}
+}  // namespace
+
+namespace sanic {
+namespace paged {
+// TMA boxes are whole pages of 8, 16, 32, 64 or 128 rows, or 128 rows of pages that are a multiple of 128; strides nest. Other
+// layouts are served by the rows form.
+bool tc_supported(const sanic_attn_paged_params* p) {
+    const int ps = p->page_size;
+    if (!(ps % 128 == 0 || ps == 8 || ps == 16 || ps == 32 || ps == 64)) return false;
+    Pool pool;
+    if (!pool_of(p->k_page_stride, p->k_row_stride, p->k_head_stride, p->n_pages, ps, p->kv_heads, p->head_dim, &pool)) return false;
+    if (!pool_of(p->v_page_stride, p->v_row_stride, p->v_head_stride, p->n_pages, ps, p->kv_heads, p->head_dim, &pool)) return false;
+    const int64_t hs = p->q_heads == 1 ? p->head_dim : p->q_head_stride;
+    return hs >= p->head_dim && (p->n_tokens == 1 || (p->q_token_stride % hs == 0 && p->q_token_stride >= hs)) && p->q_token_stride < (1ll << 38) && p->q_token_stride > 0;
+}
+int32_t tc_launch(sanic_ctx* ctx, const Params& p, int head_dim, int dtype, int ctas, void* stream) {
+    cudaStream_t st = (cudaStream_t)stream;
+    if (head_dim == 128) return dtype == SANIC_BF16 ? launch<128, true>(ctx, p, ctas, st) : launch<128, false>(ctx, p, ctas, st);
+    return dtype == SANIC_BF16 ? launch<64, true>(ctx, p, ctas, st) : launch<64, false>(ctx, p, ctas, st);
+}
+}  // namespace paged
+}  // namespace sanic
