@@ -7,7 +7,8 @@
 //   warp 0       producer: page ids of a 128-key tile one tile ahead (a lane per page), then one TMA box per page and 64
 //                columns; K and V tiles share one ring
 //   warps 1, 3   MMA issuers, one per query tile
-//   warp 2       tensor-memory allocator
+//   warp 2       tensor-memory allocator, then the walk over the CTA's segments: it hands them to the other warps through a ring of
+//                four in shared memory, so that none of them spends registers or global loads on it
 //   warps 4-7    softmax, correction and epilogue of tile 0, one thread per row;   warps 8-11 the same for tile 1
 // Tensor memory, 512 columns. head_dim 64: S0 S1 | P0 P1 | O0 O1 with P in columns of its own, so the next S is computed while
 // the exponentials of this one run. head_dim 128: S0 S1 | O0 O1, P over the S it came from: S(j+1) follows PV(j) in the
@@ -41,9 +42,23 @@ template <int D> struct Tc {
     static constexpr int TM_S = 0, TM_P = ALIAS ? 0 : 256, P_STEP = ALIAS ? 128 : 64, TM_O = ALIAS ? 256 : 384;
     static constexpr int DATA = (2 * QBUF + NS) * TILE;
 };
+// A segment as the roles read it.
+struct __align__(16) Work {
+    int row0, n_tok;       // first token row of the item's block, tokens of it
+    int b, hk, lo, hi;     // keys the item's tokens see
+    int jb, je;            // the segment's key tiles
+    int pos0;              // position of the block's first token
+    int parts;
+    int whole, slot;       // the item's only segment; else the partial slot
+};
+constexpr int END = -1;    // n_tok of the entry behind the last segment
+constexpr int SEG_READERS = 11;
+
 template <int D> struct Shared {
     uint64_t q_full[2], q_empty[2], full[Tc<D>::NS], empty[Tc<D>::NS];
-    uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], o_free[2];      // per query tile
+    uint64_t s_full[2], s_free[2], p_half[2], p_full[2], pv_done[2], o_free[2];      // per query tile
+    uint64_t seg_full[4], seg_empty[4];
+    Work seg[4];
     uint32_t tmem_base;
     volatile int abort_flag;
 };
@@ -110,9 +125,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         for (int i = 0; i < 2; ++i) { mbar_init(&sh->q_full[i], 1); mbar_init(&sh->q_empty[i], 2); }
         for (int s = 0; s < C::NS; ++s) { mbar_init(&sh->full[s], 1); mbar_init(&sh->empty[s], 2); }
         for (int t = 0; t < 2; ++t) {
-            mbar_init(&sh->s_full[t], 1); mbar_init(&sh->s_free[t], 4); mbar_init(&sh->p_full[t], 4);
+            mbar_init(&sh->s_full[t], 1); mbar_init(&sh->s_free[t], 4); mbar_init(&sh->p_half[t], 4); mbar_init(&sh->p_full[t], 4);
             mbar_init(&sh->pv_done[t], 1); mbar_init(&sh->o_free[t], 4);
         }
+        for (int i = 0; i < 4; ++i) { mbar_init(&sh->seg_full[i], 1); mbar_init(&sh->seg_empty[i], SEG_READERS); }
         sh->abort_flag = 0;
         mbar_init_fence();
     }
@@ -122,7 +138,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     long long* cum = (long long*)(aligned + 2 * C::QBUF * C::TILE);      // the prefix sums share the ring's memory
     scan_costs<BN>(p, cum, err);
     DeviceWalk<BN> walk{LoadReq{&p, nullptr}};
-    walk.init(p, cum, blockIdx.x, gridDim.x);
+    if (warp == 2) walk.init(p, cum, blockIdx.x, gridDim.x);
     fence_async_smem();      // generic accesses to the ring end before TMA writes it
     fence_before();
     __syncthreads();
@@ -130,9 +146,20 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const uint32_t tmem = sh->tmem_base;
     volatile int* abortp = &sh->abort_flag;
     const int tile_rows = a.tile_tokens * p.group;
-    Seg s;
+    // The next segment of a role: every reading warp takes every entry.
+    uint32_t n_seg = 0;
+    auto next = [&](Work& w) {
+        const int i = n_seg & 3;
+        if (!__all_sync(0xffffffffu, mbar_wait(&sh->seg_full[i], (n_seg >> 2) & 1, abortp, err, 15))) return false;
+        w = sh->seg[i];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->seg_empty[i]);
+        ++n_seg;
+        return w.n_tok != END;
+    };
+    Work s;
 
-    // Every role walks the same segments. The first warpgroup gives registers to the softmax warpgroups: 128 x 72 + 256 x 216 =
+    // The first warpgroup gives registers to the softmax warpgroups: 128 x 72 + 256 x 216 =
     // the 64,512 the launch was given.
     if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0) {
@@ -140,11 +167,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         bool ok = true;
         int n = 0;
         const int boxes = BN / a.box_rows;
-        while (ok && walk.next(p, s)) {
+        while (ok && next(s)) {
             if (s.je <= s.jb) continue;
             const int32_t* row = p.table + (int64_t)s.b * p.table_stride;
-            const int block0 = s.rb * p.block_tokens;
-            const int tiles = min(p.block_tokens, s.r.qn - block0) > a.tile_tokens ? 2 : 1;
+            const int tiles = s.n_tok > a.tile_tokens ? 2 : 1;
             // a lane's page of key tile j: -1 where no visible key lies in its box, n_pages (read as zeros) for a bad entry
             auto page_of = [&](int j) {
                 const int key = j * BN + lane * a.box_rows;
@@ -183,7 +209,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                         for (int t = 0; t < tiles; ++t)
                             for (int c = 0; c < C::SLABS; ++c)
                                 tma_load_3d(q_addr + (qb * 2 + t) * C::TILE + c * C::SLAB, &map_q, &sh->q_full[qb], c * 64, s.hk * p.group,
-                                            s.r.q0 + block0 + t * a.tile_tokens);
+                                            s.row0 + t * a.tile_tokens);
                     }
                     __syncwarp();
                 }
@@ -200,10 +226,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         uint32_t u_base = 0;                 // ring position of the segment's first key tile
         uint32_t n_qk = 0, n_pv = 0;         // QK / PV issues so far
         uint32_t n_act = 0;                  // earlier segments in which this tile had rows
-        while (ok && walk.next(p, s)) {
+        while (ok && next(s)) {
             if (s.je <= s.jb) continue;
-            const int block0 = s.rb * p.block_tokens;
-            const bool both = min(p.block_tokens, s.r.qn - block0) > a.tile_tokens;
+            const bool both = s.n_tok > a.tile_tokens;
             const int qb = C::QBUF == 2 ? n & 1 : 0;
             const uint32_t q_phase = (C::QBUF == 2 ? n >> 1 : n) & 1;
             ++n;
@@ -220,73 +245,86 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 }
                 continue;
             }
-            int jq = s.jb, jp = s.jb;        // next key tile whose QK / PV is to be issued
-            uint32_t idle = 0;
-            while (ok && jp < s.je) {
-                bool progressed = false;
-                if (jq < s.je) {
-                    const uint32_t u = u_base + 2 * (uint32_t)(jq - s.jb);
-                    const int slot = u % C::NS;
-                    const bool free_s = C::ALIAS ? jq == jp : n_qk == 0 || mbar_test(&sh->s_free[t], (n_qk - 1) & 1);
-                    if (__all_sync(0xffffffffu, free_s && mbar_test(&sh->full[slot], (u / C::NS) & 1))) {
-                        fence_after();
-                        const uint64_t ad = make_desc(q_addr + (qb * 2 + t) * C::TILE, 16, 1024);
-                        const uint64_t bd = make_desc(ring_addr + slot * C::TILE, 16, 1024);
-                        if (leader) {
+            // Every wait that is not the last of its product's is taken ahead of it, and the order of the products is fixed: the
+            // warp spends no time looking for what came first (a poll over four barriers took 600 clocks beside the softmax warps,
+            // and stood in the chain S -> P -> PV -> S twice).
+            const uint64_t q_desc = make_desc(q_addr + (qb * 2 + t) * C::TILE, 16, 1024);
+            auto wait_on = [&](uint64_t* bar, uint32_t parity, int code) {
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abortp, err, code));
+            };
+            auto ring_wait = [&](uint32_t u) { wait_on(&sh->full[u % C::NS], (u / C::NS) & 1, 13); };
+            auto issue_qk = [&](int j) {          // K's tile has arrived and S is free
+                const int slot = (u_base + 2 * (uint32_t)(j - s.jb)) % C::NS;
+                const uint64_t bd = make_desc(ring_addr + slot * C::TILE, 16, 1024);
+                fence_after();
+                if (leader) {
 #pragma unroll
-                            for (int kk = 0; kk < D / 16; ++kk) {
-                                const uint32_t o = (kk >> 2) * (C::SLAB >> 4) + (kk & 3) * 2;
-                                umma_f16(tmem + C::TM_S + t * BN, ad + o, bd + o, idesc_qk, kk > 0 ? 1u : 0u);
-                            }
-                            umma_commit(&sh->s_full[t]);
-                            umma_commit(&sh->empty[slot]);
-                            if (jq + 1 == s.je) umma_commit(&sh->q_empty[qb]);
-                        }
-                        __syncwarp();
-                        ++jq; ++n_qk; progressed = true;
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t o = (kk >> 2) * (C::SLAB >> 4) + (kk & 3) * 2;
+                        umma_f16(tmem + C::TM_S + t * BN, q_desc + o, bd + o, idesc_qk, kk > 0 ? 1u : 0u);
                     }
+                    umma_commit(&sh->s_full[t]);
+                    umma_commit(&sh->empty[slot]);
+                    if (j + 1 == s.je) umma_commit(&sh->q_empty[qb]);
                 }
-                if (jp < jq) {
-                    const uint32_t u = u_base + 2 * (uint32_t)(jp - s.jb) + 1;
-                    const int slot = u % C::NS;
-                    const bool first = jp == s.jb;
-                    // the first PV of a segment overwrites O: the epilogue of the tile's previous segment must have read it
-                    if (__all_sync(0xffffffffu, mbar_test(&sh->p_full[t], n_pv & 1) && mbar_test(&sh->full[slot], (u / C::NS) & 1) &&
-                                                 (!first || n_act == 0 || mbar_test(&sh->o_free[t], (n_act - 1) & 1)))) {
-                        const int za = max(0, s.lo - jp * BN), zb = min(BN, s.hi - jp * BN);
-                        if (za > 0 || zb < BN) {       // rows [0, za) and [zb, 128) of V hold nothing of the item's
-                            const int n_rows = za + BN - zb;
-                            for (int i = lane; i < n_rows * 8 * C::SLABS; i += 32) {
-                                const int r = i / (8 * C::SLABS), c = i % (8 * C::SLABS);
-                                const int rr = r < za ? r : zb + r - za;
-                                asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(ring_addr + slot * C::TILE + (c >> 3) * C::SLAB + rr * 128 + (c & 7) * 16), "r"(0) : "memory");
-                            }
-                            fence_async_smem();
-                            __syncwarp();
-                        }
-                        fence_after();
-                        const uint64_t vd = make_desc(ring_addr + slot * C::TILE, C::SLAB, 1024);
-                        if (leader) {
+                __syncwarp();
+                ++n_qk;
+            };
+            ring_wait(u_base);
+            if (!C::ALIAS && n_qk > 0) wait_on(&sh->s_free[t], (n_qk - 1) & 1, 17);
+            if (!ok) break;
+            issue_qk(s.jb);
+            for (int j = s.jb; j < s.je; ++j) {
+                const uint32_t u = u_base + 2 * (uint32_t)(j - s.jb) + 1;      // V's tile; K of the next key tile follows
+                const int slot = u % C::NS;
+                const bool first = j == s.jb, more = j + 1 < s.je;
+                if (more) ring_wait(u + 1);
+                if (!C::ALIAS && more) {
+                    wait_on(&sh->s_free[t], (n_qk - 1) & 1, 17);
+                    if (!ok) break;
+                    issue_qk(j + 1);
+                }
+                ring_wait(u);
+                if (!ok) break;
+                const int za = max(0, s.lo - j * BN), zb = min(BN, s.hi - j * BN);
+                if (za > 0 || zb < BN) {       // rows [0, za) and [zb, 128) of V hold nothing of the item's
+                    const int n_rows = za + BN - zb;
+                    for (int i = lane; i < n_rows * 8 * C::SLABS; i += 32) {
+                        const int r = i / (8 * C::SLABS), c = i % (8 * C::SLABS);
+                        const int rr = r < za ? r : zb + r - za;
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(ring_addr + slot * C::TILE + (c >> 3) * C::SLAB + rr * 128 + (c & 7) * 16), "r"(0) : "memory");
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                }
+                // the first PV of a segment overwrites O: the epilogue of the tile's previous segment must have read it
+                if (first && n_act > 0) wait_on(&sh->o_free[t], (n_act - 1) & 1, 18);
+                const uint64_t vd = make_desc(ring_addr + slot * C::TILE, C::SLAB, 1024);
+                // A = P from tensor memory: 16 keys = 8 columns per step; the first 64 keys while the others' weights are computed
+                wait_on(&sh->p_half[t], n_pv & 1, 20);
+                if (!ok) break;
+                fence_after();
+                if (leader) {
 #pragma unroll
-                            for (int kk = 0; kk < BN / 16; ++kk)       // A = P from tensor memory: 16 keys = 8 columns per step
-                                umma_f16_ts(tmem + C::TM_O + t * D, tmem + C::TM_P + t * C::P_STEP + 8 * kk, vd + 128 * kk, idesc_pv,
-                                            (!first || kk > 0) ? 1u : 0u);
-                            if (!C::ALIAS || jp + 1 == s.je) umma_commit(&sh->pv_done[t]);
-                            umma_commit(&sh->empty[slot]);
-                        }
-                        __syncwarp();
-                        ++jp; ++n_pv; progressed = true;
-                    }
+                    for (int kk = 0; kk < BN / 32; ++kk)
+                        umma_f16_ts(tmem + C::TM_O + t * D, tmem + C::TM_P + t * C::P_STEP + 8 * kk, vd + 128 * kk, idesc_pv, (!first || kk > 0) ? 1u : 0u);
                 }
-                if (progressed) idle = 0;
-                else {
-                    __nanosleep(32);
-                    if (++idle > (SPIN_LIMIT >> 4) || ((idle & 1023u) == 0 && __any_sync(0xffffffffu, *abortp != 0))) {
-                        if (idle > (SPIN_LIMIT >> 4) && leader) { *abortp = 1; atomicCAS(err, 0, 13); }
-                        ok = false;
-                    }
+                __syncwarp();
+                wait_on(&sh->p_full[t], n_pv & 1, 19);
+                if (!ok) break;
+                fence_after();
+                if (leader) {
+#pragma unroll
+                    for (int kk = BN / 32; kk < BN / 16; ++kk)
+                        umma_f16_ts(tmem + C::TM_O + t * D, tmem + C::TM_P + t * C::P_STEP + 8 * kk, vd + 128 * kk, idesc_pv, 1u);
+                    if (!C::ALIAS || !more) umma_commit(&sh->pv_done[t]);
+                    umma_commit(&sh->empty[slot]);
                 }
+                __syncwarp();
+                ++n_pv;
+                if (C::ALIAS && more) issue_qk(j + 1);
             }
+            if (!ok) break;
             u_base += 2 * (uint32_t)(s.je - s.jb);
             ++n_act;
         }
@@ -301,21 +339,18 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const int row_tok = row / p.group, row_head = row - row_tok * p.group;
         uint32_t n_it = 0, n_act = 0;        // key tiles folded, segments served by this tile so far
         bool ok = true, scores_ready = false;
-        int4 merge = make_int4(0, 0, 0, 0);
-        while (ok && walk.next(p, s)) {
-            const int block0 = s.rb * p.block_tokens;
-            const int n_tok = min(p.block_tokens, s.r.qn - block0);
-            if (t == 0 && s.parts > 1) merge = make_int4(s.r.q0 + block0, n_tok, s.hk, s.parts);
+        while (ok && next(s)) {
+            const int n_tok = s.n_tok;
             const int tok = t * a.tile_tokens + row_tok;
             const bool valid = row < tile_rows && tok < n_tok;
             if (t == 1 && n_tok <= a.tile_tokens) continue;
             const bool empty = s.je <= s.jb;
-            const int64_t at = ((int64_t)(s.r.q0 + block0 + tok)) * p.q_heads + s.hk * p.group + row_head;
+            const int64_t at = (int64_t)(s.row0 + tok) * p.q_heads + s.hk * p.group + row_head;
             float m = -INFINITY, l = 0.0f;
-            const int pos = s.r.kv - s.r.qn + block0 + tok;
+            const int pos = s.pos0 + tok;
             const int khi = valid ? max(0, pos + 1) : 0, klo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
             // key tiles from inner_lo to inner_hi are seen whole by every row of the tile
-            const int tile_pos = s.r.kv - s.r.qn + block0 + t * a.tile_tokens;
+            const int tile_pos = s.pos0 + t * a.tile_tokens;
             const int inner_hi = tile_pos + 1;
             const int inner_lo = p.window > 0 ? tile_pos + a.tile_tokens - p.window : 0;
             const bool busy = __any_sync(0xffffffffu, valid);      // a warp without rows only keeps the barriers' count
@@ -335,7 +370,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                         ok = __all_sync(0xffffffffu, n_it == 0 || mbar_wait(&sh->pv_done[t], (n_it - 1) & 1, abortp, err, 24));
                         if (!ok) break;
                     }
-                    if (lane == 0) mbar_arrive(&sh->p_full[t]);
+                    if (lane == 0) { mbar_arrive(&sh->p_half[t]); mbar_arrive(&sh->p_full[t]); }
                     continue;
                 }
                 const int k0 = j * BN;
@@ -432,6 +467,12 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     const float p0 = ex2(x0), p1 = ex2(x1);
                     fadd2(sums[(2 * i) & 7], sums[(2 * i + 1) & 7], p0, p1);
                     r[i] = pack2<BF16>(p0, p1);
+                    if (i == 36) {        // by now the first half has landed: its product may start
+                        tmem_st_wait();
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh->p_half[t]);
+                    }
                 }
                 tmem_st32(p_tmem + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
                 l = l * alpha + (((sums[0] + sums[1]) + (sums[2] + sums[3])) + ((sums[4] + sums[5]) + (sums[6] + sums[7])));
@@ -458,7 +499,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 for (int i = 0; i < D; ++i) o[i] = 0u;
             }
             if (!valid) continue;
-            if (s.starts && s.finishes) {
+            if (s.whole) {
                 const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;      // no visible key: zeros, and -inf for the log-sum-exp
                 uint16_t* dst = (uint16_t*)p.out + at * D;
                 if (!(l != 0.0f)) {
@@ -475,7 +516,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 }
                 if (p.lse) p.lse[at] = (m + log2f(l) - P_SHIFT) * LN2;
             } else {
-                const size_t r = (size_t)partial_slot(s, blockIdx.x) * p.rows + t * tile_rows + row;
+                const size_t r = (size_t)s.slot * p.rows + t * tile_rows + row;
                 float4* dst = (float4*)(p.ws_o + r * D);
 #pragma unroll
                 for (int q = 0; q < D / 4; ++q)
@@ -483,7 +524,30 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 p.ws_ml[r] = make_float2(m, l);
             }
         }
-        if (warp == 4 && lane == 0) p.ws_merge[blockIdx.x] = merge;
+    } else {      // warp 2
+        int4 merge = make_int4(0, 0, 0, 0);
+        Seg g;
+        for (bool more = true; more; ++n_seg) {
+            more = walk.next(p, g);
+            const int i = n_seg & 3;
+            if (!__all_sync(0xffffffffu, mbar_wait(&sh->seg_empty[i], ((n_seg >> 2) & 1) ^ 1, abortp, err, 16))) break;
+            if (lane == 0) {
+                Work w{};
+                w.n_tok = END;
+                if (more) {
+                    const int block0 = g.rb * p.block_tokens;
+                    w.row0 = g.r.q0 + block0; w.n_tok = min(p.block_tokens, g.r.qn - block0);
+                    w.b = g.b; w.hk = g.hk; w.lo = g.lo; w.hi = g.hi; w.jb = g.jb; w.je = g.je;
+                    w.pos0 = g.r.kv - g.r.qn + block0; w.parts = g.parts;
+                    w.whole = g.starts && g.finishes; w.slot = (int)partial_slot(g, blockIdx.x);
+                    if (g.parts > 1) merge = make_int4(w.row0, w.n_tok, g.hk, g.parts);
+                }
+                sh->seg[i] = w;
+                mbar_arrive(&sh->seg_full[i]);
+            }
+            __syncwarp();
+        }
+        if (lane == 0) p.ws_merge[blockIdx.x] = merge;
     }
     fence_before();
     __syncthreads();
