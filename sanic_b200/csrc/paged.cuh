@@ -22,6 +22,8 @@ struct Params : Shape {
     int n_tokens, q_heads, group, page_size, page_shift, n_pages, max_pages;
     float scale;
     int rows;              // rows of a partial slot (at least block_tokens * group)
+    int rows_above, rows_upto;   // requests of this launch: those whose chunk has more and at most this many query rows
+    int beside;            // 1: this launch runs beside the one before it (the other class of requests) and waits for it at its end
     // workspace: float [2 * ctas][rows][head_dim], float2 (max in log2 units, sum) [2 * ctas][rows], one int4 per CTA: the item
     // that starts in its range and is shared with the next CTAs (first token row, tokens, kv head, CTAs that hold a part; 0: none)
     float* ws_o; float2* ws_ml; int4* ws_merge;
@@ -39,7 +41,9 @@ struct LoadReq {
         r.q0 = min(max(s, 0), p->n_tokens);
         r.qn = min(max(e, r.q0), p->n_tokens) - r.q0;
         r.kv = (int)min((long long)max(kv, 0), (long long)p->max_pages * p->page_size);
+        const long long rows = (long long)r.qn * p->group;
         if ((r.q0 != s || r.q0 + r.qn != e || r.kv != kv) && err) atomicCAS(err, 0, STATUS_ATTN);
+        if (rows <= p->rows_above || rows > p->rows_upto) r.qn = 0;
         return r;
     }
 };

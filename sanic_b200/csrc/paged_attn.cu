@@ -21,6 +21,8 @@ using namespace sanic;
 using namespace sanic::paged;
 
 constexpr int KT = 64;
+// Chunks of more query rows than this (tokens * heads of a group) go to the tensor-memory form where its loads suit the layout.
+constexpr int TC_ABOVE_ROWS = 32;
 
 template <int D> struct Cfg {
     static constexpr int STAGES = (D == 128) ? 3 : 4;
@@ -96,19 +98,23 @@ __global__ void __launch_bounds__(128) paged_rows_kernel(const __grid_constant__
         const int block0 = s.rb * p.block_tokens;                              // first token of the item in its chunk
         const int n_tok = min(p.block_tokens, s.r.qn - block0);
 
-        // element offsets of a tile's keys, by threads 0..63
-        auto offsets = [&](int tile, int key_in_tile) {
-            longlong2 o = make_longlong2(-1, -1);
+        // Page and offsets of a tile's keys, by threads 0..63. The table entry is loaded two tiles ahead of the copies that need
+        // it: under load it takes longer to come than a tile takes to fold (one tile ahead: 434 us for 64 requests of 8000 keys).
+        auto page_of = [&](int tile, int key_in_tile) {
             const int key = (s.jb + tile) * KT + key_in_tile;
-            if (key >= s.lo && key < s.hi) {
-                int page, in_page;
-                if (locate(p, row, key, page, in_page, err))
-                    o = make_longlong2(page * p.k_page_stride + in_page * p.k_row_stride, page * p.v_page_stride + in_page * p.v_row_stride);
-            }
-            return o;
+            int page = -1, in_page;
+            if (tile < n_tiles && key >= s.lo && key < s.hi && !locate(p, row, key, page, in_page, err)) page = -1;
+            return page;
+        };
+        auto offsets = [&](int page, int tile, int key_in_tile) {
+            const int key = (s.jb + tile) * KT + key_in_tile;
+            const int in_page = p.page_shift >= 0 ? key & (p.page_size - 1) : key % p.page_size;
+            return page < 0 ? make_longlong2(-1, -1)
+                            : make_longlong2(page * p.k_page_stride + in_page * p.k_row_stride, page * p.v_page_stride + in_page * p.v_row_stride);
         };
         for (int i = tid; i < STAGES * KT; i += 128)
-            if (i / KT < n_tiles) s_off[i / KT][i % KT] = offsets(i / KT, i % KT);
+            if (i / KT < n_tiles) s_off[i / KT][i % KT] = offsets(page_of(i / KT, i % KT), i / KT, i % KT);
+        int page = tid < KT ? page_of(STAGES, tid) : -1;       // of tile it + STAGES
         __syncthreads();
 #pragma unroll
         for (int st = 0; st < STAGES - 1; ++st) {
@@ -147,9 +153,7 @@ __global__ void __launch_bounds__(128) paged_rows_kernel(const __grid_constant__
             const int nx = it + STAGES - 1;
             if (nx < n_tiles) load_tile<D>(K, V, s_off[nx % STAGES], base + (nx % STAGES) * Cfg<D>::STAGE_BYTES, tid);
             cp_async_commit();
-            longlong2 ahead;
-            const bool look = tid < KT && nx + 1 < n_tiles;
-            if (look) ahead = offsets(nx + 1, tid);
+            const int ahead = tid < KT ? page_of(nx + 2, tid) : -1;
 
             const uint32_t ks_addr = base + (it % STAGES) * Cfg<D>::STAGE_BYTES, vs_addr = ks_addr + Cfg<D>::TILE_BYTES;
             float sc[NC][2][4];
@@ -223,7 +227,8 @@ __global__ void __launch_bounds__(128) paged_rows_kernel(const __grid_constant__
                     }
                 }
             }
-            if (look) s_off[(nx + 1) % STAGES][tid] = ahead;
+            if (tid < KT) s_off[(nx + 1) % STAGES][tid] = offsets(page, nx + 1, tid);
+            page = ahead;
         }
         cp_async_wait<0>();
         __syncthreads();      // every warp is done with the ring: it takes the warps' carriers
@@ -275,20 +280,26 @@ __global__ void __launch_bounds__(128) paged_rows_kernel(const __grid_constant__
     if (tid == 0) p.ws_merge[blockIdx.x] = merge;
 }
 
-// Merge of the items that several CTAs share. Block (c, y) serves the item that starts in CTA c's range, rows y, y + gridDim.y, ..
-// groups of warps: a row's parts are split over 16 / rows warps (at least one) and joined through shared memory in a fixed order.
+// Merge of the items that several CTAs share, for one fold or for two that ran side by side. A block serves the item that starts
+// in one CTA's range (of the tensor-memory form with its up to 256 rows: an eighth of the item's rows): a row's partials are split over 16 / rows warps (at least one) and joined
+// through shared memory in a fixed order.
+constexpr int TC_MERGE_SPLIT = 8;
 template <int D, bool BF16>
-__global__ void __launch_bounds__(512) paged_merge_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(512) paged_merge_kernel(const __grid_constant__ Params first, const __grid_constant__ Params second, const int n_first) {
     griddep_wait();
     griddep_launch();
-    const int4 it = p.ws_merge[blockIdx.x];
+    const bool one = blockIdx.x < n_first;
+    const Params& p = one ? first : second;
+    const int cta = one ? blockIdx.x : (blockIdx.x - n_first) / TC_MERGE_SPLIT;
+    const int part = one ? 0 : (blockIdx.x - n_first) % TC_MERGE_SPLIT, n_parts = one ? 1 : TC_MERGE_SPLIT;
+    const int4 it = p.ws_merge[cta];
     if (it.w <= 1) return;
     __shared__ float2 s_ml[16];
     __shared__ float s_o[16][D];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int V = D / 32;                      // floats per lane
     const int rows = it.y * p.group;
-    const int r0 = (int)((long long)rows * blockIdx.y / gridDim.y), r1 = (int)((long long)rows * (blockIdx.y + 1) / gridDim.y);
+    const int r0 = (int)((long long)rows * part / n_parts), r1 = (int)((long long)rows * (part + 1) / n_parts);
     int wpr = 16;                                  // warps per row
     while (wpr > 1 && (r1 - r0) * wpr > 16) wpr >>= 1;
     const int rpp = 16 / wpr, sub = warp % wpr;    // rows at a time, this warp's share of the parts
@@ -307,7 +318,7 @@ __global__ void __launch_bounds__(512) paged_merge_kernel(const __grid_constant_
 #pragma unroll
                     for (int i = 0; i < V; ++i) a[u][i] = 0.0f;
                     if (q < it.w) {
-                        const size_t at = ((size_t)(blockIdx.x + q) * 2 + (q == 0 ? 1 : 0)) * p.rows + r;
+                        const size_t at = ((size_t)(cta + q) * 2 + (q == 0 ? 1 : 0)) * p.rows + r;
                         x[u] = __ldcg(p.ws_ml + at);
                         const float* po = p.ws_o + at * D + lane * V;
                         if (V == 4) { const float4 f = __ldcg((const float4*)po); a[u][0] = f.x; a[u][1] = f.y; a[u][V - 2] = f.z; a[u][V - 1] = f.w; }
@@ -376,23 +387,38 @@ int32_t launch_rows_any(sanic_ctx* ctx, const Params& p, int D, int dtype, int c
 // Resident CTAs of the rows kernel: two or three per SM, what its shared memory leaves (96 or 64 KB each).
 int rows_ctas(const sanic_ctx* ctx, int D) { return ctx->sm_count * (D == 128 ? 2 : 3); }
 
-// Which form serves a call, and the rows of an item.
-struct Plan { bool tc; int rows, ctas; };
+// Which forms serve a call: the rows form (`rows` query rows per item; 0: not launched) and the tensor-memory form (`tc`).
+struct Plan { int rows, rows_ctas; bool tc; int tc_ctas; };
+int pow2_rows(long long want) { int r = 16; while (r < 64 && r < want) r *= 2; return r; }
 Plan make_plan(const sanic_ctx* ctx, const sanic_attn_paged_params* p) {
     const int group = p->q_heads / p->kv_heads;
     const long long want = (long long)(p->max_query_len > 0 ? p->max_query_len : p->n_tokens) * group;
     Plan pl{};
-    pl.tc = want > 64 && tc_supported(p);
-    if (pl.tc) { pl.rows = TC_ROWS; pl.ctas = ctx->sm_count; return pl; }
-    pl.rows = 16;
-    while (pl.rows < 64 && pl.rows < want) pl.rows *= 2;
-    pl.ctas = rows_ctas(ctx, p->head_dim);
+    pl.rows_ctas = rows_ctas(ctx, p->head_dim);
+    pl.tc = want > TC_ABOVE_ROWS && tc_supported(p);
+    if (pl.tc) {
+        // A batch may hold single tokens beside its chunks: those are the rows form's, in a launch of their own (28 decodes beside
+        // four chunks of 300-600 tokens: 145 us in one launch of the tensor-memory form)
+        pl.tc_ctas = ctx->sm_count;
+        pl.rows = p->n_requests > 1 ? pow2_rows(group) : 0;
+    } else {
+        pl.rows = pow2_rows(want);
+    }
     return pl;
 }
 
+size_t slots_bytes(int ctas, int rows, int D) { return 2 * (size_t)ctas * rows * (D * 4 + 8) + (size_t)ctas * 16; }
 size_t workspace_bytes(const Plan& pl, int D) {
-    const size_t slots = 2 * (size_t)pl.ctas * pl.rows;
-    return slots * D * 4 + slots * 8 + (size_t)pl.ctas * 16;
+    return (pl.rows ? slots_bytes(pl.rows_ctas, pl.rows, D) : 0) + (pl.tc ? slots_bytes(pl.tc_ctas, TC_ROWS, D) : 0);
+}
+// Lays one launch's partials out in the workspace; returns what follows them.
+unsigned char* place(Params& q, unsigned char* ws, int ctas, int rows, int D) {
+    const size_t slots = 2 * (size_t)ctas * rows;
+    q.rows = rows;
+    q.ws_o = (float*)ws;
+    q.ws_ml = (float2*)(q.ws_o + slots * D);
+    q.ws_merge = (int4*)(q.ws_ml + slots);
+    return ws + slots_bytes(ctas, rows, D);
 }
 
 int32_t validate(sanic_ctx* ctx, const sanic_attn_paged_params* p) {
@@ -422,11 +448,10 @@ int32_t validate(sanic_ctx* ctx, const sanic_attn_paged_params* p) {
 }  // namespace
 
 namespace {
-// One block column per CTA of the fold; `row_split` blocks share an item's rows.
-void launch_merge(const Params& p, int D, int dtype, int ctas, int row_split, cudaStream_t st, cudaError_t* e) {
-    const dim3 grid(ctas, row_split), block(512);
-    if (D == 128) *e = dtype == SANIC_BF16 ? launch_pdl(paged_merge_kernel<128, true>, grid, block, 0, st, p) : launch_pdl(paged_merge_kernel<128, false>, grid, block, 0, st, p);
-    else *e = dtype == SANIC_BF16 ? launch_pdl(paged_merge_kernel<64, true>, grid, block, 0, st, p) : launch_pdl(paged_merge_kernel<64, false>, grid, block, 0, st, p);
+cudaError_t launch_merge(const Params& a, int n_a, const Params& b, int n_b, int D, int dtype, cudaStream_t st) {
+    const dim3 grid(n_a + n_b * TC_MERGE_SPLIT), block(512);
+    if (D == 128) return dtype == SANIC_BF16 ? launch_pdl(paged_merge_kernel<128, true>, grid, block, 0, st, a, b, n_a) : launch_pdl(paged_merge_kernel<128, false>, grid, block, 0, st, a, b, n_a);
+    return dtype == SANIC_BF16 ? launch_pdl(paged_merge_kernel<64, true>, grid, block, 0, st, a, b, n_a) : launch_pdl(paged_merge_kernel<64, false>, grid, block, 0, st, a, b, n_a);
 }
 }  // namespace
 
@@ -457,21 +482,26 @@ int32_t sanic_attn_paged(sanic_ctx* ctx, const sanic_attn_paged_params* p, void*
     q.page_size = p->page_size; q.n_pages = p->n_pages; q.max_pages = p->max_pages; q.window = p->window; q.scale = p->scale;
     q.page_shift = -1;
     for (int i = 0; i < 31; ++i) if ((1 << i) == p->page_size) q.page_shift = i;
-    q.rows = pl.rows;
-    q.block_tokens = pl.tc ? 2 * (128 / q.group) : pl.rows / q.group;
-    const size_t slots = 2 * (size_t)pl.ctas * pl.rows;
-    q.ws_o = (float*)p->workspace;
-    q.ws_ml = (float2*)(q.ws_o + slots * p->head_dim);
-    q.ws_merge = (int4*)(q.ws_ml + slots);
+    q.rows_upto = INT32_MAX;
+    Params t = q;             // the tensor-memory form's launch
+    unsigned char* ws = (unsigned char*)p->workspace;
     cudaStream_t st = (cudaStream_t)stream;
-    if (pl.tc) rc = tc_launch(ctx, q, p->head_dim, p->dtype, pl.ctas, st);
-    else if (pl.rows == 16) rc = launch_rows_any<1>(ctx, q, p->head_dim, p->dtype, pl.ctas, st);
-    else if (pl.rows == 32) rc = launch_rows_any<2>(ctx, q, p->head_dim, p->dtype, pl.ctas, st);
-    else rc = launch_rows_any<4>(ctx, q, p->head_dim, p->dtype, pl.ctas, st);
-    if (rc != SANIC_OK) return rc;
-    cudaError_t e = cudaSuccess;
-    launch_merge(q, p->head_dim, p->dtype, pl.ctas, pl.tc ? 8 : 1, st, &e);
-    SANIC_CUDA_CHECK(ctx, e);
+    if (pl.rows) {
+        ws = place(q, ws, pl.rows_ctas, pl.rows, p->head_dim);
+        q.block_tokens = pl.rows / q.group;
+        if (pl.tc) { q.rows_upto = t.rows_above = pl.rows; t.beside = 1; }
+        rc = pl.rows == 16   ? launch_rows_any<1>(ctx, q, p->head_dim, p->dtype, pl.rows_ctas, st)
+             : pl.rows == 32 ? launch_rows_any<2>(ctx, q, p->head_dim, p->dtype, pl.rows_ctas, st)
+                             : launch_rows_any<4>(ctx, q, p->head_dim, p->dtype, pl.rows_ctas, st);
+        if (rc != SANIC_OK) return rc;
+    }
+    if (pl.tc) {
+        place(t, ws, pl.tc_ctas, TC_ROWS, p->head_dim);
+        t.block_tokens = 2 * (128 / t.group);
+        rc = tc_launch(ctx, t, p->head_dim, p->dtype, pl.tc_ctas, st);
+        if (rc != SANIC_OK) return rc;
+    }
+    SANIC_CUDA_CHECK(ctx, launch_merge(q, pl.rows ? pl.rows_ctas : 0, t, pl.tc ? pl.tc_ctas : 0, p->head_dim, p->dtype, st));
     return SANIC_OK;
 }
 

@@ -6,7 +6,7 @@
 // once. The two tiles ping-pong on the tensor core: while one tile's softmax warpgroup turns S into P, the other tile's MMAs run.
 //   warp 0       producer: page ids of a 128-key tile one tile ahead (a lane per page), then one TMA box per page and 64
 //                columns; K and V tiles share one ring
-//   warps 1, 3   MMA issuers, one per query tile
+//   warp 1       MMA issuer (head_dim 64: of tile 0, warp 3 of tile 1)
 //   warp 2       tensor-memory allocator, then the walk over the CTA's segments: it hands them to the other warps through a ring of
 //                four in shared memory, so that none of them spends registers or global loads on it
 //   warps 4-7    softmax, correction and epilogue of tile 0, one thread per row;   warps 8-11 the same for tile 1
@@ -40,6 +40,7 @@ template <int D> struct Tc {
     static constexpr int QBUF = D == 64 ? 2 : 1;       // query buffers across items
     static constexpr int NS = D == 64 ? 10 : 5;        // ring slots, one K or V tile each
     static constexpr int TM_S = 0, TM_P = ALIAS ? 0 : 256, P_STEP = ALIAS ? 128 : 64, TM_O = ALIAS ? 256 : 384;
+    static constexpr int ISSUERS = ALIAS ? 1 : 2;      // MMA-issuing warps
     static constexpr int DATA = (2 * QBUF + NS) * TILE;
 };
 // A segment as the roles read it.
@@ -52,7 +53,6 @@ struct __align__(16) Work {
     int whole, slot;       // the item's only segment; else the partial slot
 };
 constexpr int END = -1;    // n_tok of the entry behind the last segment
-constexpr int SEG_READERS = 11;
 
 template <int D> struct Shared {
     uint64_t q_full[2], q_empty[2], full[Tc<D>::NS], empty[Tc<D>::NS];
@@ -101,6 +101,18 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
                  ::"r"(dst), "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
+// Bounded wait of a role that is ahead of the others: asks and sleeps, and leaves the issue slots of its sub-partition to the
+// softmax warps (a suspended try_wait wakes and asks again often enough to cost them a tenth of their rate).
+__device__ __forceinline__ bool mbar_wait_idle(uint64_t* bar, uint32_t parity, uint32_t ns, volatile int* abort_flag, int* err, int code) {
+    for (uint32_t it = 0; it < (SPIN_LIMIT >> 2); ++it) {
+        if (mbar_test(bar, parity)) return true;
+        __nanosleep(ns);
+        if ((it & 255u) == 255u && *abort_flag) return false;
+    }
+    *abort_flag = 1;
+    atomicCAS(err, 0, code);
+    return false;
+}
 __host__ __device__ constexpr uint32_t idesc_of(int M, int N, bool b_mn_major, bool bf16) {     // f16 operands: format fields 0
     return make_idesc(M, N, b_mn_major) & (bf16 ? ~0u : ~((1u << 7) | (1u << 10)));
 }
@@ -122,18 +134,20 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) { mbar_init(&sh->q_full[i], 1); mbar_init(&sh->q_empty[i], 2); }
-        for (int s = 0; s < C::NS; ++s) { mbar_init(&sh->full[s], 1); mbar_init(&sh->empty[s], 2); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sh->q_full[i], 1); mbar_init(&sh->q_empty[i], C::ISSUERS); }
+        for (int s = 0; s < C::NS; ++s) { mbar_init(&sh->full[s], 1); mbar_init(&sh->empty[s], C::ISSUERS); }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&sh->s_full[t], 1); mbar_init(&sh->s_free[t], 4); mbar_init(&sh->p_half[t], 4); mbar_init(&sh->p_full[t], 4);
             mbar_init(&sh->pv_done[t], 1); mbar_init(&sh->o_free[t], 4);
         }
-        for (int i = 0; i < 4; ++i) { mbar_init(&sh->seg_full[i], 1); mbar_init(&sh->seg_empty[i], SEG_READERS); }
+        for (int i = 0; i < 4; ++i) { mbar_init(&sh->seg_full[i], 1); mbar_init(&sh->seg_empty[i], 9 + C::ISSUERS); }      // producer, issuers, softmax
         sh->abort_flag = 0;
         mbar_init_fence();
     }
     if (warp == 2) tmem_alloc(&sh->tmem_base, 512);
-    griddep_wait();          // lengths, table, q and pages come from earlier kernels of the step
+    // Lengths, table, q and pages come from earlier kernels of the step. Beside a rows launch there is nothing to wait for here:
+    // that one started this one behind its own wait. It is waited for at the end, so that what follows this kernel follows both.
+    if (!p.beside) griddep_wait();
     griddep_launch();
     long long* cum = (long long*)(aligned + 2 * C::QBUF * C::TILE);      // the prefix sums share the ring's memory
     scan_costs<BN>(p, cum, err);
@@ -186,7 +200,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, page >= 0)) * a.box_rows * 128 * C::SLABS;
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sh->empty[slot], phase, abortp, err, 11));
+                    ok = __all_sync(0xffffffffu, mbar_wait_idle(&sh->empty[slot], phase, 64, abortp, err, 11));
                     if (!ok) break;
                     if (lane == 0) mbar_expect_tx(&sh->full[slot], bytes);
                     __syncwarp();
@@ -202,7 +216,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 }
                 if (ok && j == s.jb) {       // the query tiles, behind the first keys: those need not wait for the last item's last product
                     const int qb = C::QBUF == 2 ? n & 1 : 0;
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sh->q_empty[qb], ((C::QBUF == 2 ? n >> 1 : n) & 1) ^ 1, abortp, err, 10));
+                    ok = __all_sync(0xffffffffu, mbar_wait_idle(&sh->q_empty[qb], ((C::QBUF == 2 ? n >> 1 : n) & 1) ^ 1, 64, abortp, err, 10));
                     if (!ok) break;
                     if (lane == 0) {
                         mbar_expect_tx(&sh->q_full[qb], tiles * tile_rows * 128 * C::SLABS);
@@ -217,92 +231,61 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             }
             ++n;
         }
-    } else if (warp == 1 || warp == 3) {
+    } else if (warp == 1 || (C::ISSUERS == 2 && warp == 3)) {
+        // head_dim 128: one warp issues for both tiles, in the order PV0 QK0 PV1 QK1. Two issuers interleave on the tensor core,
+        // both tiles' scores then arrive at the same moment and the tiles fall into step (softmax together, products
+        // together: 4200 clocks per key tile); in one order tile 0's scores arrive while tile 1's products run, and the tiles
+        // stay half a period apart. head_dim 64: the scores run one key tile ahead of the weights and the exponentials set
+        // the pace, so a warp per tile waits for its own tile only (one for both: 1330 against 1000 us).
+        const int t_first = __shfl_sync(0xffffffffu, warp == 3 ? 1 : 0, 0);
         const bool leader = elect_one();
-        const int t = __shfl_sync(0xffffffffu, warp == 3 ? 1 : 0, 0);
         constexpr uint32_t idesc_qk = idesc_of(BM, BN, false, BF16), idesc_pv = idesc_of(BM, D, true, BF16);
         bool ok = true;
         int n = 0;
         uint32_t u_base = 0;                 // ring position of the segment's first key tile
-        uint32_t n_qk = 0, n_pv = 0;         // QK / PV issues so far
-        uint32_t n_act = 0;                  // earlier segments in which this tile had rows
+        uint32_t n_qk[2] = {0, 0}, n_pv[2] = {0, 0};      // products issued so far
+        uint32_t n_act[2] = {0, 0};          // earlier segments in which the tile had rows
         while (ok && next(s)) {
             if (s.je <= s.jb) continue;
             const bool both = s.n_tok > a.tile_tokens;
+            const int last_t = both && C::ISSUERS == 1 ? 1 : t_first;      // the tile behind which this issuer hands K, V and Q back
             const int qb = C::QBUF == 2 ? n & 1 : 0;
             const uint32_t q_phase = (C::QBUF == 2 ? n >> 1 : n) & 1;
             ++n;
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh->q_full[qb], q_phase, abortp, err, 12));
-            if (!ok) break;
-            fence_after();
-            if (t == 1 && !both) {
-                // No rows for this tile: everything goes back untouched, but in step with the producer, so that no barrier is
-                // ever asked for a phase more than one ahead of its own.
-                if (leader) mbar_arrive(&sh->q_empty[qb]);
-                for (int i = 0; i < 2 * (s.je - s.jb) && ok; ++i, ++u_base) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sh->full[u_base % C::NS], (u_base / C::NS) & 1, abortp, err, 14));
-                    if (ok && leader) mbar_arrive(&sh->empty[u_base % C::NS]);
-                }
-                continue;
-            }
-            // Every wait that is not the last of its product's is taken ahead of it, and the order of the products is fixed: the
-            // warp spends no time looking for what came first (a poll over four barriers took 600 clocks beside the softmax warps,
-            // and stood in the chain S -> P -> PV -> S twice).
-            const uint64_t q_desc = make_desc(q_addr + (qb * 2 + t) * C::TILE, 16, 1024);
             auto wait_on = [&](uint64_t* bar, uint32_t parity, int code) {
                 if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abortp, err, code));
             };
             auto ring_wait = [&](uint32_t u) { wait_on(&sh->full[u % C::NS], (u / C::NS) & 1, 13); };
-            auto issue_qk = [&](int j) {          // K's tile has arrived and S is free
+            auto qk = [&](int t, int j) {          // K's tile has arrived
+                if (!C::ALIAS && n_qk[t] > 0) wait_on(&sh->s_free[t], (n_qk[t] - 1) & 1, 17);
+                if (!ok) return;
                 const int slot = (u_base + 2 * (uint32_t)(j - s.jb)) % C::NS;
-                const uint64_t bd = make_desc(ring_addr + slot * C::TILE, 16, 1024);
+                const uint64_t ad = make_desc(q_addr + (qb * 2 + t) * C::TILE, 16, 1024), bd = make_desc(ring_addr + slot * C::TILE, 16, 1024);
                 fence_after();
                 if (leader) {
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
                         const uint32_t o = (kk >> 2) * (C::SLAB >> 4) + (kk & 3) * 2;
-                        umma_f16(tmem + C::TM_S + t * BN, q_desc + o, bd + o, idesc_qk, kk > 0 ? 1u : 0u);
+                        umma_f16(tmem + C::TM_S + t * BN, ad + o, bd + o, idesc_qk, kk > 0 ? 1u : 0u);
                     }
                     umma_commit(&sh->s_full[t]);
-                    umma_commit(&sh->empty[slot]);
-                    if (j + 1 == s.je) umma_commit(&sh->q_empty[qb]);
+                    if (t == last_t) {
+                        umma_commit(&sh->empty[slot]);
+                        if (j + 1 == s.je) umma_commit(&sh->q_empty[qb]);
+                    }
                 }
                 __syncwarp();
-                ++n_qk;
+                ++n_qk[t];
             };
-            ring_wait(u_base);
-            if (!C::ALIAS && n_qk > 0) wait_on(&sh->s_free[t], (n_qk - 1) & 1, 17);
-            if (!ok) break;
-            issue_qk(s.jb);
-            for (int j = s.jb; j < s.je; ++j) {
-                const uint32_t u = u_base + 2 * (uint32_t)(j - s.jb) + 1;      // V's tile; K of the next key tile follows
-                const int slot = u % C::NS;
-                const bool first = j == s.jb, more = j + 1 < s.je;
-                if (more) ring_wait(u + 1);
-                if (!C::ALIAS && more) {
-                    wait_on(&sh->s_free[t], (n_qk - 1) & 1, 17);
-                    if (!ok) break;
-                    issue_qk(j + 1);
-                }
-                ring_wait(u);
-                if (!ok) break;
-                const int za = max(0, s.lo - j * BN), zb = min(BN, s.hi - j * BN);
-                if (za > 0 || zb < BN) {       // rows [0, za) and [zb, 128) of V hold nothing of the item's
-                    const int n_rows = za + BN - zb;
-                    for (int i = lane; i < n_rows * 8 * C::SLABS; i += 32) {
-                        const int r = i / (8 * C::SLABS), c = i % (8 * C::SLABS);
-                        const int rr = r < za ? r : zb + r - za;
-                        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(ring_addr + slot * C::TILE + (c >> 3) * C::SLAB + rr * 128 + (c & 7) * 16), "r"(0) : "memory");
-                    }
-                    fence_async_smem();
-                    __syncwarp();
-                }
-                // the first PV of a segment overwrites O: the epilogue of the tile's previous segment must have read it
-                if (first && n_act > 0) wait_on(&sh->o_free[t], (n_act - 1) & 1, 18);
+            auto pv = [&](int t, int j) {          // V's tile has arrived
+                const int slot = (u_base + 2 * (uint32_t)(j - s.jb) + 1) % C::NS;
+                const bool first = j == s.jb;
                 const uint64_t vd = make_desc(ring_addr + slot * C::TILE, C::SLAB, 1024);
+                // the first PV of a segment overwrites O: the epilogue of the tile's previous segment must have read it
+                if (first && n_act[t] > 0) wait_on(&sh->o_free[t], (n_act[t] - 1) & 1, 18);
                 // A = P from tensor memory: 16 keys = 8 columns per step; the first 64 keys while the others' weights are computed
-                wait_on(&sh->p_half[t], n_pv & 1, 20);
-                if (!ok) break;
+                wait_on(&sh->p_half[t], n_pv[t] & 1, 20);
+                if (!ok) return;
                 fence_after();
                 if (leader) {
 #pragma unroll
@@ -310,23 +293,74 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                         umma_f16_ts(tmem + C::TM_O + t * D, tmem + C::TM_P + t * C::P_STEP + 8 * kk, vd + 128 * kk, idesc_pv, (!first || kk > 0) ? 1u : 0u);
                 }
                 __syncwarp();
-                wait_on(&sh->p_full[t], n_pv & 1, 19);
-                if (!ok) break;
+                wait_on(&sh->p_full[t], n_pv[t] & 1, 19);
+                if (!ok) return;
                 fence_after();
                 if (leader) {
 #pragma unroll
                     for (int kk = BN / 32; kk < BN / 16; ++kk)
                         umma_f16_ts(tmem + C::TM_O + t * D, tmem + C::TM_P + t * C::P_STEP + 8 * kk, vd + 128 * kk, idesc_pv, 1u);
-                    if (!C::ALIAS || !more) umma_commit(&sh->pv_done[t]);
-                    umma_commit(&sh->empty[slot]);
+                    if (!C::ALIAS || j + 1 == s.je) umma_commit(&sh->pv_done[t]);
+                    if (t == last_t) umma_commit(&sh->empty[slot]);
                 }
                 __syncwarp();
-                ++n_pv;
-                if (C::ALIAS && more) issue_qk(j + 1);
+                ++n_pv[t];
+            };
+            auto values = [&](int j) {             // V's tile, with nothing in its rows [0, za) and [zb, 128) but zeros
+                const uint32_t u = u_base + 2 * (uint32_t)(j - s.jb) + 1;
+                ring_wait(u);
+                const int za = max(0, s.lo - j * BN), zb = min(BN, s.hi - j * BN);
+                if (ok && (za > 0 || zb < BN)) {
+                    const int n_rows = za + BN - zb;
+                    for (int i = lane; i < n_rows * 8 * C::SLABS; i += 32) {
+                        const int r = i / (8 * C::SLABS), c = i % (8 * C::SLABS);
+                        const int rr = r < za ? r : zb + r - za;
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(ring_addr + (u % C::NS) * C::TILE + (c >> 3) * C::SLAB + rr * 128 + (c & 7) * 16), "r"(0) : "memory");
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                }
+            };
+            wait_on(&sh->q_full[qb], q_phase, 12);
+            if (C::ISSUERS == 2 && t_first == 1 && !both) {
+                // No rows for this tile: everything goes back untouched, but in step with the producer, so that no barrier is
+                // ever asked for a phase more than one ahead of its own.
+                if (ok && leader) mbar_arrive(&sh->q_empty[qb]);
+                for (int i = 0; i < 2 * (s.je - s.jb) && ok; ++i, ++u_base) {
+                    ring_wait(u_base);
+                    if (ok && leader) mbar_arrive(&sh->empty[u_base % C::NS]);
+                }
+                continue;
             }
-            if (!ok) break;
+            ring_wait(u_base);
+            if (C::ALIAS) {
+                qk(0, s.jb);
+                if (both) qk(1, s.jb);
+                for (int j = s.jb; j < s.je && ok; ++j) {
+                    const bool more = j + 1 < s.je;
+                    values(j);
+                    if (more) ring_wait(u_base + 2 * (uint32_t)(j + 1 - s.jb));
+                    pv(0, j);
+                    if (more) qk(0, j + 1);
+                    if (both) {
+                        pv(1, j);
+                        if (more) qk(1, j + 1);
+                    }
+                }
+            } else {
+                qk(t_first, s.jb);
+                for (int j = s.jb; j < s.je && ok; ++j) {
+                    if (j + 1 < s.je) {
+                        ring_wait(u_base + 2 * (uint32_t)(j + 1 - s.jb));
+                        qk(t_first, j + 1);
+                    }
+                    values(j);
+                    pv(t_first, j);
+                }
+            }
             u_base += 2 * (uint32_t)(s.je - s.jb);
-            ++n_act;
+            if (t_first == 0) ++n_act[0];
+            if (t_first == 1 || (C::ISSUERS == 1 && both)) ++n_act[1];
         }
     } else if (warp >= 4) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
@@ -524,13 +558,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 p.ws_ml[r] = make_float2(m, l);
             }
         }
-    } else {      // warp 2
+    } else if (warp == 2) {
         int4 merge = make_int4(0, 0, 0, 0);
         Seg g;
         for (bool more = true; more; ++n_seg) {
             more = walk.next(p, g);
             const int i = n_seg & 3;
-            if (!__all_sync(0xffffffffu, mbar_wait(&sh->seg_empty[i], ((n_seg >> 2) & 1) ^ 1, abortp, err, 16))) break;
+            if (!__all_sync(0xffffffffu, mbar_wait_idle(&sh->seg_empty[i], ((n_seg >> 2) & 1) ^ 1, 256, abortp, err, 16))) break;
             if (lane == 0) {
                 Work w{};
                 w.n_tok = END;
@@ -552,6 +586,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     fence_before();
     __syncthreads();
     if (warp == 2) { fence_after(); tmem_dealloc(tmem, 512); }
+    if (p.beside) griddep_wait();
 }
 
 // Row-major view of rank 3 or 4, 128-byte swizzle, zero fill out of bounds; strides in elements of 2 bytes, dims innermost first.
