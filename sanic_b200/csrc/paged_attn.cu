@@ -14,7 +14,7 @@
 // to the storage type (bf16: 2^-9 per weight; f16 likewise after a shift by 2^8, which keeps the weights of a long flat
 // softmax out of f16's subnormals), sums and maxima are f32.
 // Rows are spread over an exactly resident grid as one contiguous range of (item, key tile) per CTA (see paged.cuh).
-#include "paged.cuh"
+#include "paged_tma.cuh"
 
 namespace {
 using namespace sanic;
@@ -70,15 +70,179 @@ __device__ __forceinline__ void load_tile(const uint16_t* k, const uint16_t* v, 
     }
 }
 
+// The fold of one item's rows by one warp: 16 MT rows of the item over the four warps of a CTA, warp (wr, wk) taking rows
+// 16 wr .. and the wk-th part of a tile's keys.
+template <int D, int MT, bool BF16> struct Fold {
+    static constexpr int R = 16 * MT, WK = 4 / MT, KW = KT / WK, NC = KW / 16;    // rows, warps along keys, keys and 16-key chunks per warp
+    static constexpr int KS = D / 16, NT = D / 8;
+    int wr, wk, g, t, lane;
+    uint32_t qf[KS][4];
+    float o[NT][4], m0, m1, l0, l1;      // of rows ra and ra + 8; maxima in log2 units
+    int lo_a, lo_c;                      // keys a row sees: [lo, lo + cnt)
+    unsigned cnt_a, cnt_c;
+    int inner_lo, inner_hi;              // every row of the item sees the whole of a tile between these
+
+    __device__ __forceinline__ void place(int warp, int lane_) { wr = warp % MT; wk = warp / MT; lane = lane_; g = lane >> 2; t = lane & 3; }
+    __device__ __forceinline__ int ra() const { return wr * 16 + g; }
+
+    // row r of the item is head r % group of token r / group
+    __device__ __forceinline__ void begin(const Params& p, const Seg& s, int block0, int n_tok) {
+        const int r0 = ra(), r1 = r0 + 8, ta = r0 / p.group, tc = r1 / p.group;
+        const uint16_t* Q = (const uint16_t*)p.q + (int64_t)(s.r.q0 + block0) * p.q_token_stride + (int64_t)s.hk * p.group * p.q_head_stride;
+        const uint16_t* qa = Q + ta * p.q_token_stride + (r0 - ta * p.group) * p.q_head_stride + 2 * t;
+        const uint16_t* qc = Q + tc * p.q_token_stride + (r1 - tc * p.group) * p.q_head_stride + 2 * t;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            qf[ks][0] = ta < n_tok ? *(const uint32_t*)(qa + ks * 16) : 0u;
+            qf[ks][1] = tc < n_tok ? *(const uint32_t*)(qc + ks * 16) : 0u;
+            qf[ks][2] = ta < n_tok ? *(const uint32_t*)(qa + ks * 16 + 8) : 0u;
+            qf[ks][3] = tc < n_tok ? *(const uint32_t*)(qc + ks * 16 + 8) : 0u;
+        }
+        const int pos0 = s.r.kv - s.r.qn + block0, pos_a = pos0 + ta, pos_c = pos0 + tc;
+        lo_a = p.window > 0 ? max(0, pos_a - p.window + 1) : 0;
+        lo_c = p.window > 0 ? max(0, pos_c - p.window + 1) : 0;
+        cnt_a = ta < n_tok ? max(0, pos_a + 1 - lo_a) : 0;
+        cnt_c = tc < n_tok ? max(0, pos_c + 1 - lo_c) : 0;
+        inner_hi = pos0 + 1;
+        inner_lo = p.window > 0 ? pos0 + n_tok - p.window : 0;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) { o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f; }
+        m0 = m1 = -INFINITY; l0 = l1 = 0.0f;
+    }
+
+    // One tile: [D/64 halves][64 keys][128 B] of K and of V, chunk index xor (key & 7).
+    __device__ __forceinline__ void tile(uint32_t ks_addr, uint32_t vs_addr, int tile_key, float sl2) {
+        float sc[NC][2][4];
+        const int mi = lane >> 3, r = lane & 7;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[c][0][i] = sc[c][1][i] = 0.0f;
+            const int krow = wk * KW + c * 16 + (mi >> 1) * 8 + r;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const int ch = 2 * ks + (mi & 1);
+                uint32_t r0, r1, r2, r3;
+                ldmatrix_x4(ks_addr + (ch >> 3) * (KT * 128) + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4), r0, r1, r2, r3);
+                mma16816<BF16>(sc[c][0], qf[ks], r0, r1);
+                mma16816<BF16>(sc[c][1], qf[ks], r2, r3);
+            }
+        }
+        float mx0 = -INFINITY, mx1 = -INFINITY;
+        const int key0 = tile_key + wk * KW + 2 * t;
+        const bool edge = tile_key + KT > inner_hi || tile_key < inner_lo;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (edge) {
+                        const int key = key0 + c * 16 + h * 8 + i;
+                        if (!((unsigned)(key - lo_a) < cnt_a)) sc[c][h][i] = -INFINITY;
+                        if (!((unsigned)(key - lo_c) < cnt_c)) sc[c][h][2 + i] = -INFINITY;
+                    }
+                    mx0 = fmaxf(mx0, sc[c][h][i]); mx1 = fmaxf(mx1, sc[c][h][2 + i]);
+                }
+        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1)); mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1)); mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+        const float mn0 = fmaxf(m0, mx0 * sl2), mn1 = fmaxf(m1, mx1 * sl2);      // the scale is positive
+        // (a maximum that is still -inf has nothing to scale; 1 keeps such rows from asking for it)
+        const float a0 = m0 > -INFINITY ? ex2(m0 - mn0) : 1.0f, a1 = m1 > -INFINITY ? ex2(m1 - mn1) : 1.0f;
+        const float sub0 = (mn0 > -INFINITY ? mn0 : 0.0f) - p_shift<BF16>(), sub1 = (mn1 > -INFINITY ? mn1 : 0.0f) - p_shift<BF16>();
+        m0 = mn0; m1 = mn1;
+        float t0 = 0.0f, t1 = 0.0f;
+        uint32_t pf[NC][4];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float e[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                e[h][0] = ex2(fmaf(sc[c][h][0], sl2, -sub0)); e[h][1] = ex2(fmaf(sc[c][h][1], sl2, -sub0));
+                e[h][2] = ex2(fmaf(sc[c][h][2], sl2, -sub1)); e[h][3] = ex2(fmaf(sc[c][h][3], sl2, -sub1));
+                t0 += e[h][0] + e[h][1]; t1 += e[h][2] + e[h][3];
+            }
+            pf[c][0] = pack2<BF16>(e[0][0], e[0][1]); pf[c][1] = pack2<BF16>(e[0][2], e[0][3]);
+            pf[c][2] = pack2<BF16>(e[1][0], e[1][1]); pf[c][3] = pack2<BF16>(e[1][2], e[1][3]);
+        }
+        l0 = l0 * a0 + t0; l1 = l1 * a1 + t1;
+        if (__any_sync(0xffffffffu, a0 != 1.0f || a1 != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) { o[i][0] *= a0; o[i][1] *= a0; o[i][2] *= a1; o[i][3] *= a1; }
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int krow = wk * KW + c * 16 + (mi & 1) * 8 + r;
+#pragma unroll
+            for (int dp = 0; dp < D / 16; ++dp) {
+                const int ch = 2 * dp + (mi >> 1);
+                uint32_t r0, r1, r2, r3;
+                ldmatrix_x4_trans(vs_addr + (ch >> 3) * (KT * 128) + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4), r0, r1, r2, r3);
+                mma16816<BF16>(o[2 * dp], pf[c], r0, r1);
+                mma16816<BF16>(o[2 * dp + 1], pf[c], r2, r3);
+            }
+        }
+    }
+
+    // The end of a segment: the carriers of the warps that share rows meet in shared memory (`os`, [WK][R][D] floats with the column
+    // xor 8 (row & 3) against bank conflicts; `ml`, [WK][R]) and the rows leave, to out or to the segment's partial. `meet` is
+    // a barrier of the 128 threads; all of them are done with what `os` held when this begins.
+    template <class Meet>
+    __device__ __forceinline__ void finish(const Params& p, const Seg& s, int block0, int n_tok, float* os, float2* ml, int tid, Meet meet) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+        const int r0 = ra(), r1 = r0 + 8;
+        if (t == 0) { ml[wk * R + r0] = make_float2(m0, l0); ml[wk * R + r1] = make_float2(m1, l1); }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const int c = (8 * i + 2 * t) ^ ((g & 3) << 3);
+            *(float2*)(os + (wk * R + r0) * D + c) = make_float2(o[i][0], o[i][1]);
+            *(float2*)(os + (wk * R + r1) * D + c) = make_float2(o[i][2], o[i][3]);
+        }
+        meet();
+        const bool whole = s.starts && s.finishes;
+        const size_t slot = partial_slot(s, blockIdx.x);
+        const int rows = n_tok * p.group;
+        for (int idx = tid; idx < rows * (D / 4); idx += 128) {
+            const int r = idx / (D / 4), d = (idx % (D / 4)) * 4, c = d ^ ((r & 3) << 3);
+            float m = -INFINITY, l = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) m = fmaxf(m, ml[w * R + r].x);
+            float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int w = 0; w < WK; ++w) {
+                const float2 x = ml[w * R + r];
+                const float f = x.x > -INFINITY ? ex2(x.x - m) : 0.0f;       // a side that saw nothing has weight 0
+                const float4 v4 = *(const float4*)(os + (w * R + r) * D + c);
+                l += f * x.y;
+                acc.x += f * v4.x; acc.y += f * v4.y; acc.z += f * v4.z; acc.w += f * v4.w;
+            }
+            if (whole) {
+                const int tok = r / p.group, head = s.hk * p.group + r - tok * p.group;
+                const int64_t at = (int64_t)(s.r.q0 + block0 + tok) * p.q_heads + head;
+                const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;      // no visible key: zeros, and -inf for the log-sum-exp
+                *(uint2*)((uint16_t*)p.out + at * D + d) =
+                    make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
+                if (p.lse && d == 0) p.lse[at] = (m + log2f(l) - p_shift<BF16>()) * LN2;
+            } else {
+                *(float4*)(p.ws_o + (slot * p.rows + r) * D + d) = acc;
+                if (d == 0) p.ws_ml[slot * p.rows + r] = make_float2(m, l);
+            }
+        }
+    }
+};
+
+// Any layout: the four warps copy the tiles themselves, 16 bytes a time (cp.async).
 template <int D, int MT, bool BF16>
 __global__ void __launch_bounds__(128) paged_rows_kernel(const __grid_constant__ Params p, int* err) {
-    constexpr int R = 16 * MT, WK = 4 / MT, KW = KT / WK, NC = KW / 16;    // rows, warps along keys, keys and 16-key chunks per warp
-    constexpr int KS = D / 16, NT = D / 8, STAGES = Cfg<D>::STAGES;
+    constexpr int STAGES = Cfg<D>::STAGES;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ longlong2 s_off[STAGES][KT];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int wr = warp % MT, wk = warp / MT;
+    __shared__ float2 s_ml[64];
+    const int tid = threadIdx.x;
     const uint32_t base = smem_u32(smem);
+    Fold<D, MT, BF16> f;
+    f.place(tid >> 5, tid & 31);
 
     griddep_wait();        // q, the pages, the table and the lengths come from earlier kernels of the step
     griddep_launch();
@@ -98,8 +262,7 @@ __global__ void __launch_bounds__(128) paged_rows_kernel(const __grid_constant__
         const int block0 = s.rb * p.block_tokens;                              // first token of the item in its chunk
         const int n_tok = min(p.block_tokens, s.r.qn - block0);
 
-        // Page and offsets of a tile's keys, by threads 0..63. The table entry is loaded two tiles ahead of the copies that need
-        // it: under load it takes longer to come than a tile takes to fold (one tile ahead: 434 us for 64 requests of 8000 keys).
+        // Page and offsets of a tile's keys, by threads 0..63; the table entry is loaded two tiles ahead of the copies that need it.
         auto page_of = [&](int tile, int key_in_tile) {
             const int key = (s.jb + tile) * KT + key_in_tile;
             int page = -1, in_page;
@@ -121,32 +284,7 @@ __global__ void __launch_bounds__(128) paged_rows_kernel(const __grid_constant__
             if (st < n_tiles) load_tile<D>(K, V, s_off[st], base + st * Cfg<D>::STAGE_BYTES, tid);
             cp_async_commit();
         }
-
-        // query fragments: row r of the item is head r % group of token r / group
-        const int ra = wr * 16 + g, rc = ra + 8;
-        const int ta = ra / p.group, tc = rc / p.group;
-        uint32_t qf[KS][4];
-        {
-            const uint16_t* Q = (const uint16_t*)p.q + (int64_t)(s.r.q0 + block0) * p.q_token_stride + (int64_t)s.hk * p.group * p.q_head_stride;
-            const uint16_t* qa = Q + ta * p.q_token_stride + (ra - ta * p.group) * p.q_head_stride + 2 * t;
-            const uint16_t* qc = Q + tc * p.q_token_stride + (rc - tc * p.group) * p.q_head_stride + 2 * t;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                qf[ks][0] = ta < n_tok ? *(const uint32_t*)(qa + ks * 16) : 0u;
-                qf[ks][1] = tc < n_tok ? *(const uint32_t*)(qc + ks * 16) : 0u;
-                qf[ks][2] = ta < n_tok ? *(const uint32_t*)(qa + ks * 16 + 8) : 0u;
-                qf[ks][3] = tc < n_tok ? *(const uint32_t*)(qc + ks * 16 + 8) : 0u;
-            }
-        }
-        // keys a row sees: [first, first + count)
-        const int pos_a = s.r.kv - s.r.qn + block0 + ta, pos_c = s.r.kv - s.r.qn + block0 + tc;
-        const int lo_a = p.window > 0 ? max(0, pos_a - p.window + 1) : 0, lo_c = p.window > 0 ? max(0, pos_c - p.window + 1) : 0;
-        const unsigned cnt_a = ta < n_tok ? max(0, pos_a + 1 - lo_a) : 0, cnt_c = tc < n_tok ? max(0, pos_c + 1 - lo_c) : 0;
-
-        float o[NT][4];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) { o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f; }
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;      // rows ra and rc, log2 units
+        f.begin(p, s, block0, n_tok);
         for (int it = 0; it < n_tiles; ++it) {
             cp_async_wait<STAGES - 2>();
             __syncthreads();
@@ -154,128 +292,136 @@ __global__ void __launch_bounds__(128) paged_rows_kernel(const __grid_constant__
             if (nx < n_tiles) load_tile<D>(K, V, s_off[nx % STAGES], base + (nx % STAGES) * Cfg<D>::STAGE_BYTES, tid);
             cp_async_commit();
             const int ahead = tid < KT ? page_of(nx + 2, tid) : -1;
-
-            const uint32_t ks_addr = base + (it % STAGES) * Cfg<D>::STAGE_BYTES, vs_addr = ks_addr + Cfg<D>::TILE_BYTES;
-            float sc[NC][2][4];
-            {
-                const int mi = lane >> 3, r = lane & 7;
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sc[c][0][i] = sc[c][1][i] = 0.0f;
-                    const int krow = wk * KW + c * 16 + (mi >> 1) * 8 + r;
-#pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        const int ch = 2 * ks + (mi & 1);
-                        uint32_t r0, r1, r2, r3;
-                        ldmatrix_x4(ks_addr + (ch >> 3) * (KT * 128) + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4), r0, r1, r2, r3);
-                        mma16816<BF16>(sc[c][0], qf[ks], r0, r1);
-                        mma16816<BF16>(sc[c][1], qf[ks], r2, r3);
-                    }
-                }
-            }
-            float mx0 = -INFINITY, mx1 = -INFINITY;
-            const int key0 = (s.jb + it) * KT + wk * KW + 2 * t;
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int key = key0 + c * 16 + h * 8 + i;
-                        sc[c][h][i] = (unsigned)(key - lo_a) < cnt_a ? sc[c][h][i] * sl2 : -INFINITY;
-                        sc[c][h][2 + i] = (unsigned)(key - lo_c) < cnt_c ? sc[c][h][2 + i] * sl2 : -INFINITY;
-                        mx0 = fmaxf(mx0, sc[c][h][i]); mx1 = fmaxf(mx1, sc[c][h][2 + i]);
-                    }
-            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1)); mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1)); mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-            const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
-            const float a0 = m0 > -INFINITY ? ex2(m0 - mn0) : 0.0f, a1 = m1 > -INFINITY ? ex2(m1 - mn1) : 0.0f;
-            const float sub0 = (mn0 > -INFINITY ? mn0 : 0.0f) - p_shift<BF16>(), sub1 = (mn1 > -INFINITY ? mn1 : 0.0f) - p_shift<BF16>();
-            m0 = mn0; m1 = mn1;
-            float t0 = 0.0f, t1 = 0.0f;
-            uint32_t pf[NC][4];
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                float e[2][4];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    e[h][0] = ex2(sc[c][h][0] - sub0); e[h][1] = ex2(sc[c][h][1] - sub0);
-                    e[h][2] = ex2(sc[c][h][2] - sub1); e[h][3] = ex2(sc[c][h][3] - sub1);
-                    t0 += e[h][0] + e[h][1]; t1 += e[h][2] + e[h][3];
-                }
-                pf[c][0] = pack2<BF16>(e[0][0], e[0][1]); pf[c][1] = pack2<BF16>(e[0][2], e[0][3]);
-                pf[c][2] = pack2<BF16>(e[1][0], e[1][1]); pf[c][3] = pack2<BF16>(e[1][2], e[1][3]);
-            }
-            l0 = l0 * a0 + t0; l1 = l1 * a1 + t1;
-            if (__any_sync(0xffffffffu, a0 != 1.0f || a1 != 1.0f)) {
-#pragma unroll
-                for (int i = 0; i < NT; ++i) { o[i][0] *= a0; o[i][1] *= a0; o[i][2] *= a1; o[i][3] *= a1; }
-            }
-            {
-                const int mi = lane >> 3, r = lane & 7;
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    const int krow = wk * KW + c * 16 + (mi & 1) * 8 + r;
-#pragma unroll
-                    for (int dp = 0; dp < D / 16; ++dp) {
-                        const int ch = 2 * dp + (mi >> 1);
-                        uint32_t r0, r1, r2, r3;
-                        ldmatrix_x4_trans(vs_addr + (ch >> 3) * (KT * 128) + krow * 128 + (((ch & 7) ^ (krow & 7)) << 4), r0, r1, r2, r3);
-                        mma16816<BF16>(o[2 * dp], pf[c], r0, r1);
-                        mma16816<BF16>(o[2 * dp + 1], pf[c], r2, r3);
-                    }
-                }
-            }
+            const uint32_t ks_addr = base + (it % STAGES) * Cfg<D>::STAGE_BYTES;
+            f.tile(ks_addr, ks_addr + Cfg<D>::TILE_BYTES, (s.jb + it) * KT, sl2);
             if (tid < KT) s_off[(nx + 1) % STAGES][tid] = offsets(page, nx + 1, tid);
             page = ahead;
         }
         cp_async_wait<0>();
         __syncthreads();      // every warp is done with the ring: it takes the warps' carriers
-
-        l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-        float2* ml = (float2*)smem;                        // [WK][R] (max, sum)
-        float* os = (float*)(smem + WK * R * 8);           // [WK][R][D + 4]
-        constexpr int OW = D + 4;
-        if (t == 0) { ml[wk * R + ra] = make_float2(m0, l0); ml[wk * R + rc] = make_float2(m1, l1); }
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            *(float2*)(os + (wk * R + ra) * OW + 8 * i + 2 * t) = make_float2(o[i][0], o[i][1]);
-            *(float2*)(os + (wk * R + rc) * OW + 8 * i + 2 * t) = make_float2(o[i][2], o[i][3]);
-        }
+        f.finish(p, s, block0, n_tok, (float*)smem, s_ml, tid, [] { __syncthreads(); });
+        if (s.parts > 1) merge = make_int4(s.r.q0 + block0, n_tok, s.hk, s.parts);
         __syncthreads();
-        const bool whole = s.starts && s.finishes;
-        const size_t slot = partial_slot(s, blockIdx.x);
-        const int rows = n_tok * p.group;
-        for (int idx = tid; idx < rows * (D / 4); idx += 128) {
-            const int r = idx / (D / 4), d = (idx % (D / 4)) * 4;
-            float m = -INFINITY, l = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WK; ++w) m = fmaxf(m, ml[w * R + r].x);
-            float4 acc = make_float4(0, 0, 0, 0);
-#pragma unroll
-            for (int w = 0; w < WK; ++w) {
-                const float2 x = ml[w * R + r];
-                const float f = x.x > -INFINITY ? ex2(x.x - m) : 0.0f;       // a side that saw nothing has weight 0
-                const float4 v4 = *(const float4*)(os + (w * R + r) * OW + d);
-                l += f * x.y;
-                acc.x += f * v4.x; acc.y += f * v4.y; acc.z += f * v4.z; acc.w += f * v4.w;
+    }
+    if (tid == 0) p.ws_merge[blockIdx.x] = merge;
+}
+
+// Pools that TMA can read (paged_tma.cuh): a fifth warp produces. It walks the same segments ahead of the others, through the ends
+// of items, so that bytes stay in flight while they merge and store; it looks up a tile's pages one tile ahead and issues one
+// copy per lane (a box of a page's rows, 64 columns, of K or of V). The four warps wait for a tile, fold it and hand the stage
+// back, each for itself: no barrier between tiles. (With the copies issued by the folding warps: 434 us by cp.async, 363 us
+// by TMA from warp 0, for 64 requests of 8000 keys on average.)
+struct RowsArgs { int box_rows, k_heads_inner, v_heads_inner; };
+constexpr int TMA_THREADS = 160;
+template <int D, int MT> constexpr int tma_ctas_per_sm() { return D == 128 ? 2 : (MT == 1 ? 3 : 2); }
+
+template <int D, int MT, bool BF16>
+__global__ void __launch_bounds__(TMA_THREADS, (tma_ctas_per_sm<D, MT>()))
+paged_rows_tma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Params p, const RowsArgs a, int* err) {
+    using F = Fold<D, MT, BF16>;
+    constexpr int STAGES = Cfg<D>::STAGES;
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* smem = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);      // the swizzle counts from 1024-byte lines
+    __shared__ uint64_t s_full[STAGES], s_empty[STAGES];
+    __shared__ float2 s_ml[64];
+    __shared__ volatile int s_abort;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t base = smem_u32(smem);
+    if (tid == 0) {
+        for (int i = 0; i < STAGES; ++i) { tc::mbar_init(&s_full[i], 1); tc::mbar_init(&s_empty[i], 4); }
+        s_abort = 0;
+        tc::mbar_init_fence();
+    }
+    griddep_wait();
+    griddep_launch();
+    scan_costs<KT>(p, (long long*)smem, err);
+    DeviceWalk<KT> walk{LoadReq{&p, nullptr}};
+    walk.init(p, (long long*)smem, blockIdx.x, gridDim.x);
+    tc::fence_async_smem();
+    __syncthreads();       // the prefix sums' memory becomes the tile ring
+    Seg s;
+    uint32_t u = 0;        // tiles so far: position in the ring
+
+    if (warp == 4) {
+        constexpr int COPIES = 2 * (D / 64);
+        const int box = lane / COPIES, slab = (lane % COPIES) >> 1, of_v = lane & 1;
+        const bool inner = of_v ? a.v_heads_inner : a.k_heads_inner;
+        const CUtensorMap* map = of_v ? &map_v : &map_k;
+        const int in_tile = box * a.box_rows;
+        const uint32_t to = base + of_v * Cfg<D>::TILE_BYTES + slab * (KT * 128) + in_tile * 128;
+        while (walk.next(p, s)) {
+            const int32_t* row = p.table + (int64_t)s.b * p.table_stride;
+            // -1 where no visible key lies in the box, n_pages (read as zeros) for a bad entry
+            auto page_of = [&](int j) {
+                const int key = j * KT + in_tile;
+                if (j >= s.je || in_tile >= KT || key >= s.hi || key + a.box_rows <= s.lo) return -1;
+                int page, in_page;
+                return locate(p, row, key, page, in_page, err) ? page : p.n_pages;
+            };
+            int page = page_of(s.jb), next = page_of(s.jb + 1);
+            for (int j = s.jb; j < s.je; ++j, ++u) {
+                const int after = page_of(j + 2);
+                const int st = u % STAGES;
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(&s_empty[st], ((u / STAGES) & 1) ^ 1, &s_abort, err, 26))) return;
+                const int key = j * KT + in_tile, in_page = p.page_shift >= 0 ? key & (p.page_size - 1) : key % p.page_size;
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, page >= 0)) * a.box_rows * 128;
+                if (lane == 0) tc::mbar_expect_tx(&s_full[st], bytes);
+                __syncwarp();
+                if (page >= 0) tma_load_4d(to + st * Cfg<D>::STAGE_BYTES, map, &s_full[st], slab * 64, inner ? s.hk : in_page, inner ? in_page : s.hk, page);
+                page = next; next = after;
             }
-            if (whole) {
-                const int tok = r / p.group, head = s.hk * p.group + r - tok * p.group;
-                const int64_t at = (int64_t)(s.r.q0 + block0 + tok) * p.q_heads + head;
-                const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;      // no visible key: zeros, and -inf for the log-sum-exp
-                *(uint2*)((uint16_t*)p.out + at * D + d) =
-                    make_uint2(pack2<BF16>(acc.x * inv, acc.y * inv), pack2<BF16>(acc.z * inv, acc.w * inv));
-                if (p.lse && d == 0) p.lse[at] = (m + log2f(l) - p_shift<BF16>()) * LN2;
-            } else {
-                *(float4*)(p.ws_o + (slot * p.rows + r) * D + d) = acc;
-                if (d == 0) p.ws_ml[slot * p.rows + r] = make_float2(m, l);
+        }
+        return;
+    }
+
+    F f;
+    f.place(warp, lane);
+    auto meet = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+    int4 merge = make_int4(0, 0, 0, 0);
+    const float sl2 = p.scale * LOG2E;
+    bool ok = true;        // a wait that ran out is not repeated; the barriers below are still met by every warp
+    while (walk.next(p, s)) {
+        const int block0 = s.rb * p.block_tokens;
+        const int n_tok = min(p.block_tokens, s.r.qn - block0);
+        f.begin(p, s, block0, n_tok);
+        uint32_t ks_addr = base;
+        for (int j = s.jb; j < s.je; ++j, ++u) {
+            const int st = u % STAGES;
+            if (ok) ok = tc::mbar_wait(&s_full[st], (u / STAGES) & 1, &s_abort, err, 27);
+            __syncwarp();
+            ks_addr = base + st * Cfg<D>::STAGE_BYTES;
+            const uint32_t vs_addr = ks_addr + Cfg<D>::TILE_BYTES;
+            const int tile_key = j * KT, first = tile_key + f.wk * F::KW;
+            if (first < s.lo || first + F::KW > s.hi) {
+                // rows of V outside the keys the item sees hold whatever the page does: zeros, where this warp reads
+                for (int i = lane; i < F::KW * (D / 8); i += 32) {
+                    const int r = i / (D / 8), c = i % (D / 8), rr = f.wk * F::KW + r;
+                    if (tile_key + rr < s.lo || tile_key + rr >= s.hi)
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(vs_addr + (c >> 3) * (KT * 128) + rr * 128 + (c & 7) * 16), "r"(0) : "memory");
+                }
+                tc::fence_async_smem();        // before a later copy into the stage
+                __syncwarp();
+            }
+            f.tile(ks_addr, vs_addr, tile_key, sl2);
+            __syncwarp();
+            if (lane == 0 && j + 1 < s.je) tc::mbar_arrive(&s_empty[st]);
+        }
+        // the last tile's stage takes the warps' carriers, then it goes back too
+        meet();
+        if (s.je > s.jb) {
+            f.finish(p, s, block0, n_tok, (float*)(smem + (ks_addr - base)), s_ml, tid, meet);
+            tc::fence_async_smem();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&s_empty[(u - 1) % STAGES]);
+        } else {                               // no key is visible: zeros, and -inf for the log-sum-exp
+            for (int i = tid; i < n_tok * p.group * (D / 4); i += 128) {
+                const int r = i / (D / 4), d = (i % (D / 4)) * 4, tok = r / p.group;
+                const int64_t at = (int64_t)(s.r.q0 + block0 + tok) * p.q_heads + s.hk * p.group + r - tok * p.group;
+                *(uint2*)((uint16_t*)p.out + at * D + d) = make_uint2(0, 0);
+                if (p.lse && d == 0) p.lse[at] = -INFINITY;
             }
         }
         if (s.parts > 1) merge = make_int4(s.r.q0 + block0, n_tok, s.hk, s.parts);
-        __syncthreads();
     }
     if (tid == 0) p.ws_merge[blockIdx.x] = merge;
 }
@@ -367,25 +513,38 @@ __global__ void __launch_bounds__(512) paged_merge_kernel(const __grid_constant_
 }
 
 template <int D, int MT, bool BF16>
-int32_t launch_rows(sanic_ctx* ctx, const Params& p, int ctas, cudaStream_t st) {
-    constexpr int merge_bytes = (4 / MT) * 16 * MT * (8 + (D + 4) * 4);
-    constexpr int smem = Cfg<D>::RING > merge_bytes ? Cfg<D>::RING : merge_bytes;
+int32_t launch_rows(sanic_ctx* ctx, const Params& p, bool tma, int ctas, cudaStream_t st) {
+    constexpr int smem = Cfg<D>::RING;
+    static_assert(4 * 16 * D * 4 <= Cfg<D>::STAGE_BYTES, "the warps' carriers fit a stage");
     static thread_local int ready_on = -1;       // the attribute is per device
     if (ready_on != ctx->device) {
         SANIC_CUDA_CHECK(ctx, cudaFuncSetAttribute(paged_rows_kernel<D, MT, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        SANIC_CUDA_CHECK(ctx, cudaFuncSetAttribute(paged_rows_tma_kernel<D, MT, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem + 1024));
         ready_on = ctx->device;
     }
-    SANIC_CUDA_CHECK(ctx, launch_pdl(paged_rows_kernel<D, MT, BF16>, dim3(ctas), dim3(128), smem, st, p, ctx->status_dev));
+    if (!tma) {
+        SANIC_CUDA_CHECK(ctx, launch_pdl(paged_rows_kernel<D, MT, BF16>, dim3(ctas), dim3(128), smem, st, p, ctx->status_dev));
+        return SANIC_OK;
+    }
+    CUtensorMap mk, mv;
+    RowsArgs a{};
+    a.box_rows = std::min(p.page_size, KT);
+    bool ki, vi;
+    int32_t rc = encode_pool(ctx, &mk, BF16, p, 0, D, a.box_rows, &ki);
+    if (rc == SANIC_OK) rc = encode_pool(ctx, &mv, BF16, p, 1, D, a.box_rows, &vi);
+    if (rc != SANIC_OK) return rc;
+    a.k_heads_inner = ki; a.v_heads_inner = vi;
+    SANIC_CUDA_CHECK(ctx, launch_pdl(paged_rows_tma_kernel<D, MT, BF16>, dim3(ctas), dim3(TMA_THREADS), smem + 1024, st, mk, mv, p, a, ctx->status_dev));
     return SANIC_OK;
 }
 template <int MT>
-int32_t launch_rows_any(sanic_ctx* ctx, const Params& p, int D, int dtype, int ctas, cudaStream_t st) {
-    if (D == 128) return dtype == SANIC_BF16 ? launch_rows<128, MT, true>(ctx, p, ctas, st) : launch_rows<128, MT, false>(ctx, p, ctas, st);
-    return dtype == SANIC_BF16 ? launch_rows<64, MT, true>(ctx, p, ctas, st) : launch_rows<64, MT, false>(ctx, p, ctas, st);
+int32_t launch_rows_any(sanic_ctx* ctx, const Params& p, int D, int dtype, bool tma, int ctas, cudaStream_t st) {
+    if (D == 128) return dtype == SANIC_BF16 ? launch_rows<128, MT, true>(ctx, p, tma, ctas, st) : launch_rows<128, MT, false>(ctx, p, tma, ctas, st);
+    return dtype == SANIC_BF16 ? launch_rows<64, MT, true>(ctx, p, tma, ctas, st) : launch_rows<64, MT, false>(ctx, p, tma, ctas, st);
 }
 
-// Resident CTAs of the rows kernel: two or three per SM, what its shared memory leaves (96 or 64 KB each).
-int rows_ctas(const sanic_ctx* ctx, int D) { return ctx->sm_count * (D == 128 ? 2 : 3); }
+// Resident CTAs of the rows form: what its shared memory (96 or 64 KB) and registers leave.
+int rows_ctas(const sanic_ctx* ctx, int D, int rows) { return ctx->sm_count * (D == 128 ? tma_ctas_per_sm<128, 1>() : rows == 16 ? tma_ctas_per_sm<64, 1>() : tma_ctas_per_sm<64, 2>()); }
 
 // Which forms serve a call: the rows form (`rows` query rows per item; 0: not launched) and the tensor-memory form (`tc`).
 struct Plan { int rows, rows_ctas; bool tc; int tc_ctas; };
@@ -394,7 +553,6 @@ Plan make_plan(const sanic_ctx* ctx, const sanic_attn_paged_params* p) {
     const int group = p->q_heads / p->kv_heads;
     const long long want = (long long)(p->max_query_len > 0 ? p->max_query_len : p->n_tokens) * group;
     Plan pl{};
-    pl.rows_ctas = rows_ctas(ctx, p->head_dim);
     pl.tc = want > TC_ABOVE_ROWS && tc_supported(p);
     if (pl.tc) {
         // A batch may hold single tokens beside its chunks: those are the rows form's, in a launch of their own (28 decodes beside
@@ -404,6 +562,7 @@ Plan make_plan(const sanic_ctx* ctx, const sanic_attn_paged_params* p) {
     } else {
         pl.rows = pow2_rows(want);
     }
+    pl.rows_ctas = rows_ctas(ctx, p->head_dim, pl.rows);
     return pl;
 }
 
@@ -490,9 +649,9 @@ int32_t sanic_attn_paged(sanic_ctx* ctx, const sanic_attn_paged_params* p, void*
         ws = place(q, ws, pl.rows_ctas, pl.rows, p->head_dim);
         q.block_tokens = pl.rows / q.group;
         if (pl.tc) { q.rows_upto = t.rows_above = pl.rows; t.beside = 1; }
-        rc = pl.rows == 16   ? launch_rows_any<1>(ctx, q, p->head_dim, p->dtype, pl.rows_ctas, st)
-             : pl.rows == 32 ? launch_rows_any<2>(ctx, q, p->head_dim, p->dtype, pl.rows_ctas, st)
-                             : launch_rows_any<4>(ctx, q, p->head_dim, p->dtype, pl.rows_ctas, st);
+        rc = pl.rows == 16   ? launch_rows_any<1>(ctx, q, p->head_dim, p->dtype, pool_supported(p, KT), pl.rows_ctas, st)
+             : pl.rows == 32 ? launch_rows_any<2>(ctx, q, p->head_dim, p->dtype, pool_supported(p, KT), pl.rows_ctas, st)
+                             : launch_rows_any<4>(ctx, q, p->head_dim, p->dtype, pool_supported(p, KT), pl.rows_ctas, st);
         if (rc != SANIC_OK) return rc;
     }
     if (pl.tc) {

@@ -23,8 +23,7 @@
 // per clock and SM): equal at head_dim 128, SFU-bound at 64.
 #include <algorithm>
 
-#include "paged.cuh"
-#include "tc_common.cuh"
+#include "paged_tma.cuh"
 
 namespace {
 using namespace sanic;
@@ -92,14 +91,6 @@ __device__ __forceinline__ bool elect_one() {
     uint32_t pred;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
     return pred != 0;
-}
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-                 ::"r"(dst), "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
-}
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-                 ::"r"(dst), "l"((uint64_t)map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 // Bounded wait of a role that is ahead of the others: asks and sleeps, and leaves the issue slots of its sub-partition to the
 // softmax warps (a suspended try_wait wakes and asks again often enough to cost them a tenth of their rate).
@@ -589,38 +580,6 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     if (p.beside) griddep_wait();
 }
 
-// Row-major view of rank 3 or 4, 128-byte swizzle, zero fill out of bounds; strides in elements of 2 bytes, dims innermost first.
-int32_t encode(sanic_ctx* ctx, CUtensorMap* map, bool bf16, const void* ptr, int rank, const cuuint64_t* dims, const int64_t* strides,
-               const cuuint32_t* box) {
-    if (!ctx->encode_tiled) {
-        void* fn = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
-        if (e != cudaSuccess || !fn) return sanic_fail(ctx, SANIC_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-        ctx->encode_tiled = fn;
-    }
-    cuuint64_t st[3];
-    for (int i = 0; i + 1 < rank; ++i) st[i] = (cuuint64_t)strides[i] * 2;
-    const cuuint32_t ones[4] = {1, 1, 1, 1};
-    const CUresult r = ((encode_tiled_fn)ctx->encode_tiled)(
-        map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, (cuuint32_t)rank, const_cast<void*>(ptr), dims, st, box, ones,
-        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return sanic_fail(ctx, SANIC_ERR_CUDA, "attn_paged: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
-    return SANIC_OK;
-}
-
-// Strides of a pool as the tensor map wants them: (heads, rows) ordered by stride, every stride a multiple of the one before.
-struct Pool { int64_t inner, outer; bool heads_inner; };
-bool pool_of(int64_t page, int64_t row, int64_t head, int n_pages, int page_size, int heads, int d, Pool* out) {
-    if (heads == 1) head = d;              // a single head's stride is never used
-    if (page_size == 1) row = d;
-    const bool hi = head <= row;
-    const int64_t in = hi ? head : row, o = hi ? row : head;
-    if (n_pages == 1) page = o * (hi ? page_size : heads);
-    *out = Pool{in, o, hi};
-    return in >= d && o % in == 0 && page % o == 0 && page >= o && page < (1ll << 38);
-}
-
 template <int D, bool BF16>
 int32_t launch(sanic_ctx* ctx, const Params& p, int ctas, cudaStream_t st) {
     using C = Tc<D>;
@@ -632,21 +591,14 @@ int32_t launch(sanic_ctx* ctx, const Params& p, int ctas, cudaStream_t st) {
         const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)p.q_heads, (cuuint64_t)p.n_tokens};
         const int64_t strides[2] = {p.q_heads == 1 ? D : p.q_head_stride, p.q_token_stride};
         const cuuint32_t box[3] = {64, (cuuint32_t)p.group, (cuuint32_t)a.tile_tokens};
-        const int32_t rc = encode(ctx, &mq, BF16, p.q, 3, dims, strides, box);
+        const int32_t rc = encode_map(ctx, &mq, BF16, p.q, 3, dims, strides, box);
         if (rc != SANIC_OK) return rc;
     }
     for (int kv = 0; kv < 2; ++kv) {
-        Pool pool;
-        pool_of(kv ? p.v_page_stride : p.k_page_stride, kv ? p.v_row_stride : p.k_row_stride, kv ? p.v_head_stride : p.k_head_stride, p.n_pages,
-                p.page_size, p.kv_heads, D, &pool);
-        const cuuint64_t hd = p.kv_heads, rd = p.page_size;
-        const cuuint64_t dims[4] = {(cuuint64_t)D, pool.heads_inner ? hd : rd, pool.heads_inner ? rd : hd, (cuuint64_t)p.n_pages};
-        const int64_t strides[3] = {pool.inner, pool.outer, p.n_pages == 1 ? pool.outer * (int64_t)dims[2] : (kv ? p.v_page_stride : p.k_page_stride)};
-        const cuuint32_t br = a.box_rows;
-        const cuuint32_t box[4] = {64, pool.heads_inner ? 1u : br, pool.heads_inner ? br : 1u, 1};
-        const int32_t rc = encode(ctx, kv ? &mv : &mk, BF16, kv ? p.v : p.k, 4, dims, strides, box);
+        bool inner;
+        const int32_t rc = encode_pool(ctx, kv ? &mv : &mk, BF16, p, kv, D, a.box_rows, &inner);
         if (rc != SANIC_OK) return rc;
-        (kv ? a.v_heads_inner : a.k_heads_inner) = pool.heads_inner;
+        (kv ? a.v_heads_inner : a.k_heads_inner) = inner;
     }
     const int smem = C::DATA + (int)sizeof(Shared<D>) + 1024;
     static_assert(C::NS * C::TILE >= (MAX_REQUESTS + 1) * 8, "prefix sums fit the ring");
@@ -662,14 +614,9 @@ int32_t launch(sanic_ctx* ctx, const Params& p, int ctas, cudaStream_t st) {
 
 namespace sanic {
 namespace paged {
-// TMA boxes are whole pages of 8, 16, 32, 64 or 128 rows, or 128 rows of pages that are a multiple of 128; strides nest. Other
-// layouts are served by the rows form.
+// The page pool as TMA needs it, and the heads of a group side by side within a token. Other layouts are served by the rows form.
 bool tc_supported(const sanic_attn_paged_params* p) {
-    const int ps = p->page_size;
-    if (!(ps % 128 == 0 || ps == 8 || ps == 16 || ps == 32 || ps == 64)) return false;
-    Pool pool;
-    if (!pool_of(p->k_page_stride, p->k_row_stride, p->k_head_stride, p->n_pages, ps, p->kv_heads, p->head_dim, &pool)) return false;
-    if (!pool_of(p->v_page_stride, p->v_row_stride, p->v_head_stride, p->n_pages, ps, p->kv_heads, p->head_dim, &pool)) return false;
+    if (!pool_supported(p, BN)) return false;
     const int64_t hs = p->q_heads == 1 ? p->head_dim : p->q_head_stride;
     return hs >= p->head_dim && (p->n_tokens == 1 || (p->q_token_stride % hs == 0 && p->q_token_stride >= hs)) && p->q_token_stride < (1ll << 38) && p->q_token_stride > 0;
 }
