@@ -27,6 +27,9 @@ class RunError(Exception):
 _TORCH_DTYPE = {abi.F32: torch.float32, abi.BF16: torch.bfloat16, abi.F16: torch.float16}
 
 
+_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _ptr(t):
     return C.c_void_p(t.data_ptr()) if t is not None else None
 
@@ -79,7 +82,9 @@ class CudaDevice:
         raise RunError(f"{what}: status {rc}: {msg}")
 
     def stream(self):
-        return C.c_void_p(torch.cuda.current_stream(self.torch_device).cuda_stream)
+        # the handle itself where torch gives it (0.1 us; the stream object around it costs 2 us, which a small call feels)
+        raw = _RAW_STREAM(self.ordinal) if _RAW_STREAM else torch.cuda.current_stream(self.torch_device).cuda_stream
+        return C.c_void_p(raw)
 
     def sync(self):
         """Wait for the current stream and surface any device-side status (bounded waits that ran out)."""
@@ -397,27 +402,30 @@ class CudaDevice:
         return out
 
     # ── serving over a paged cache ──
-    def _paged(self, name, t, dtypes, rank):
-        """A tensor of this device with one of `dtypes`, dense along its last axis; any strides before it."""
+    def _refuse(self, name, t, dtypes, rank=None, n=None):
         if not isinstance(t, torch.Tensor) or t.get_device() != self.ordinal:
             raise RunError(f"input `{name}` is not a tensor on {self.torch_device}")
         if t.dtype not in dtypes:
             raise RunError(f"input `{name}` has dtype {t.dtype}; expected {' or '.join(map(str, dtypes))}")
+        if rank is None:
+            raise RunError(f"input `{name}` must hold {n} contiguous elements; its shape is {tuple(t.shape)}")
         if t.dim() != rank:
             raise RunError(f"input `{name}` has {t.dim()} axes; expected {rank}")
-        st = t.stride()
-        if st[-1] != 1 and t.shape[-1] > 1 and t.numel():
-            raise RunError(f"input `{name}` must be contiguous along its last axis")
-        return st
+        raise RunError(f"input `{name}` must be contiguous along its last axis")
+
+    def _paged(self, name, t, dtypes, rank):
+        """Strides of a tensor of this device with one of `dtypes`, dense along its last axis; any strides before it."""
+        if isinstance(t, torch.Tensor) and t.get_device() == self.ordinal and t.dtype in dtypes and t.dim() == rank:
+            st = t.stride()
+            if st[-1] == 1 or t.shape[-1] <= 1 or not t.numel():
+                return st
+        self._refuse(name, t, dtypes, rank=rank)
 
     def _flat(self, name, t, dtype, n):
-        if not isinstance(t, torch.Tensor) or t.get_device() != self.ordinal:
-            raise RunError(f"input `{name}` is not a tensor on {self.torch_device}")
-        if t.dtype != dtype:
-            raise RunError(f"input `{name}` has dtype {t.dtype}; expected {dtype}")
-        if t.numel() != n or not t.is_contiguous():
-            raise RunError(f"input `{name}` must hold {n} contiguous elements; its shape is {tuple(t.shape)}")
-        return t.data_ptr()
+        """Address of `n` contiguous elements of this device."""
+        if isinstance(t, torch.Tensor) and t.get_device() == self.ordinal and t.dtype == dtype and t.numel() == n and t.is_contiguous():
+            return t.data_ptr()
+        self._refuse(name, t, (dtype,), n=n)
 
     def page_table_append(self, seq_lens, new_lens, block_table, free_pages, free_count, page_size, n_tokens, held_pages=None):
         """Page tables, slots and positions of one step from the requests' lengths: request b (seq_lens[b] tokens held in
@@ -433,19 +441,17 @@ class CudaDevice:
         n_tokens = int(n_tokens)
         if n_tokens < 0:
             raise RunError("n_tokens must not be negative")
-        # one allocation for the five int32 outputs, each 16-byte aligned
-        pad = lambda k: (k + 3) // 4 * 4
-        a, b, c = pad(n + 1), pad(n), pad(n_tokens)
-        ints = torch.empty(a + 2 * b + 4 + c, dtype=i32, device=self.torch_device)
-        out = PageStep(ints[:n + 1], ints[a:a + n], ints[a + b:a + b + n], ints[a + 2 * b:a + 2 * b + 1],
-                       ints[a + 2 * b + 4:a + 2 * b + 4 + n_tokens], torch.empty(n_tokens, dtype=torch.int64, device=self.torch_device))
-        base = ints.data_ptr()
+        # one allocation for all outputs: an allocation or a view costs more host time than the kernel takes
+        block = seq_lens.new_empty(3 * n_tokens + 3 * n + 2, dtype=i32)
+        slots, start, kv, held, count, pos = block.split_with_sizes((2 * n_tokens, n + 1, n, n, 1, n_tokens))
+        out = PageStep(start, kv, held, count, pos, slots.view(torch.int64))
+        base = block.data_ptr()
+        at = base + 8 * n_tokens
         p = abi.PageAppendParams(
             self._flat("seq_lens", seq_lens, i32, n), self._flat("new_lens", new_lens, i32, n),
             None if held_pages is None else self._flat("held_pages", held_pages, i32, n),
             self._flat("free_pages", free_pages, i32, free_pages.numel()), self._flat("free_count", free_count, i32, 1),
-            block_table.data_ptr(), st[0], base, base + 4 * a, base + 4 * (a + b), base + 4 * (a + 2 * b), base + 4 * (a + 2 * b + 4),
-            out.slots.data_ptr(), n, n_tokens, int(page_size), block_table.shape[1], free_pages.numel())
+            block_table.data_ptr(), st[0], at, at + 4 * n + 4, at + 8 * n + 4, at + 12 * n + 4, at + 12 * n + 8, base, n, n_tokens, int(page_size), block_table.shape[1], free_pages.numel())
         self._check(self.lib.sanic_page_table_append(self.h, C.byref(p), self.stream()), "page_table_append")
         return out
 
@@ -481,7 +487,7 @@ class CudaDevice:
             hq = q.shape[1]
             qst = self._token_rows("q", q, src, t, hq, d)
             if q_out is None:
-                q_out = torch.empty((t, hq, d), dtype=k_pages.dtype, device=self.torch_device)
+                q_out = q.new_empty((t, hq, d), dtype=k_pages.dtype)
             qost = self._token_rows("q_out", q_out, k_pages.dtype, t, hq, d)
         elif q_out is not None:
             raise RunError("q_out needs q")
@@ -518,9 +524,11 @@ class CudaDevice:
         if dk != d or q.dtype != k_pages.dtype:
             raise RunError(f"attention shapes disagree: q {tuple(q.shape)} {q.dtype}, pages {tuple(k_pages.shape)} {k_pages.dtype}")
         if out is None:
-            out = torch.empty((T, hq, d), dtype=q.dtype, device=self.torch_device)
-        out_ptr = self._flat("out", out, q.dtype, T * hq * d)
-        lse = torch.empty((T, hq), dtype=torch.float32, device=self.torch_device) if return_lse else None
+            out = q.new_empty((T, hq, d))
+            out_ptr = out.data_ptr()
+        else:
+            out_ptr = self._flat("out", out, q.dtype, T * hq * d)
+        lse = q.new_empty((T, hq), dtype=torch.float32) if return_lse else None
         p = abi.AttnPagedParams(
             q.data_ptr(), out_ptr, lse.data_ptr() if return_lse else None, k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
             self._flat("query_start", query_start, torch.int32, n + 1), self._flat("kv_lens", kv_lens, torch.int32, n), None, 0,
@@ -528,7 +536,7 @@ class CudaDevice:
             n_pages, max_pages, int(window), float(scale) if scale is not None else 1.0 / math.sqrt(d))
         # a workspace per call: calls on other streams, and graphs that replay side by side, never share one
         nbytes = self.lib.sanic_attn_paged_workspace_bytes(self.h, C.byref(p))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.torch_device)
+        ws = kv_lens.new_empty(nbytes // 4)
         p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
         self._check(self.lib.sanic_attn_paged(self.h, C.byref(p), self.stream()), "attn_paged")
         return (out, lse) if return_lse else out
@@ -549,8 +557,8 @@ class CudaDevice:
             if tuple(draft_probs.shape) != (n, k, vocab):
                 raise RunError(f"input `draft_probs` has shape {tuple(draft_probs.shape)}; expected {(n, k, vocab)}")
         i32, f32 = torch.int32, torch.float32
-        out = torch.empty((n, k + 1), dtype=i32, device=self.torch_device)
-        accepted = torch.empty(n, dtype=i32, device=self.torch_device)
+        out = draft_tokens.new_empty((n, k + 1), dtype=i32)
+        accepted = u_sample.new_empty(n, dtype=i32)
         p = abi.DraftVerifyParams(
             target_probs.data_ptr(), ts[0], rows, None if target_start is None else self._flat("target_start", target_start, i32, n),
             None if draft_probs is None or not k else draft_probs.data_ptr(), ds[0], ds[1], self._flat("draft_tokens", draft_tokens, i32, n * k) or None,

@@ -6,10 +6,11 @@
 // Only one row of p (and of q after a rejection) is read per request: which one is known after at most max_draft gathered
 // pairs, which one warp takes at once. HBM bounds a batch (4 or 8 bytes per vocabulary entry); a single request is a chain of
 // latencies: lengths and tokens, their probabilities, the row, the join. One cluster of CTAs serves a request: each CTA sums
-// its slice of the row, the slices' totals are exchanged through distributed shared memory, and the CTA that holds the drawn
-// token finds it from the sums of 128-entry chunks that it kept, so that only one chunk is read twice. No workspace, no atomics:
-// the sums have a fixed order for a given cluster size. They are f64: a running sum in f32 would put the border of about one
-// entry in a thousand on its other side at a vocabulary of 1e5.
+// its slice of the row in groups of 1024 entries, the slices' totals are exchanged through distributed shared memory, and the
+// CTA that holds the drawn token finds its group from the sums that it kept, so that only one group is read twice. No
+// workspace, no atomics: the sums have a fixed order for a given cluster size. They are f64 (a running sum in f32 would put
+// the border of about one entry in a thousand on its other side at a vocabulary of 1e5), with one reduction over the lanes per
+// group: a 64-bit butterfly costs as much as reading 512 entries.
 #include <cooperative_groups.h>
 
 #include "paged.cuh"
@@ -18,48 +19,51 @@ namespace {
 using namespace sanic;
 namespace cg = cooperative_groups;
 
-constexpr int THREADS = 512, WARPS = THREADS / 32;
-constexpr int CHUNK = 128;                        // entries of a warp's step
-constexpr int STEP = WARPS * CHUNK;               // entries of a block's step
-constexpr int MAX_STEPS = 256;                    // per CTA: 2^19 entries
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int CHUNK = 128, PER_GROUP = 8, GROUP = CHUNK * PER_GROUP;      // entries of a warp's load, loads of a group
+constexpr int MAX_GROUPS = 512;                   // of a CTA: 2^19 entries
 constexpr int MAX_CLUSTER = 16;
 
 enum { FROM_TARGET = 0, FROM_DIFFERENCE = 1, WITHOUT_TOKEN = 2 };
 
 struct Row { const float* p; const float* q; int mode, token; bool vec; };
 
+// The weight of entry j. NaN, infinities and weights that are not positive count as 0: p - q > 0 exactly where p > q.
 __device__ __forceinline__ double weight(float p, float q, const Row& r, int j) {
-    double w = r.mode == FROM_DIFFERENCE ? (double)p - (double)q : (double)p;
-    if (r.mode == WITHOUT_TOKEN && j == r.token) w = 0.0;
-    return w > 0.0 && w <= 3.402823466e38 ? w : 0.0;      // NaN, infinities and negative values count as 0
+    const bool counts = p > q && p <= 3.402823466e38f && q >= -3.402823466e38f && !(r.mode == WITHOUT_TOKEN && j == r.token);
+    return counts ? (double)p - (double)q : 0.0;
 }
-
-// sum over one warp chunk of entries [c, c + 128) below `end`; all lanes receive it
-__device__ __forceinline__ double chunk_sum(const Row& r, int c, int end, int lane) {
-    float p[4], q[4];
-    const bool full = c + CHUNK <= end;
-    if (full && r.vec) {
+// A lane's four entries of the chunk at c: neighbours where the rows start on 16-byte boundaries, else 32 apart.
+__device__ __forceinline__ int entry(const Row& r, int c, int lane, int i) { return r.vec ? c + lane * 4 + i : c + i * 32 + lane; }
+__device__ __forceinline__ void load4(const Row& r, int c, int end, int lane, float (&p)[4], float (&q)[4]) {
+    if (r.vec && c + CHUNK <= end) {
         const float4 a = __ldcs((const float4*)(r.p + c + lane * 4));
         p[0] = a.x; p[1] = a.y; p[2] = a.z; p[3] = a.w;
         if (r.mode == FROM_DIFFERENCE) {
             const float4 b = __ldcs((const float4*)(r.q + c + lane * 4));
             q[0] = b.x; q[1] = b.y; q[2] = b.z; q[3] = b.w;
         } else q[0] = q[1] = q[2] = q[3] = 0.0f;
-        double s = 0.0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s += weight(p[i], q[i], r, c + lane * 4 + i);
-        return s;
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int j = entry(r, c, lane, i);
+        p[i] = j < end ? __ldcs(r.p + j) : 0.0f;
+        q[i] = j < end && r.mode == FROM_DIFFERENCE ? __ldcs(r.q + j) : 0.0f;
+    }
+}
+__device__ __forceinline__ double group_sum(const Row& r, int g, int end, int lane) {      // this lane's part
     double s = 0.0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {                          // rows that start off a 16-byte boundary: lanes side by side
-        const int j = c + i * 32 + lane;
-        const bool in = j < end;
-        p[i] = in ? __ldcs(r.p + j) : 0.0f;
-        q[i] = in && r.mode == FROM_DIFFERENCE ? __ldcs(r.q + j) : 0.0f;
-    }
+    for (int h = 0; h < 2; ++h) {                 // four loads of p and of q in flight
+        float p[PER_GROUP / 2][4], q[PER_GROUP / 2][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s += weight(p[i], q[i], r, c + i * 32 + lane);
+        for (int k = 0; k < PER_GROUP / 2; ++k) load4(r, g * GROUP + (h * PER_GROUP / 2 + k) * CHUNK, end, lane, p[k], q[k]);
+#pragma unroll
+        for (int k = 0; k < PER_GROUP / 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s += weight(p[k][i], q[k][i], r, entry(r, g * GROUP + (h * PER_GROUP / 2 + k) * CHUNK, lane, i));
+    }
     return s;
 }
 __device__ __forceinline__ double warp_sum64(double v) {
@@ -73,33 +77,37 @@ __device__ __forceinline__ double warp_scan64(double v, int lane) {     // inclu
     return v;
 }
 
-__global__ void __launch_bounds__(THREADS) draft_verify_kernel(const sanic_draft_verify_params p, int* err) {
+__global__ void __launch_bounds__(THREADS, 4) draft_verify_kernel(const sanic_draft_verify_params p, int* err) {
     cg::cluster_group cluster = cg::this_cluster();
     const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int b = blockIdx.x / cs;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    __shared__ double s_sum[MAX_STEPS * WARPS];       // per warp chunk: its sum, then the sum of all chunks up to it
+    __shared__ double s_sum[MAX_GROUPS];              // per group: its sum, then the sum of all groups of this CTA up to it
     __shared__ double s_total;
     __shared__ int s_count, s_len, s_start, s_token;
+    __shared__ float s_u;
     griddep_wait();
     griddep_launch();
 
     if (warp == 0) {
         const int K = p.max_draft;
+        // everything that no other load decides is asked for together
         int len = p.draft_lens ? p.draft_lens[b] : K;
-        int start = p.target_start ? p.target_start[b] : b * (K + 1);
+        const int start = p.target_start ? p.target_start[b] : b * (K + 1);
+        int tok = lane < K ? p.draft_tokens[(int64_t)b * K + lane] : -1;
+        const float u = lane < K ? p.u_accept[(int64_t)b * K + lane] : 0.0f;
+        if (lane == 0) s_u = p.u_sample[b];
         bool bad = len < 0 || len > K;
         len = min(max(len, 0), K);
         const bool no_rows = start < 0 || (long long)start + len >= p.target_rows;
         bad |= no_rows;
         bool ok = false;
-        int tok = -1;
+        if (lane >= len) tok = -1;
         if (lane < len && !no_rows) {
-            tok = p.draft_tokens[(int64_t)b * K + lane];
             if ((unsigned)tok < (unsigned)p.vocab) {
                 const float pt = p.target_probs[(int64_t)(start + lane) * p.target_stride + tok];
                 const float qt = p.draft_probs ? p.draft_probs[(int64_t)b * p.draft_request_stride + (int64_t)lane * p.draft_stride + tok] : 1.0f;
-                ok = (double)p.u_accept[(int64_t)b * K + lane] * (double)qt < (double)pt;
+                ok = (double)u * (double)qt < (double)pt;
             } else bad = true;
         }
         const unsigned failed = ~__ballot_sync(0xffffffffu, ok);      // lanes past the drafts are among them
@@ -125,82 +133,94 @@ __global__ void __launch_bounds__(THREADS) draft_verify_kernel(const sanic_draft
     row.token = s_token;
     row.mode = !rejected ? FROM_TARGET : (p.draft_probs ? FROM_DIFFERENCE : WITHOUT_TOKEN);
 
-    // this CTA's slice: whole block steps
-    const int steps_all = (p.vocab + STEP - 1) / STEP;
-    const int st0 = (int)((long long)steps_all * rank / cs), st1 = (int)((long long)steps_all * (rank + 1) / cs);
-    const int n_chunks = (st1 - st0) * WARPS;
-    double total = 0.0, base = 0.0;
+    // this CTA's slice: whole groups
+    const int groups_all = (p.vocab + GROUP - 1) / GROUP;
+    const int g0 = (int)((long long)groups_all * rank / cs), g1 = (int)((long long)groups_all * (rank + 1) / cs);
+    const int n_groups = g1 - g0;
+    double total = 0.0, upto = 0.0;
     while (true) {
         row.vec = ((uintptr_t)row.p % 16) == 0 && (row.mode != FROM_DIFFERENCE || ((uintptr_t)row.q % 16) == 0);
-#pragma unroll 4
-        for (int st = st0; st < st1; ++st) {
-            const int c = st * STEP + warp * CHUNK;
-            double v = c < p.vocab ? chunk_sum(row, c, p.vocab, lane) : 0.0;
-            v = warp_sum64(v);
-            if (lane == 0) s_sum[(st - st0) * WARPS + warp] = v;
+        for (int g = g0 + warp; g < g1; g += WARPS) {
+            const double v = warp_sum64(group_sum(row, g, p.vocab, lane));
+            if (lane == 0) s_sum[g - g0] = v;
         }
         __syncthreads();
-        if (warp == 0) {                              // running sums over the chunks
+        if (warp == 0) {                              // running sums over the groups
             double carry = 0.0;
-            for (int i = 0; i < n_chunks; i += 32) {
-                double v = warp_scan64(i + lane < n_chunks ? s_sum[i + lane] : 0.0, lane) + carry;
-                if (i + lane < n_chunks) s_sum[i + lane] = v;
+            for (int i = 0; i < n_groups; i += 32) {
+                double v = warp_scan64(i + lane < n_groups ? s_sum[i + lane] : 0.0, lane) + carry;
+                if (i + lane < n_groups) s_sum[i + lane] = v;
                 carry = __shfl_sync(0xffffffffu, v, 31);
             }
             if (lane == 0) s_total = carry;
         }
         cluster.sync();
-        total = 0.0;
-        for (int r = 0; r < cs; ++r) {
-            if (r == rank) base = total;
-            total += *cluster.map_shared_rank(&s_total, r);
-        }
+        // every warp takes the slices' running sums: a lane per CTA of the cluster
+        upto = warp_scan64(lane < cs ? *cluster.map_shared_rank(&s_total, lane) : 0.0, lane);
+        total = __shfl_sync(0xffffffffu, upto, 31);
         const bool again = !(total > 0.0) && row.mode != FROM_TARGET;
         if (!again) break;
         row.mode = FROM_TARGET;                       // nothing left of p - q: p itself
         cluster.sync();                               // the totals are read before they are written again
     }
-    const double x = (double)p.u_sample[b] * total;
+    const double x = (double)s_u * total;
     // the owner: the first CTA whose running sum exceeds x; the last one with any weight if rounding left none
-    int owner = -1, last = -1;
-    double run = 0.0;
-    for (int r = 0; r < cs; ++r) {
-        const double mine = *cluster.map_shared_rank(&s_total, r);
-        run += mine;
-        if (mine > 0.0) last = r;
-        if (owner < 0 && run > x) owner = r;
-    }
-    if (owner < 0) owner = last;
+    const double before_me = __shfl_up_sync(0xffffffffu, upto, 1);
+    const unsigned over = __ballot_sync(0xffffffffu, lane < cs && upto > x);
+    const unsigned any = __ballot_sync(0xffffffffu, lane < cs && upto > (lane > 0 ? before_me : 0.0));
+    const int owner = over ? __ffs(over) - 1 : any ? 31 - __clz(any) : -1;
+    const double base = rank > 0 ? __shfl_sync(0xffffffffu, upto, max(rank - 1, 0)) : 0.0;
     int32_t* drawn = p.tokens_out + (int64_t)b * (p.max_draft + 1) + count;
     if (owner < 0) { if (rank == 0 && tid == 0) *drawn = -1; }
     else if (rank == owner && warp == 0) {
-        int chunk = -1, final_chunk = 0;
-        for (int i = 0; i < n_chunks && chunk < 0; i += 32) {
-            const bool in = i + lane < n_chunks;
+        int group = -1, final_group = 0;
+        for (int i = 0; i < n_groups && group < 0; i += 32) {
+            const bool in = i + lane < n_groups;
             const double v = in ? s_sum[i + lane] : 0.0, before = in && i + lane > 0 ? s_sum[i + lane - 1] : 0.0;
             const unsigned over = __ballot_sync(0xffffffffu, in && base + v > x), some = __ballot_sync(0xffffffffu, in && v > before);
-            if (over) chunk = i + __ffs(over) - 1;
-            if (some) final_chunk = i + 31 - __clz(some);
+            if (over) group = i + __ffs(over) - 1;
+            if (some) final_group = i + 31 - __clz(some);
         }
-        if (chunk < 0) chunk = final_chunk;
-        const int c = st0 * STEP + chunk * CHUNK;
-        double w[4], own = 0.0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int j = c + lane * 4 + i;
-            w[i] = j < p.vocab ? weight(row.p[j], row.mode == FROM_DIFFERENCE ? row.q[j] : 0.0f, row, j) : 0.0;
-            own += w[i];
-        }
-        double acc = base + (chunk > 0 ? s_sum[chunk - 1] : 0.0) + (warp_scan64(own, lane) - own);
+        if (group < 0) group = final_group;
+        // the group's chunks: their sums first, then the entries of the one that crosses x
+        const int c0 = (g0 + group) * GROUP;
+        row.vec = true;                               // a lane's entries are neighbours here, whatever the alignment
+        double acc = base + (group > 0 ? s_sum[group - 1] : 0.0);
         int hit = -1, positive = -1;
+        unsigned hits = 0;
+        for (int half = 0; half < 2; ++half) {
+            float w_p[PER_GROUP / 2][4], w_q[PER_GROUP / 2][4];
+            const int ch = c0 + half * (GROUP / 2);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            acc += w[i];
-            if (w[i] > 0.0) { positive = c + lane * 4 + i; if (hit < 0 && acc > x) hit = positive; }
+            for (int k = 0; k < PER_GROUP / 2; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = ch + k * CHUNK + lane * 4 + i;
+                    w_p[k][i] = j < p.vocab ? row.p[j] : 0.0f;
+                    w_q[k][i] = j < p.vocab && row.mode == FROM_DIFFERENCE ? row.q[j] : 0.0f;
+                }
+#pragma unroll
+            for (int k = 0; k < PER_GROUP / 2; ++k) {
+                double w[4], own = 0.0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { w[i] = weight(w_p[k][i], w_q[k][i], row, ch + k * CHUNK + lane * 4 + i); own += w[i]; }
+                const double scan = warp_scan64(own, lane);
+                double at = acc + (scan - own);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    at += w[i];
+                    if (w[i] > 0.0 && !hits) { positive = ch + k * CHUNK + lane * 4 + i; if (hit < 0 && at > x) hit = positive; }
+                }
+                if (!hits) hits = __ballot_sync(0xffffffffu, hit >= 0);      // the first chunk with a crossing; in it, the first lane
+                acc += __shfl_sync(0xffffffffu, scan, 31);
+            }
         }
-        const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), pos = __ballot_sync(0xffffffffu, positive >= 0);
-        const int from = hits ? __ffs(hits) - 1 : (pos ? 31 - __clz(pos) : 0);
-        const int token = __shfl_sync(0xffffffffu, hits ? hit : positive, from);
+        if (!hits) {                                  // rounding left no crossing: the last entry with a weight
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) positive = max(positive, __shfl_xor_sync(0xffffffffu, positive, o));
+            hit = positive; hits = 1;
+        }
+        const int token = __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
         if (lane == 0) *drawn = token;
     }
     cluster.sync();                                   // no CTA leaves while another may read its total
@@ -219,10 +239,10 @@ extern "C" int32_t sanic_draft_verify(sanic_ctx* ctx, const sanic_draft_verify_p
     SANIC_REQUIRE(ctx, !p->draft_probs || (p->draft_stride >= p->vocab && p->draft_request_stride >= 0), "draft_verify: draft rows overlap");
     sanic_set_device(ctx);
     // CTAs per request: enough that the batch covers four blocks per SM, at most 16 (a cluster's limit) and never less than a
-    // block step each
-    const int steps = (p->vocab + STEP - 1) / STEP;
+    // group each (64 requests of 128256 entries: 8 each 21 us, 16 each 34 us, 4 each 23 us; one request: 16 10.6 us, 8 13.1 us)
+    const int groups = (p->vocab + GROUP - 1) / GROUP;
     int cs = 1;
-    while (cs < MAX_CLUSTER && 2 * cs * (long long)p->n_requests <= 4ll * ctx->sm_count && 2 * cs <= steps) cs *= 2;
+    while (cs < MAX_CLUSTER && 2 * cs * (long long)p->n_requests <= 4ll * ctx->sm_count && 2 * cs <= groups) cs *= 2;
     static thread_local int ready_on = -1;
     if (ready_on != ctx->device) {
         SANIC_CUDA_CHECK(ctx, cudaFuncSetAttribute(draft_verify_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
