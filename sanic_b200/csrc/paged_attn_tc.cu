@@ -381,7 +381,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             const bool busy = __any_sync(0xffffffffu, valid);      // a warp without rows only keeps the barriers' count
             for (int j = s.jb; j < s.je && ok; ++j, ++n_it) {
                 const bool first = j == s.jb;
-                if (!scores_ready) ok = mbar_wait_spin(&sh->s_full[t], n_it & 1, abortp, err, 21);
+                if (!scores_ready) ok = mbar_wait(&sh->s_full[t], n_it & 1, abortp, err, 21);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 scores_ready = false;
@@ -409,9 +409,19 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh->s_free[t]);        // S is in registers
                 }
-                if (edge) {
+                if (edge) {        // 32 columns at a time, where an edge of some row's is
+                    const int hi = khi - k0, lo = klo - k0;
 #pragma unroll
-                    for (int i = 0; i < BN; ++i) { const int kk = k0 + i; if (!(kk >= klo && kk < khi)) r[i] = 0xFF800000u; }  // -inf
+                    for (int c = 0; c < BN; c += 32) {
+                        if (k0 + c + 32 <= inner_hi && k0 + c >= inner_lo) continue;
+                        if (p.window > 0) {
+#pragma unroll
+                            for (int i = c; i < c + 32; ++i) if (!(i >= lo && i < hi)) r[i] = 0xFF800000u;      // -inf
+                        } else {
+#pragma unroll
+                            for (int i = c; i < c + 32; ++i) if (!(i < hi)) r[i] = 0xFF800000u;
+                        }
+                    }
                 }
                 const bool spec = !first;
                 float mxs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -532,20 +542,22 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     for (int i = 0; i < D; ++i) o[i] = 0u;                   // every weight of the row was 0: V's zero rows and NaN alike
                 }
 #pragma unroll
-                for (int q = 0; q < D / 8; ++q) {
-                    uint32_t wv[4];
+                for (int q = 0; q < D / 16; ++q) {
+                    uint32_t wv[8];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        wv[j] = pack2<BF16>(__uint_as_float(o[8 * q + 2 * j]) * inv, __uint_as_float(o[8 * q + 2 * j + 1]) * inv);
-                    *(uint4*)(dst + q * 8) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
+                    for (int j = 0; j < 8; ++j)
+                        wv[j] = pack2<BF16>(__uint_as_float(o[16 * q + 2 * j]) * inv, __uint_as_float(o[16 * q + 2 * j + 1]) * inv);
+                    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + q * 16), "r"(wv[0]), "r"(wv[1]),
+                                 "r"(wv[2]), "r"(wv[3]), "r"(wv[4]), "r"(wv[5]), "r"(wv[6]), "r"(wv[7]) : "memory");
                 }
                 if (p.lse) p.lse[at] = (m + log2f(l) - P_SHIFT) * LN2;
             } else {
                 const size_t r = (size_t)s.slot * p.rows + t * tile_rows + row;
-                float4* dst = (float4*)(p.ws_o + r * D);
+                float* dst = p.ws_o + r * D;
 #pragma unroll
-                for (int q = 0; q < D / 4; ++q)
-                    dst[q] = make_float4(__uint_as_float(o[4 * q]), __uint_as_float(o[4 * q + 1]), __uint_as_float(o[4 * q + 2]), __uint_as_float(o[4 * q + 3]));
+                for (int q = 0; q < D / 8; ++q)
+                    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + q * 8), "r"(o[8*q]), "r"(o[8*q+1]),
+                                 "r"(o[8*q+2]), "r"(o[8*q+3]), "r"(o[8*q+4]), "r"(o[8*q+5]), "r"(o[8*q+6]), "r"(o[8*q+7]) : "memory");
                 p.ws_ml[r] = make_float2(m, l);
             }
         }
