@@ -429,23 +429,26 @@ paged_rows_tma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 // Merge of the items that several CTAs share, for one fold or for two that ran side by side. A block serves the item that starts
 // in one CTA's range (of the tensor-memory form with its up to 256 rows: an eighth of the item's rows): a row's partials are split over 16 / rows warps (at least one) and joined
 // through shared memory in a fixed order.
-constexpr int TC_MERGE_SPLIT = 8;
+constexpr int TC_MERGE_SPLIT = 8;      // blocks per item of the tensor-memory form
+struct Merge { const float* ws_o; const float2* ws_ml; const int4* ws_merge; int rows; };      // one fold's partials
 template <int D, bool BF16>
-__global__ void __launch_bounds__(512) paged_merge_kernel(const __grid_constant__ Params first, const __grid_constant__ Params second, const int n_first) {
+__global__ void __launch_bounds__(512) paged_merge_kernel(const Merge first, const Merge second, const int n_first, void* out, float* lse, const int q_heads, const int group) {
     griddep_wait();
     griddep_launch();
     const bool one = blockIdx.x < n_first;
-    const Params& p = one ? first : second;
     const int cta = one ? blockIdx.x : (blockIdx.x - n_first) / TC_MERGE_SPLIT;
     const int part = one ? 0 : (blockIdx.x - n_first) % TC_MERGE_SPLIT, n_parts = one ? 1 : TC_MERGE_SPLIT;
-    const int4 it = p.ws_merge[cta];
+    // field by field: a reference to one of two parameters would be read through memory at every use
+    const float* ws_o = one ? first.ws_o : second.ws_o;
+    const float2* ws_ml = one ? first.ws_ml : second.ws_ml;
+    const int slot_rows = one ? first.rows : second.rows;
+    const int4 it = (one ? first.ws_merge : second.ws_merge)[cta];
     if (it.w <= 1) return;
     __shared__ float2 s_ml[16];
     __shared__ float s_o[16][D];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int V = D / 32;                      // floats per lane
-    const int rows = it.y * p.group;
-    const int r0 = (int)((long long)rows * part / n_parts), r1 = (int)((long long)rows * (part + 1) / n_parts);
+    const int rows = it.y * group, r0 = rows * part / n_parts, r1 = rows * (part + 1) / n_parts;
     int wpr = 16;                                  // warps per row
     while (wpr > 1 && (r1 - r0) * wpr > 16) wpr >>= 1;
     const int rpp = 16 / wpr, sub = warp % wpr;    // rows at a time, this warp's share of the parts
@@ -464,9 +467,9 @@ __global__ void __launch_bounds__(512) paged_merge_kernel(const __grid_constant_
 #pragma unroll
                     for (int i = 0; i < V; ++i) a[u][i] = 0.0f;
                     if (q < it.w) {
-                        const size_t at = ((size_t)(cta + q) * 2 + (q == 0 ? 1 : 0)) * p.rows + r;
-                        x[u] = __ldcg(p.ws_ml + at);
-                        const float* po = p.ws_o + at * D + lane * V;
+                        const size_t at = ((size_t)(cta + q) * 2 + (q == 0 ? 1 : 0)) * slot_rows + r;
+                        x[u] = __ldcg(ws_ml + at);
+                        const float* po = ws_o + at * D + lane * V;
                         if (V == 4) { const float4 f = __ldcg((const float4*)po); a[u][0] = f.x; a[u][1] = f.y; a[u][V - 2] = f.z; a[u][V - 1] = f.w; }
                         else { const float2 f = __ldcg((const float2*)po); a[u][0] = f.x; a[u][1] = f.y; }
                     }
@@ -501,13 +504,13 @@ __global__ void __launch_bounds__(512) paged_merge_kernel(const __grid_constant_
             __syncthreads();
         }
         if (r < r1 && sub == 0) {
-            const int tok = r / p.group, head = it.z * p.group + r - tok * p.group;
-            const int64_t at = (int64_t)(it.x + tok) * p.q_heads + head;
+            const int tok = r / group, head = it.z * group + r - tok * group;
+            const int64_t at = (int64_t)(it.x + tok) * q_heads + head;
             const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-            uint16_t* dst = (uint16_t*)p.out + at * D + lane * V;
+            uint16_t* dst = (uint16_t*)out + at * D + lane * V;
             *(uint32_t*)dst = pack2<BF16>(o[0] * inv, o[1] * inv);
             if (V == 4) *(uint32_t*)(dst + 2) = pack2<BF16>(o[V - 2] * inv, o[V - 1] * inv);
-            if (p.lse && lane == 0) p.lse[at] = (m + log2f(l) - p_shift<BF16>()) * LN2;
+            if (lse && lane == 0) lse[at] = (m + log2f(l) - p_shift<BF16>()) * LN2;
         }
     }
 }
@@ -609,8 +612,10 @@ int32_t validate(sanic_ctx* ctx, const sanic_attn_paged_params* p) {
 namespace {
 cudaError_t launch_merge(const Params& a, int n_a, const Params& b, int n_b, int D, int dtype, cudaStream_t st) {
     const dim3 grid(n_a + n_b * TC_MERGE_SPLIT), block(512);
-    if (D == 128) return dtype == SANIC_BF16 ? launch_pdl(paged_merge_kernel<128, true>, grid, block, 0, st, a, b, n_a) : launch_pdl(paged_merge_kernel<128, false>, grid, block, 0, st, a, b, n_a);
-    return dtype == SANIC_BF16 ? launch_pdl(paged_merge_kernel<64, true>, grid, block, 0, st, a, b, n_a) : launch_pdl(paged_merge_kernel<64, false>, grid, block, 0, st, a, b, n_a);
+    const Merge x{a.ws_o, a.ws_ml, a.ws_merge, a.rows}, y{b.ws_o, b.ws_ml, b.ws_merge, b.rows};
+    auto go = [&](auto kernel) { return launch_pdl(kernel, grid, block, 0, st, x, y, n_a, a.out, a.lse, a.q_heads, a.group); };
+    if (D == 128) return dtype == SANIC_BF16 ? go(paged_merge_kernel<128, true>) : go(paged_merge_kernel<128, false>);
+    return dtype == SANIC_BF16 ? go(paged_merge_kernel<64, true>) : go(paged_merge_kernel<64, false>);
 }
 }  // namespace
 
