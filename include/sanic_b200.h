@@ -610,7 +610,8 @@ int32_t sanic_paged_cache_write(sanic_ctx* ctx, const sanic_paged_write_params* 
  * the pages already. out [n_tokens, q_heads, head_dim] at dtype, dense; lse (optional) [n_tokens, q_heads] f32, the natural
  * log of the sum of exp(scale q.k). A token that sees no key (position < 0) gets zeros and -inf. Rows of q outside every
  * request's range, and their out and lse, are neither read for a result nor written. Keys no token of the request sees
- * (behind kv_lens, before the window) are not read, whatever the pages hold there. Scores, maxima, sums and the output
+ * (behind kv_lens, before the window) do not count, whatever the pages hold there; a key that some token of the chunk sees is
+ * read once for many of them, and a value row of it that is not finite may make NaN of tokens it is hidden from. Scores, maxima, sums and the output
  * accumulator are f32; the weights exp(s - max) are rounded to dtype for the product with v. max_query_len, a bound on the
  * chunk lengths (0: n_tokens), only selects a kernel: a longer chunk is still computed. dtype SANIC_BF16 or SANIC_F16,
  * head_dim 64 or 128, at most 64 query heads per kv head. A table entry outside [0, n_pages) reads as zeros; it, and lengths

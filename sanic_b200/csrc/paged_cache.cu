@@ -93,23 +93,22 @@ __global__ void __launch_bounds__(AT) page_append_kernel(const sanic_page_append
     // token rows
     const int used = s_tok[n];
     for (int t = first; t < p.n_tokens; t += stride) {
-        int pos = 0;
-        long long slot = -1;
+        long long pos = 0, slot = -1;            // 64 bits: a length near 2^31 must not wrap into a page index
         if (t < used) {
             int lo = 0, hi = n - 1;              // the last request with s_tok[b] <= t
             while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (s_tok[mid] <= t) lo = mid; else hi = mid - 1; }
             const int seq = max(p.seq_lens[lo], 0), held = held_of(p, lo, seq);
-            pos = seq + t - s_tok[lo];
-            const int idx = pos / p.page_size;
+            pos = (long long)seq + t - s_tok[lo];
+            const int idx = (int)(pos / p.page_size);
             int page = -1;
             if (idx < held) page = p.block_table[(int64_t)lo * p.table_stride + idx];      // entries of earlier steps: nobody writes them here
             else if (idx < p.max_pages) {
                 const int r = s_pg[lo] + idx - held;
                 if (r < free_n) page = p.free_pages[free_n - 1 - r];
             }
-            if (page >= 0) slot = (long long)page * p.page_size + pos - idx * p.page_size;
+            if (page >= 0) slot = (long long)page * p.page_size + pos - (long long)idx * p.page_size;
         }
-        p.positions[t] = pos;
+        p.positions[t] = (int)min(pos, (long long)INT32_MAX);
         p.slots[t] = slot;
     }
 }

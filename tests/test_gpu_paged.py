@@ -242,6 +242,69 @@ def test_attn_large_scores(dev):
         assert ((lse.double() - wl).abs() <= 2e-2).all()
 
 
+@pytest.mark.parametrize("maxq", [1, 200])
+def test_attn_many_requests_and_a_table_cut_from_a_wider_one(dev, maxq):
+    # more requests than threads of a block; rows of the table further apart than its width
+    r = np.random.default_rng(3)
+    new = r.integers(0, 3, 1500)
+    if maxq > 1:
+        new[700] = 150
+    ctx = r.integers(0, 90, 1500)
+    args, keys, values = make_problem(dev, new.tolist(), ctx.tolist(), 4, 2, 64, "bf16", 16, seed=14)
+    wide = torch.full((1500, args["block_table"].shape[1] + 37), 1 << 29, dtype=torch.int32, device=dev.torch_device)
+    wide[:, 5:5 + args["block_table"].shape[1]] = args["block_table"]
+    args["block_table"] = wide[:, 5:5 + args["block_table"].shape[1]]
+    got, lse = dev.attn_paged(**args, max_query_len=maxq, return_lse=True)
+    dev.sync()
+    check_attention(got, lse, *plain_attention(args["q"], keys, values, new.tolist(), (ctx + new).tolist(), 0, 0.125))
+
+
+FIRST_IN_CAPTURE = r'''
+import torch
+from sanic_b200 import CudaDevice
+dev = CudaDevice(0)
+z = lambda *s, t=torch.bfloat16: torch.zeros(*s, dtype=t, device="cuda")
+i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+kp, vp, table, free = z(8, 16, 2, 64), z(8, 16, 2, 64), i32([[0, 0], [0, 0]]), i32([7, 6, 5, 4, 3, 2, 1, 0])
+seq, new, count = i32([0, 0]), i32([20, 3]), i32([8])
+k, q = torch.randn(23, 2, 64, device="cuda").bfloat16(), torch.randn(23, 4, 64, device="cuda").bfloat16()
+probs, drafts, ua, us = torch.full((4, 50), 0.02, device="cuda"), i32([[1], [2]]), z(2, 1, t=torch.float32), z(2, t=torch.float32)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    step = dev.page_table_append(seq, new, table, free, count, 16, 23)
+    qr = dev.paged_cache_write(k, k, kp, vp, step.slots, q=q)
+    a = dev.attn_paged(qr, kp, vp, table, step.query_start, step.kv_lens, max_query_len=20)
+    b = dev.attn_paged(qr, kp, vp, table, step.query_start, step.kv_lens, max_query_len=1)
+    t, n = dev.draft_verify(probs, drafts, ua, us)
+for _ in range(3):
+    g.replay()
+torch.cuda.synchronize()
+dev.sync()
+assert torch.equal(a[0], b[0]) and torch.isfinite(a.float()).all() and (a.float() - b.float()).abs().max() < 0.05
+assert n.tolist() == [1, 1] and table.tolist() == [[0, 1], [2, 0]], (n, table)
+print("captured")
+'''
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_IN_CAPTURE], cwd=root, capture_output=True, text=True, timeout=180)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("code,what", [(53, "page_table_append"), (54, "attn_paged"), (55, "draft_verify"), (56, "paged_cache_write")])
+def test_status_codes_name_their_operator(dev, code, what):
+    from sanic_b200 import RunError
+    assert dev.lib.sanic_status_inject(dev.h, code) == 0
+    with pytest.raises(RunError, match=what):
+        dev.sync()
+    dev.sync()
+
+
 @pytest.mark.parametrize("maxq", [1, 64])
 def test_attn_bad_pages_and_lengths_are_reported(dev, maxq):
     from sanic_b200 import RunError
@@ -357,14 +420,14 @@ def plain_append(seq, new, held, table, free, count, page, n_tokens):
                 table[b, col] = -1
                 bad = True
         pages.append(got)
-        kv.append(s + n)
+        kv.append(min(s + n, (1 << 31) - 1))
         for i in range(n):
             if len(pos) >= n_tokens:
                 bad = True
                 break
             p = s + i
             e = table[b, p // page] if p // page < max_pages else -1
-            pos.append(p)
+            pos.append(min(p, (1 << 31) - 1))
             slots.append(-1 if e < 0 else int(e) * page + p % page)
         start.append(len(pos))
     rest = n_tokens - len(pos)
@@ -424,6 +487,7 @@ def test_append_shortages_are_reported(dev):
     check_append(dev, [60, 10], [30, 3], 16, 4, 8, 33)                            # a table row too short
     check_append(dev, [3, 3, 3], [10, 10, 10], 16, 4, 8, 17)                      # more new tokens than token rows
     check_append(dev, [-4, 9], [3, -2], 16, 4, 8, 6)                              # negative lengths read as 0
+    check_append(dev, [(1 << 31) - 5, 3], [9, 4], 16, 4, 8, 13, held=[1, 1])      # a length that nearly wraps: no page, no slot
     check_append(dev, [5], [2], 16, 4, 8, 2)                                      # and the next call is clean again
 
 
