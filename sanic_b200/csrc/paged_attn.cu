@@ -6,14 +6,15 @@
 // CTAs share, and the entry point. paged_attn_tc.cu: the form for many rows.
 //
 // With R = tokens * (query heads per kv head) rows the fold does 4 R flop per key element and reads it once (2 bytes for
-// each of k and v), so below about 64 rows HBM bounds it: what matters is bytes in flight and equal ranges. A CTA of four
-// warps folds 64-key tiles that arrive by 16-byte cp.async through a ring of 3 (head_dim 128) or 4 (64) stages; a tile's
-// page lookups run one tile ahead of its copies. The rows of an item are 16 MT rows of m16n8k16 MMAs: with MT = 1 each warp
-// takes 16 of the tile's keys, with MT = 2 a warp takes 16 rows and half of the keys, with MT = 4 a warp takes 16 rows and
-// all keys. Carriers stay in registers; the warps that share rows merge once per segment. P goes to the tensor core rounded
+// each of k and v), so up to some tens of rows HBM bounds it: what matters is bytes in flight and equal ranges. Four warps fold
+// 64-key tiles out of a ring of 3 (head_dim 128) or 4 (64) stages that a fifth fills. (128-key tiles at head_dim 64, two CTAs
+// per SM instead of three: 77 instead of 67 us for 64 decodes of 2000 keys.) The rows of an item are 16 MT rows of m16n8k16
+// MMAs: with MT = 1 each warp takes 16 of the tile's keys, with MT = 2 a warp takes 16 rows and half of the keys, with MT = 4 a
+// warp takes 16 rows and all keys. Carriers stay in registers; the warps that share rows merge once per segment. P goes to the tensor core rounded
 // to the storage type (bf16: 2^-9 per weight; f16 likewise after a shift by 2^8, which keeps the weights of a long flat
 // softmax out of f16's subnormals), sums and maxima are f32.
-// Rows are spread over an exactly resident grid as one contiguous range of (item, key tile) per CTA (see paged.cuh).
+// The work is spread over an exactly resident grid as one contiguous range of (item, key tile) per CTA (paged_sched.h).
+// 64 decodes of 8000 keys on average, 32 + 8 heads of 128, bf16 (2.14 GB): 340 us = 6.3 TB/s, 0.96 of the measured copy rate.
 #include "paged_tma.cuh"
 
 namespace {
