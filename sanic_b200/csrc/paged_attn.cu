@@ -23,6 +23,8 @@ using namespace sanic::paged;
 
 constexpr int KT = 64;
 // Chunks of more query rows than this (tokens * heads of a group) go to the tensor-memory form where its loads suit the layout.
+// Groups of 4 heads of 128 over 4000 keys, rows form against tensor-memory form: 20 rows of 32 requests 104 / 125 us, 32 rows
+// 107 / 126 us, 64 rows of 16 requests 92 / 80 us, of 2 requests 53 / 28 us.
 constexpr int TC_ABOVE_ROWS = 32;
 
 template <int D> struct Cfg {
