@@ -443,7 +443,7 @@ class CudaDevice:
             raise RunError("n_tokens must not be negative")
         # one allocation for all outputs: an allocation or a view costs more host time than the kernel takes
         block = seq_lens.new_empty(3 * n_tokens + 3 * n + 2, dtype=i32)
-        slots, start, kv, held, count, pos = block.split_with_sizes((2 * n_tokens, n + 1, n, n, 1, n_tokens))
+        slots, start, kv, held, count, pos = block.unsafe_split_with_sizes((2 * n_tokens, n + 1, n, n, 1, n_tokens))
         out = PageStep(start, kv, held, count, pos, slots.view(torch.int64))
         base = block.data_ptr()
         at = base + 8 * n_tokens
@@ -461,13 +461,15 @@ class CudaDevice:
         return (self._paged("k_pages", k_pages, (torch.bfloat16, torch.float16), 4),
                 self._paged("v_pages", v_pages, (torch.bfloat16, torch.float16), 4))
 
-    def _token_rows(self, name, t, dtype, n_tokens, heads, dim):
-        st = self._paged(name, t, (dtype,), 3)
-        if t.shape[0] != n_tokens or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
-            raise RunError(f"input `{name}` has shape {tuple(t.shape)}; expected [{n_tokens}, {heads if heads is not None else 'heads'}, {dim}]")
-        if t.shape[1] > 1 and st[1] != dim:
+    def _token_rows(self, name, t, dtype, shape):
+        """Stride between the token rows of [n_tokens, heads, dim] whose heads lie side by side."""
+        if isinstance(t, torch.Tensor) and t.get_device() == self.ordinal and t.dtype == dtype and t.shape == shape:
+            st = t.stride()
+            if (st[2] == 1 and (st[1] == shape[2] or shape[1] == 1)) or not t.numel():
+                return st[0]
             raise RunError(f"the heads of `{name}` must lie side by side")
-        return st[0]
+        self._paged(name, t, (dtype,), 3)
+        raise RunError(f"input `{name}` has shape {tuple(t.shape)}; expected {list(shape)}")
 
     def paged_cache_write(self, k, v, k_pages, v_pages, slots, q=None, positions=None, rope_table=None, q_out=None):
         """k, v [n_tokens, kv_heads, D] -> rows slots[t] (page * page_size + row, int64; negative: skipped) of k_pages, v_pages
@@ -481,14 +483,18 @@ class CudaDevice:
         src = k.dtype
         if src != torch.float32 and src != k_pages.dtype:
             raise RunError(f"input `k` has dtype {src}; expected torch.float32 or {k_pages.dtype}")
-        kst, vst = self._token_rows("k", k, src, t, hkv, d), self._token_rows("v", v, src, t, hkv, d)
+        rows = (t, hkv, d)
+        kst, vst = self._token_rows("k", k, src, rows), self._token_rows("v", v, src, rows)
         qst = qost = hq = 0
         if q is not None:
             hq = q.shape[1]
-            qst = self._token_rows("q", q, src, t, hq, d)
+            rows = (t, hq, d)
+            qst = self._token_rows("q", q, src, rows)
             if q_out is None:
-                q_out = q.new_empty((t, hq, d), dtype=k_pages.dtype)
-            qost = self._token_rows("q_out", q_out, k_pages.dtype, t, hq, d)
+                q_out = k_pages.new_empty_strided(rows, (hq * d, d, 1))
+                qost = hq * d
+            else:
+                qost = self._token_rows("q_out", q_out, k_pages.dtype, rows)
         elif q_out is not None:
             raise RunError("q_out needs q")
         n_pos = 0
@@ -496,15 +502,16 @@ class CudaDevice:
             if positions is None:
                 raise RunError("rope_table needs positions")
             n_pos = rope_table.shape[0]
-            if tuple(rope_table.shape[1:]) != (d // 2, 2):
+            if rope_table.shape != (n_pos, d // 2, 2):
                 raise RunError(f"rope_table has shape {tuple(rope_table.shape)}; expected [positions, {d // 2}, 2]")
-            self._flat("rope_table", rope_table, torch.float32, rope_table.numel())
+            table_ptr, pos_ptr = self._flat("rope_table", rope_table, torch.float32, n_pos * d), self._flat("positions", positions, torch.int32, t)
+        else:
+            table_ptr = pos_ptr = None
         p = abi.PagedWriteParams(
             None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), qst, kst, vst, None if q is None else q_out.data_ptr(), qost,
             k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-            None if rope_table is None else rope_table.data_ptr(),
-            None if rope_table is None else self._flat("positions", positions, torch.int32, t), n_pos, self._flat("slots", slots, torch.int64, t),
-            t, hq, hkv, d, page_size, n_pages, abi.F32 if src == torch.float32 else _HALF[src], _HALF[k_pages.dtype])
+            table_ptr, pos_ptr, n_pos, self._flat("slots", slots, torch.int64, t), t, hq, hkv, d, page_size, n_pages,
+            abi.F32 if src == torch.float32 else _HALF[src], _HALF[k_pages.dtype])
         self._check(self.lib.sanic_paged_cache_write(self.h, C.byref(p), self.stream()), "paged_cache_write")
         return q_out
 
@@ -524,11 +531,11 @@ class CudaDevice:
         if dk != d or q.dtype != k_pages.dtype:
             raise RunError(f"attention shapes disagree: q {tuple(q.shape)} {q.dtype}, pages {tuple(k_pages.shape)} {k_pages.dtype}")
         if out is None:
-            out = q.new_empty((T, hq, d))
+            out = q.new_empty_strided((T, hq, d), (hq * d, d, 1))
             out_ptr = out.data_ptr()
         else:
             out_ptr = self._flat("out", out, q.dtype, T * hq * d)
-        lse = q.new_empty((T, hq), dtype=torch.float32) if return_lse else None
+        lse = q.new_empty_strided((T, hq), (hq, 1), dtype=torch.float32) if return_lse else None
         p = abi.AttnPagedParams(
             q.data_ptr(), out_ptr, lse.data_ptr() if return_lse else None, k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
             self._flat("query_start", query_start, torch.int32, n + 1), self._flat("kv_lens", kv_lens, torch.int32, n), None, 0,
@@ -557,8 +564,8 @@ class CudaDevice:
             if tuple(draft_probs.shape) != (n, k, vocab):
                 raise RunError(f"input `draft_probs` has shape {tuple(draft_probs.shape)}; expected {(n, k, vocab)}")
         i32, f32 = torch.int32, torch.float32
-        out = draft_tokens.new_empty((n, k + 1), dtype=i32)
-        accepted = u_sample.new_empty(n, dtype=i32)
+        out = draft_tokens.new_empty_strided((n, k + 1), (k + 1, 1), dtype=i32)
+        accepted = draft_tokens.new_empty(n, dtype=i32)
         p = abi.DraftVerifyParams(
             target_probs.data_ptr(), ts[0], rows, None if target_start is None else self._flat("target_start", target_start, i32, n),
             None if draft_probs is None or not k else draft_probs.data_ptr(), ds[0], ds[1], self._flat("draft_tokens", draft_tokens, i32, n * k) or None,
