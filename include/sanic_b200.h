@@ -641,12 +641,12 @@ size_t sanic_attn_paged_workspace_bytes(sanic_ctx* ctx, const sanic_attn_paged_p
  * [0, target_rows) ends the request with -1; each is reported (code 55). */
 typedef struct {
     const float* target_probs; int64_t target_stride; int32_t target_rows; const int32_t* target_start;
-    const float* draft_probs; int64_t draft_request_stride, draft_stride;     /* [n, max_draft, vocab] or NULL */
+    const float* draft_probs; int64_t draft_request_stride, draft_stride;     /* [n, max_draft, vocab] or NULL; requests may share rows (stride 0) */
     const int32_t* draft_tokens;                                              /* [n, max_draft] */
     const int32_t* draft_lens;                                                /* [n], NULL: max_draft */
     const float* u_accept; const float* u_sample;                             /* [n, max_draft], [n], in [0, 1) */
     int32_t* tokens_out; int32_t* accepted;
-    int32_t n_requests, max_draft, vocab;                                     /* max_draft <= 32 */
+    int32_t n_requests, max_draft, vocab;                                     /* max_draft <= 32, vocab <= 2^19 */
 } sanic_draft_verify_params;
 int32_t sanic_draft_verify(sanic_ctx* ctx, const sanic_draft_verify_params* p, void* stream);
 

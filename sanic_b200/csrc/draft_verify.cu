@@ -235,8 +235,10 @@ extern "C" int32_t sanic_draft_verify(sanic_ctx* ctx, const sanic_draft_verify_p
     if (p->n_requests == 0) return SANIC_OK;
     SANIC_REQUIRE(ctx, p->target_probs && p->u_sample && p->tokens_out && p->accepted && p->target_rows > 0, "draft_verify: null tensor");
     SANIC_REQUIRE(ctx, p->max_draft == 0 || (p->draft_tokens && p->u_accept), "draft_verify: drafts need tokens and u_accept");
+    SANIC_REQUIRE(ctx, (long long)p->n_requests * (p->max_draft + 1) < (1ll << 31), "draft_verify: too many rows");
     SANIC_REQUIRE(ctx, p->target_stride >= p->vocab || p->target_rows == 1, "draft_verify: target rows overlap");
-    SANIC_REQUIRE(ctx, !p->draft_probs || (p->draft_stride >= p->vocab && p->draft_request_stride >= 0), "draft_verify: draft rows overlap");
+    SANIC_REQUIRE(ctx, !p->draft_probs || ((p->draft_stride >= p->vocab || p->max_draft == 1) && p->draft_stride >= 0 && p->draft_request_stride >= 0),
+                  "draft_verify: draft rows overlap");
     sanic_set_device(ctx);
     // CTAs per request: enough that the batch covers four blocks per SM, at most 16 (a cluster's limit) and never less than a
     // group each (64 requests of 128256 entries: 8 each 21 us, 16 each 34 us, 4 each 23 us; one request: 16 10.6 us, 8 13.1 us)

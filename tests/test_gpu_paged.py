@@ -259,6 +259,59 @@ def test_attn_many_requests_and_a_table_cut_from_a_wider_one(dev, maxq):
     check_attention(got, lse, *plain_attention(args["q"], keys, values, new.tolist(), (ctx + new).tolist(), 0, 0.125))
 
 
+@pytest.mark.parametrize("page", [192, 384, 2048])
+@pytest.mark.parametrize("maxq", [1, 200])
+def test_attn_large_and_odd_pages(dev, page, maxq):
+    # pages that are a multiple of a tile but no power of two; a pool of one page
+    new, ctx = ([1, 140, 3], [500, 300, 0]) if page < 2048 else ([150], [1000])
+    args, keys, values = make_problem(dev, new, ctx, 8, 2, 128, "bf16", page, seed=15, extra_pages=0 if page == 2048 else 2)
+    assert page < 2048 or args["k_pages"].shape[0] == 1
+    got, lse = dev.attn_paged(**args, max_query_len=maxq, return_lse=True)
+    dev.sync()
+    check_attention(got, lse, *plain_attention(args["q"], keys, values, new, [n + c for n, c in zip(new, ctx)], 0, 128 ** -0.5))
+
+
+@pytest.mark.parametrize("maxq", [1, 100])
+def test_attn_shared_prefix_pages(dev, maxq):
+    # two requests whose tables name the same pages for their common prefix
+    args, keys, values = make_problem(dev, [1, 40, 1], [64, 100, 64], 4, 2, 64, "f16", 16, seed=16)
+    table = args["block_table"]
+    table[2, :4] = table[0, :4]
+    keys[2] = torch.cat([keys[0][:64], keys[2][64:]]); values[2] = torch.cat([values[0][:64], values[2][64:]])
+    got, lse = dev.attn_paged(**args, max_query_len=maxq, return_lse=True)
+    dev.sync()
+    check_attention(got, lse, *plain_attention(args["q"], keys, values, [1, 40, 1], [65, 140, 65], 0, 0.125))
+
+
+@pytest.mark.parametrize("maxq", [1, 100])
+def test_attn_and_append_at_the_largest_batch(dev, maxq):
+    # 8000 requests of 5 held tokens and one new one, through the page tables
+    from sanic_b200 import RunError
+    n, page, td = 8000, 4, dev.torch_device
+    g = gen(dev, 17)
+    seq, one = torch.full((n,), 5, dtype=torch.int32, device=td), torch.ones(n, dtype=torch.int32, device=td)
+    table = torch.full((n, 2), -1, dtype=torch.int32, device=td)
+    free = torch.randperm(2 * n, generator=g, device=td).to(torch.int32)
+    first = dev.page_table_append(torch.zeros_like(seq), seq, table, free, ints(dev, [2 * n]), page, 5 * n)
+    step = dev.page_table_append(seq, one, table, free, first.free_count, page, n, held_pages=first.held_pages)
+    dev.sync()
+    assert step.free_count.item() == 0 and sorted(table.flatten().tolist()) == list(range(2 * n)) and (step.positions == 5).all()
+    k, v = (torch.randn(n, 6, 1, 64, generator=g, device=td).to(torch.bfloat16) for _ in range(2))
+    kp, vp = (torch.full((2 * n, page, 1, 64), float("nan"), dtype=torch.bfloat16, device=td) for _ in range(2))
+    dev.paged_cache_write(k[:, :5].reshape(-1, 1, 64), v[:, :5].reshape(-1, 1, 64), kp, vp, first.slots)
+    dev.paged_cache_write(k[:, 5], v[:, 5], kp, vp, step.slots)
+    q = torch.randn(n, 4, 64, generator=g, device=td).to(torch.bfloat16)
+    got, lse = dev.attn_paged(q, kp, vp, table, step.query_start, step.kv_lens, max_query_len=maxq, return_lse=True)
+    dev.sync()
+    s = torch.einsum("nhd,nkd->nhk", q.double(), k[:, :, 0].double()) * 0.125
+    w = torch.softmax(s, -1)
+    check_attention(got, lse, torch.einsum("nhk,nkd->nhd", w, v[:, :, 0].double()), torch.einsum("nhk,nkd->nhd", w, v[:, :, 0].double().abs()),
+                    torch.logsumexp(s, -1))
+    with pytest.raises(RunError, match="8000"):
+        dev.attn_paged(q, kp, vp, torch.zeros(8001, 2, dtype=torch.int32, device=td), torch.zeros(8002, dtype=torch.int32, device=td),
+                       torch.zeros(8001, dtype=torch.int32, device=td))
+
+
 FIRST_IN_CAPTURE = r'''
 import torch
 from sanic_b200 import CudaDevice
@@ -726,6 +779,22 @@ def test_verify_unaligned_rows(dev):
     assert got.tolist() == want and acc.tolist() == counts
 
 
+def test_verify_one_draft_whatever_its_stride(dev):
+    # one drafted token: the stride between a request's drafts is never used; requests may share one row of probabilities
+    n, vocab, td = 3, 700, dev.torch_device
+    g = gen(dev, 31)
+    target = torch.softmax(torch.randn(2 * n, vocab, generator=g, device=td), -1)
+    rows = torch.softmax(torch.randn(n, vocab, generator=g, device=td), -1)
+    tokens = ints(dev, [[5], [699], [0]])
+    ua, us = torch.full((n, 1), 0.999, device=td), torch.full((n,), 0.6, device=td)
+    for probs in (rows.as_strided((n, 1, vocab), (vocab, 1, 1)), rows[:1].as_strided((n, 1, vocab), (0, 0, 1))):
+        got, acc = dev.draft_verify(target, tokens, ua, us, draft_probs=probs)
+        dev.sync()
+        want, counts, _ = plain_verify(target.cpu().numpy(), tokens.cpu().numpy(), ua.cpu().numpy(), us.cpu().numpy(),
+                                       probs.cpu().contiguous().numpy(), [1] * n, [2 * b for b in range(n)])
+        assert got.tolist() == want and acc.tolist() == counts
+
+
 def test_verify_out_of_range_is_reported(dev):
     from sanic_b200 import CompileError, RunError
     td = dev.torch_device
@@ -749,6 +818,11 @@ def test_verify_out_of_range_is_reported(dev):
         assert acc[bad] == 0 and got[bad].tolist() == [-1, -1, -1] and acc[1 - bad] == 2
     with pytest.raises(CompileError, match="32 drafted"):
         dev.draft_verify(torch.zeros(34, 8, device=td), torch.zeros(1, 33, dtype=torch.int32, device=td), torch.zeros(1, 33, device=td), us[:1])
+    from sanic_b200 import abi
+    x = target.data_ptr()
+    p = abi.DraftVerifyParams(x, 40, 6, None, None, 0, 0, x, None, x, x, x, x, 1 << 26, 31, 40)      # 2^31 rows: refused, nothing is read
+    with pytest.raises(RunError, match="too many rows"):
+        dev._check(dev.lib.sanic_draft_verify(dev.h, C.byref(p), dev.stream()), "draft_verify")
     got, acc = dev.draft_verify(target, ok, ua, us)
     dev.sync()
     assert acc.tolist() == [2, 2]
