@@ -87,6 +87,16 @@ template <bool BF16> __device__ __forceinline__ uint32_t pack2(float lo, float h
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// 32 bytes to a 16-byte boundary; `wide`: to a 32-byte one
+__device__ __forceinline__ void store8(void* dst, const uint32_t (&w)[8], bool wide) {
+    if (wide) {
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                     "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+    } else {
+        ((uint4*)dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        ((uint4*)dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+}
 __device__ __forceinline__ bool elect_one() {
     uint32_t pred;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
@@ -537,6 +547,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             if (s.whole) {
                 const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;      // no visible key: zeros, and -inf for the log-sum-exp
                 uint16_t* dst = (uint16_t*)p.out + at * D;
+                const bool wide = ((uintptr_t)p.out & 31) == 0;
                 if (!(l != 0.0f)) {
 #pragma unroll
                     for (int i = 0; i < D; ++i) o[i] = 0u;                   // every weight of the row was 0: V's zero rows and NaN alike
@@ -547,17 +558,15 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         wv[j] = pack2<BF16>(__uint_as_float(o[16 * q + 2 * j]) * inv, __uint_as_float(o[16 * q + 2 * j + 1]) * inv);
-                    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + q * 16), "r"(wv[0]), "r"(wv[1]),
-                                 "r"(wv[2]), "r"(wv[3]), "r"(wv[4]), "r"(wv[5]), "r"(wv[6]), "r"(wv[7]) : "memory");
+                    store8(dst + q * 16, wv, wide);
                 }
                 if (p.lse) p.lse[at] = (m + log2f(l) - P_SHIFT) * LN2;
             } else {
                 const size_t r = (size_t)s.slot * p.rows + t * tile_rows + row;
                 float* dst = p.ws_o + r * D;
+                const bool wide = ((uintptr_t)p.ws_o & 31) == 0;
 #pragma unroll
-                for (int q = 0; q < D / 8; ++q)
-                    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + q * 8), "r"(o[8*q]), "r"(o[8*q+1]),
-                                 "r"(o[8*q+2]), "r"(o[8*q+3]), "r"(o[8*q+4]), "r"(o[8*q+5]), "r"(o[8*q+6]), "r"(o[8*q+7]) : "memory");
+                for (int q = 0; q < D / 8; ++q) store8(dst + q * 8, *reinterpret_cast<uint32_t(*)[8]>(&o[8 * q]), wide);
                 p.ws_ml[r] = make_float2(m, l);
             }
         }

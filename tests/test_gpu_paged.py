@@ -312,6 +312,40 @@ def test_attn_and_append_at_the_largest_batch(dev, maxq):
                        torch.zeros(8001, dtype=torch.int32, device=td))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("maxq", [1, 200])
+def test_attn_outputs_and_workspaces_on_16_byte_boundaries(dev, d, maxq):
+    from sanic_b200 import abi
+    new, ctx, hq, hkv = [1, 140, 3], [500, 300, 0], 4, 2
+    args, keys, values = make_problem(dev, new, ctx, hq, hkv, d, "bf16", 16, seed=18)
+    T, td, n = sum(new), dev.torch_device, 3
+    want = plain_attention(args["q"], keys, values, new, [a + b for a, b in zip(new, ctx)], 0, d ** -0.5)
+    flat = torch.full((T * hq * d + 16,), 3.0, dtype=torch.bfloat16, device=td)
+    out = flat[8:8 + T * hq * d].view(T, hq, d)
+    assert out.data_ptr() % 32 == 16
+    got, lse = dev.attn_paged(**args, max_query_len=maxq, return_lse=True, out=out)
+    dev.sync()
+    check_attention(got, lse, *want)
+    assert (flat[:8] == 3.0).all() and (flat[-8:] == 3.0).all()
+    # the same with a workspace on a 16-byte boundary, its bytes of any value, and nothing written past its end
+    q, kp, vp, bt = args["q"], args["k_pages"], args["v_pages"], args["block_table"]
+    out.fill_(3.0); lse = torch.empty(T, hq, device=td)
+    p = abi.AttnPagedParams(q.data_ptr(), out.data_ptr(), lse.data_ptr(), kp.data_ptr(), vp.data_ptr(), bt.data_ptr(), args["query_start"].data_ptr(),
+                            args["kv_lens"].data_ptr(), None, 0, q.stride(0), q.stride(1), kp.stride(0), kp.stride(1), kp.stride(2), vp.stride(0),
+                            vp.stride(1), vp.stride(2), bt.stride(0), abi.BF16, n, T, maxq, hq, hkv, d, 16, kp.shape[0], bt.shape[1], 0, d ** -0.5)
+    nbytes = dev.lib.sanic_attn_paged_workspace_bytes(dev.h, C.byref(p))
+    ws = torch.full((nbytes // 4 + 8,), -1, dtype=torch.int32, device=td)
+    p.workspace, p.workspace_bytes = ws.data_ptr() + 16, nbytes
+    dev._check(dev.lib.sanic_attn_paged(dev.h, C.byref(p), dev.stream()), "attn_paged")
+    dev.sync()
+    check_attention(out, lse, *want)
+    assert (ws[:4] == -1).all() and (ws[4 + nbytes // 4:] == -1).all() and (flat[:8] == 3.0).all() and (flat[-8:] == 3.0).all()
+    p.workspace = ws.data_ptr() + 8
+    from sanic_b200 import RunError
+    with pytest.raises(RunError, match="workspace"):
+        dev._check(dev.lib.sanic_attn_paged(dev.h, C.byref(p), dev.stream()), "attn_paged")
+
+
 FIRST_IN_CAPTURE = r'''
 import torch
 from sanic_b200 import CudaDevice
