@@ -539,8 +539,8 @@ class CudaDevice:
         p = abi.AttnPagedParams(
             q.data_ptr(), out_ptr, lse.data_ptr() if return_lse else None, k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
             self._flat("query_start", query_start, torch.int32, n + 1), self._flat("kv_lens", kv_lens, torch.int32, n), None, 0,
-            qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], ts[0], _HALF[q.dtype], n, T, int(max_query_len), hq, hkv, d, page_size,
-            n_pages, max_pages, int(window), float(scale) if scale is not None else 1.0 / math.sqrt(d))
+            qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], ts[0], _HALF[q.dtype], n, T, min(int(max_query_len), 0x7fffffff), hq, hkv, d, page_size,
+            n_pages, max_pages, min(int(window), 0x7fffffff), float(scale) if scale is not None else 1.0 / math.sqrt(d))
         # a workspace per call: calls on other streams, and graphs that replay side by side, never share one
         nbytes = self.lib.sanic_attn_paged_workspace_bytes(self.h, C.byref(p))
         ws = kv_lens.new_empty(nbytes // 4)

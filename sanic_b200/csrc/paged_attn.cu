@@ -597,8 +597,9 @@ int32_t validate(sanic_ctx* ctx, const sanic_attn_paged_params* p) {
     if (p->q_heads / p->kv_heads > 64) return sanic_fail(ctx, SANIC_ERR_UNSUPPORTED, "attn_paged: at most 64 query heads per key/value head");
     SANIC_REQUIRE(ctx, p->n_requests <= MAX_REQUESTS, "attn_paged: at most 8000 requests per call");
     SANIC_REQUIRE(ctx, p->page_size > 0 && p->n_pages > 0 && p->max_pages > 0, "attn_paged: empty page pool or table");
-    SANIC_REQUIRE(ctx, (long long)p->max_pages * p->page_size < (1ll << 31) - 256, "attn_paged: a table row spans 2^31 keys or more");
     SANIC_REQUIRE(ctx, (long long)p->n_tokens * p->q_heads < (1ll << 31), "attn_paged: too many rows");
+    // positions run from -n_tokens (more tokens than keys) to the row's last key, and a window's start below them: all in 32 bits
+    SANIC_REQUIRE(ctx, (long long)p->max_pages * p->page_size + p->n_tokens < (1ll << 31) - 256, "attn_paged: a table row spans 2^31 keys or more");
     SANIC_REQUIRE(ctx, p->window >= 0, "attn_paged: negative window");
     SANIC_REQUIRE(ctx, p->scale > 0.0f && p->scale < INFINITY, "attn_paged: scale must be positive and finite");
     SANIC_REQUIRE(ctx, p->q_token_stride % 8 == 0 && p->q_head_stride % 8 == 0 && p->k_page_stride % 8 == 0 && p->k_row_stride % 8 == 0 &&
@@ -646,7 +647,8 @@ int32_t sanic_attn_paged(sanic_ctx* ctx, const sanic_attn_paged_params* p, void*
     q.v_page_stride = p->v_page_stride; q.v_row_stride = p->v_row_stride; q.v_head_stride = p->v_head_stride;
     q.table_stride = p->table_stride;
     q.n_requests = p->n_requests; q.n_tokens = p->n_tokens; q.q_heads = p->q_heads; q.kv_heads = p->kv_heads; q.group = p->q_heads / p->kv_heads;
-    q.page_size = p->page_size; q.n_pages = p->n_pages; q.max_pages = p->max_pages; q.window = p->window; q.scale = p->scale;
+    q.page_size = p->page_size; q.n_pages = p->n_pages; q.max_pages = p->max_pages; q.scale = p->scale;
+    q.window = p->window < (long long)p->max_pages * p->page_size ? p->window : 0;      // wider than a table row: it hides nothing
     q.page_shift = -1;
     for (int i = 0; i < 31; ++i) if ((1 << i) == p->page_size) q.page_shift = i;
     q.rows_upto = INT32_MAX;

@@ -346,6 +346,21 @@ def test_attn_outputs_and_workspaces_on_16_byte_boundaries(dev, d, maxq):
         dev._check(dev.lib.sanic_attn_paged(dev.h, C.byref(p), dev.stream()), "attn_paged")
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 400, 2 ** 63 - 1])
+@pytest.mark.parametrize("maxq", [1, 300])
+def test_attn_windows_wider_than_the_table(dev, window, maxq):
+    # and more tokens than keys, so that the first positions are negative
+    from sanic_b200 import RunError
+    args, keys, values = make_problem(dev, [40, 9], [0, 30], 4, 2, 64, "bf16", 16, seed=19)
+    args["kv_lens"] = ints(dev, [25, 39])
+    got, lse = dev.attn_paged(**args, max_query_len=maxq, window=window, return_lse=True)
+    dev.sync()
+    check_attention(got, lse, *plain_attention(args["q"], [keys[0][:25], keys[1]], [values[0][:25], values[1]], [40, 9], [25, 39], 0, 0.125))
+    wide = torch.zeros(1, (2 ** 31 - 300) // 16, dtype=torch.int32, device=dev.torch_device)       # positions would pass 32 bits
+    with pytest.raises(RunError, match="2\\^31 keys"):
+        dev.attn_paged(args["q"], args["k_pages"], args["v_pages"], wide, ints(dev, [0, 49]), ints(dev, [49]))
+
+
 FIRST_IN_CAPTURE = r'''
 import torch
 from sanic_b200 import CudaDevice
