@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(AT) page_append_kernel(const sanic_page_append
         }
         if (b < n) {
             s_tok[b + 1] = (int)min(bt + ct, (long long)p.n_tokens);
-            s_pg[b + 1] = (int)min(bp + cp, (long long)INT32_MAX);
+            s_pg[b + 1] = (int)min(bp + cp, 1ll << 30);      // a free list holds no more: what is beyond gets no pages
             bad |= bt + ct > p.n_tokens || bp + cp > free_n;
         }
         tok_carry += at; pg_carry += ap;
@@ -99,14 +99,14 @@ __global__ void __launch_bounds__(AT) page_append_kernel(const sanic_page_append
             while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (s_tok[mid] <= t) lo = mid; else hi = mid - 1; }
             const int seq = max(p.seq_lens[lo], 0), held = held_of(p, lo, seq);
             pos = (long long)seq + t - s_tok[lo];
-            const int idx = (int)(pos / p.page_size);
+            const long long idx = pos / p.page_size;
             int page = -1;
             if (idx < held) page = p.block_table[(int64_t)lo * p.table_stride + idx];      // entries of earlier steps: nobody writes them here
             else if (idx < p.max_pages) {
-                const int r = s_pg[lo] + idx - held;
+                const int r = s_pg[lo] + (int)idx - held;
                 if (r < free_n) page = p.free_pages[free_n - 1 - r];
             }
-            if (page >= 0) slot = (long long)page * p.page_size + pos - (long long)idx * p.page_size;
+            if (page >= 0) slot = (long long)page * p.page_size + pos - idx * p.page_size;
         }
         p.positions[t] = (int)min(pos, (long long)INT32_MAX);
         p.slots[t] = slot;
@@ -231,6 +231,7 @@ int32_t sanic_page_table_append(sanic_ctx* ctx, const sanic_page_append_params* 
     SANIC_REQUIRE(ctx, p->n_requests <= MAX_REQUESTS, "page_table_append: at most 8000 requests per call");
     SANIC_REQUIRE(ctx, p->n_tokens < (1 << 30), "page_table_append: too many token rows");
     SANIC_REQUIRE(ctx, p->page_size > 0 && p->max_pages > 0, "page_table_append: empty pages or table rows");
+    SANIC_REQUIRE(ctx, p->max_pages <= (1 << 30) && p->free_capacity <= (1 << 30), "page_table_append: too many pages");
     SANIC_REQUIRE(ctx, p->free_count && p->query_start && p->free_count_out, "page_table_append: null scalar or query_start");
     SANIC_REQUIRE(ctx, p->n_requests == 0 || (p->seq_lens && p->new_lens && p->block_table && p->kv_lens && p->pages_out),
                   "page_table_append: null tensor");

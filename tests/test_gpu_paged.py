@@ -590,6 +590,7 @@ def test_append_shortages_are_reported(dev):
     check_append(dev, [3, 3, 3], [10, 10, 10], 16, 4, 8, 17)                      # more new tokens than token rows
     check_append(dev, [-4, 9], [3, -2], 16, 4, 8, 6)                              # negative lengths read as 0
     check_append(dev, [(1 << 31) - 5, 3], [9, 4], 16, 4, 8, 13, held=[1, 1])      # a length that nearly wraps: no page, no slot
+    check_append(dev, [(1 << 31) - 5, 3], [9, 4], 1, 4, 8, 13, held=[1, 1])       # the same where a position is a page
     check_append(dev, [5], [2], 16, 4, 8, 2)                                      # and the next call is clean again
 
 
@@ -604,6 +605,12 @@ def test_append_refusals(dev):
     t = z(12)
     with pytest.raises(RunError, match="overlaps"):
         dev.page_table_append(**dict(args, block_table=t[:8].view(2, 4), seq_lens=t[6:8]))
+    from sanic_b200 import abi
+    x = t.data_ptr()
+    for max_pages, capacity in (((1 << 30) + 1, 4), (4, (1 << 30) + 1)):          # refused, nothing is read
+        p = abi.PageAppendParams(x, x, None, x, x, x, max_pages, x, x, x, x, x, x, 2, 4, 16, max_pages, capacity)
+        with pytest.raises(RunError, match="too many pages"):
+            dev._check(dev.lib.sanic_page_table_append(dev.h, C.byref(p), dev.stream()), "page_table_append")
 
 
 # ───────────────────────── cache writes ─────────────────────────
