@@ -52,6 +52,9 @@ struct __align__(16) Work {
     int whole, slot;       // the item's only segment; else the partial slot
 };
 constexpr int END = -1;    // n_tok of the entry behind the last segment
+// Waits for a segment last as long as the segments before it, not as one tile: a limit beyond any (at least 8 s; every other wait is
+// for one tile and ends these too when it runs out)
+constexpr uint32_t SEGMENT_SPINS = 1u << 28;
 
 template <int D> struct Shared {
     uint64_t q_full[2], q_empty[2], full[Tc<D>::NS], empty[Tc<D>::NS];
@@ -104,8 +107,9 @@ __device__ __forceinline__ bool elect_one() {
 }
 // Bounded wait of a role that is ahead of the others: asks and sleeps, and leaves the issue slots of its sub-partition to the
 // softmax warps (a suspended try_wait wakes and asks again often enough to cost them a tenth of their rate).
-__device__ __forceinline__ bool mbar_wait_idle(uint64_t* bar, uint32_t parity, uint32_t ns, volatile int* abort_flag, int* err, int code) {
-    for (uint32_t it = 0; it < (SPIN_LIMIT >> 2); ++it) {
+__device__ __forceinline__ bool mbar_wait_idle(uint64_t* bar, uint32_t parity, uint32_t ns, volatile int* abort_flag, int* err, int code,
+                                               uint32_t limit = SPIN_LIMIT >> 2) {
+    for (uint32_t it = 0; it < limit; ++it) {
         if (mbar_test(bar, parity)) return true;
         __nanosleep(ns);
         if ((it & 255u) == 255u && *abort_flag) return false;
@@ -165,7 +169,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     uint32_t n_seg = 0;
     auto next = [&](Work& w) {
         const int i = n_seg & 3;
-        if (!__all_sync(0xffffffffu, mbar_wait(&sh->seg_full[i], (n_seg >> 2) & 1, abortp, err, 15))) return false;
+        bool there = mbar_test(&sh->seg_full[i], (n_seg >> 2) & 1);
+        if (!there) there = mbar_wait_idle(&sh->seg_full[i], (n_seg >> 2) & 1, 32, abortp, err, 15, SEGMENT_SPINS);
+        if (!__all_sync(0xffffffffu, there)) return false;
         w = sh->seg[i];
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->seg_empty[i]);
@@ -576,7 +582,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         for (bool more = true; more; ++n_seg) {
             more = walk.next(p, g);
             const int i = n_seg & 3;
-            if (!__all_sync(0xffffffffu, mbar_wait_idle(&sh->seg_empty[i], ((n_seg >> 2) & 1) ^ 1, 256, abortp, err, 16))) break;
+            if (!__all_sync(0xffffffffu, mbar_wait_idle(&sh->seg_empty[i], ((n_seg >> 2) & 1) ^ 1, 256, abortp, err, 16, SEGMENT_SPINS))) break;
             if (lane == 0) {
                 Work w{};
                 w.n_tok = END;
