@@ -290,23 +290,26 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 const uint64_t vd = make_desc(ring_addr + slot * C::TILE, C::SLAB, 1024);
                 // the first PV of a segment overwrites O: the epilogue of the tile's previous segment must have read it
                 if (first && n_act[t] > 0) wait_on(&sh->o_free[t], (n_act[t] - 1) & 1, 18);
-                // A = P from tensor memory: 16 keys = 8 columns per step; the first 64 keys while the others' weights are computed
-                wait_on(&sh->p_half[t], n_pv[t] & 1, 20);
-                if (!ok) return;
-                fence_after();
-                if (leader) {
+                // A = P from tensor memory: 16 keys = 8 columns per step. head_dim 128: the first 64 keys while the others' weights are
+                // computed. (head_dim 64, where the exponentials set the pace, in one go: 8 sequences of 4096 keys 975 us, 999 in two.)
+                if (C::ALIAS) {
+                    wait_on(&sh->p_half[t], n_pv[t] & 1, 20);
+                    if (!ok) return;
+                    fence_after();
+                    if (leader) {
 #pragma unroll
-                    for (int kk = 0; kk < BN / 32; ++kk)
-                        umma_f16_ts(tmem + C::TM_O + t * D, tmem + C::TM_P + t * C::P_STEP + 8 * kk, vd + 128 * kk, idesc_pv, (!first || kk > 0) ? 1u : 0u);
+                        for (int kk = 0; kk < BN / 32; ++kk)
+                            umma_f16_ts(tmem + C::TM_O + t * D, tmem + C::TM_P + t * C::P_STEP + 8 * kk, vd + 128 * kk, idesc_pv, (!first || kk > 0) ? 1u : 0u);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
                 wait_on(&sh->p_full[t], n_pv[t] & 1, 19);
                 if (!ok) return;
                 fence_after();
                 if (leader) {
 #pragma unroll
-                    for (int kk = BN / 32; kk < BN / 16; ++kk)
-                        umma_f16_ts(tmem + C::TM_O + t * D, tmem + C::TM_P + t * C::P_STEP + 8 * kk, vd + 128 * kk, idesc_pv, 1u);
+                    for (int kk = C::ALIAS ? BN / 32 : 0; kk < BN / 16; ++kk)
+                        umma_f16_ts(tmem + C::TM_O + t * D, tmem + C::TM_P + t * C::P_STEP + 8 * kk, vd + 128 * kk, idesc_pv, (!first || kk > 0) ? 1u : 0u);
                     if (!C::ALIAS || j + 1 == s.je) umma_commit(&sh->pv_done[t]);
                     if (t == last_t) umma_commit(&sh->empty[slot]);
                 }
@@ -411,7 +414,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                         ok = __all_sync(0xffffffffu, n_it == 0 || mbar_wait(&sh->pv_done[t], (n_it - 1) & 1, abortp, err, 24));
                         if (!ok) break;
                     }
-                    if (lane == 0) { mbar_arrive(&sh->p_half[t]); mbar_arrive(&sh->p_full[t]); }
+                    if (lane == 0) {
+                        if (C::ALIAS) mbar_arrive(&sh->p_half[t]);
+                        mbar_arrive(&sh->p_full[t]);
+                    }
                     continue;
                 }
                 const int k0 = j * BN;
@@ -518,7 +524,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     const float p0 = ex2(x0), p1 = ex2(x1);
                     fadd2(sums[(2 * i) & 7], sums[(2 * i + 1) & 7], p0, p1);
                     r[i] = pack2<BF16>(p0, p1);
-                    if (i == 36) {        // by now the first half has landed: its product may start
+                    if (C::ALIAS && i == 36) {        // by now the first half has landed: its product may start
                         tmem_st_wait();
                         fence_before();
                         __syncwarp();
