@@ -153,47 +153,71 @@ template <bool BF16> __device__ __forceinline__ void store8(void* base, int64_t 
     *(uint4*)((uint16_t*)base + at) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// heads per thread, threads per block (at most). 8191 tokens of 32 + 2 * 8 heads of 128, f16 (206 MB): 42 us = 4.9 TB/s; 49 us with
-// two heads and 256 threads, 57 us with the rows asked for behind the slot.
+// A resident grid walks the tokens: the slot and position of a thread's next token are asked for under the rows of this one, so a
+// token costs one latency after the other only for its rows and rotation, which are asked for together.
+// HP heads per thread, WT threads per block. 8191 tokens of 32 + 2 * 8 heads of 128, f16 (206 MB): 36.9 us = 5.6 TB/s, 0.85 of the
+// measured copy rate; 41.7 us with a block per token (its slot, position, rotation in turn), 39.0 us with blocks of 256, 41.0 us with
+// four heads and four blocks per SM, 38.8 us with four times the resident blocks. (Stores marked as streaming: 35.8 us; not taken, since attention
+// reads q and the new keys next.)
 constexpr int HP = 3, WT = 128;
+template <typename S> constexpr int write_blocks() { return sizeof(Raw<S>) == 16 ? 5 : 4; }      // resident per SM
 
 template <typename S, bool BF16>
-__global__ void __launch_bounds__(WT, 6) paged_write_kernel(const __grid_constant__ sanic_paged_write_params p, const int tokens_per_block, const int page_shift, int* err) {
+__global__ void __launch_bounds__(WT, write_blocks<S>()) paged_write_kernel(const __grid_constant__ sanic_paged_write_params p, const int tokens_per_block, const int page_shift, int* err) {
     const int per_head = p.head_dim / 16, nq = p.q ? p.q_heads : 0, heads = nq + 2 * p.kv_heads, half = p.head_dim / 2;
     const int groups = (heads + HP - 1) / HP, per_token = groups * per_head;      // threads of a token
+    const int passes = (tokens_per_block * per_token + WT - 1) / WT;              // of a block over its tokens: more than one where one has many heads
+    const int64_t n_work = (int64_t)((p.n_tokens + tokens_per_block - 1) / tokens_per_block) * passes;
     griddep_wait();
     griddep_launch();
-    for (int i = threadIdx.x; i < tokens_per_block * per_token; i += blockDim.x) {
-        const int tl = i / per_token, rem = i - tl * per_token;
-        const int64_t t = (int64_t)blockIdx.x * tokens_per_block + tl;
-        if (t >= p.n_tokens) return;
+    // this thread's token and part of it in pass w, and what the row's address and rotation depend on
+    auto token = [&](int64_t w, int& rem) -> int64_t {
+        const int64_t g = passes == 1 ? w : w / passes;
+        const int i = threadIdx.x + (passes == 1 ? 0 : (int)(w - g * passes) * WT), tl = i / per_token;
+        rem = i - tl * per_token;
+        const int64_t t = g * tokens_per_block + tl;
+        return w < n_work && tl < tokens_per_block && t < p.n_tokens ? t : -1;
+    };
+    int64_t w = blockIdx.x;
+    int rem;
+    int64_t t = token(w, rem);
+    int64_t slot = t >= 0 ? p.slots[t] : -1;
+    int pos = t >= 0 && p.table ? p.positions[t] : 0;
+    for (; w < n_work; w += gridDim.x) {
         const int hg = rem / per_head, c = (rem - hg * per_head) * 8;
-        // everything that can be asked for is, before anything is waited for: the rows do not depend on the slot
-        const int64_t slot = p.slots[t];
-        const int pos = p.table ? p.positions[t] : 0;
         Raw<S> a_raw[HP], b_raw[HP];
-#pragma unroll
-        for (int u = 0; u < HP; ++u) {
-            const int hh = hg + u * groups;
-            if (hh >= heads) continue;
-            const bool is_q = hh < nq, is_k = !is_q && hh < nq + p.kv_heads;
-            const void* src = is_q ? p.q : is_k ? p.k : p.v;
-            const int64_t at = t * (is_q ? p.q_stride : is_k ? p.k_stride : p.v_stride) + (int64_t)(hh - (is_q ? 0 : is_k ? nq : nq + p.kv_heads)) * p.head_dim + c;
-            a_raw[u].load(src, at); b_raw[u].load(src, at + half);
-        }
-        if (slot < 0) continue;
-        if (slot >= (int64_t)p.n_pages * p.page_size || (p.table && (unsigned)pos >= (unsigned)p.n_positions)) {
+        bool ok = slot >= 0;
+        if (ok && (slot >= (int64_t)p.n_pages * p.page_size || (p.table && (unsigned)pos >= (unsigned)p.n_positions))) {
             if (rem == 0 && err) atomicCAS(err, 0, STATUS_WRITE);
-            continue;
+            ok = false;
+        }
+        if (ok) {
+#pragma unroll
+            for (int u = 0; u < HP; ++u) {
+                const int hh = hg + u * groups;
+                if (hh >= heads) continue;
+                const bool is_q = hh < nq, is_k = !is_q && hh < nq + p.kv_heads;
+                const void* src = is_q ? p.q : is_k ? p.k : p.v;
+                const int64_t at = t * (is_q ? p.q_stride : is_k ? p.k_stride : p.v_stride) + (int64_t)(hh - (is_q ? 0 : is_k ? nq : nq + p.kv_heads)) * p.head_dim + c;
+                a_raw[u].load(src, at); b_raw[u].load(src, at + half);
+            }
         }
         float cs[16];
-        if (p.table) {
-            const float4* w = (const float4*)(p.table + ((int64_t)pos * half + c) * 2);
+        if (ok && p.table) {
+            const float4* x = (const float4*)(p.table + ((int64_t)pos * half + c) * 2);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { const float4 x = __ldg(w + i); cs[4 * i] = x.x; cs[4 * i + 1] = x.y; cs[4 * i + 2] = x.z; cs[4 * i + 3] = x.w; }
+            for (int i = 0; i < 4; ++i) { const float4 y = __ldg(x + i); cs[4 * i] = y.x; cs[4 * i + 1] = y.y; cs[4 * i + 2] = y.z; cs[4 * i + 3] = y.w; }
         }
-        const int64_t page = page_shift >= 0 ? slot >> page_shift : (slot >> 32) == 0 ? (int64_t)((uint32_t)slot / (uint32_t)p.page_size) : slot / p.page_size;
-        const int64_t row = slot - page * p.page_size;
+        // the next token's, under this one's rows
+        const int64_t t_now = t, slot_now = slot;
+        int rem_next;
+        t = token(w + gridDim.x, rem_next);
+        slot = t >= 0 ? p.slots[t] : -1;
+        pos = t >= 0 && p.table ? p.positions[t] : 0;
+        rem = rem_next;
+        if (!ok) continue;
+        const int64_t page = page_shift >= 0 ? slot_now >> page_shift : (slot_now >> 32) == 0 ? (int64_t)((uint32_t)slot_now / (uint32_t)p.page_size) : slot_now / p.page_size;
+        const int64_t row = slot_now - page * p.page_size;
 #pragma unroll
         for (int u = 0; u < HP; ++u) {
             const int hh = hg + u * groups;
@@ -209,7 +233,7 @@ __global__ void __launch_bounds__(WT, 6) paged_write_kernel(const __grid_constan
                 }
             }
             void* dst = is_q ? p.q_out : is_k ? p.k_pages : p.v_pages;
-            const int64_t at = is_q ? t * p.q_out_stride + (int64_t)hh * p.head_dim + c
+            const int64_t at = is_q ? t_now * p.q_out_stride + (int64_t)hh * p.head_dim + c
                              : is_k ? page * p.k_page_stride + row * p.k_row_stride + (int64_t)(hh - nq) * p.k_head_stride + c
                                     : page * p.v_page_stride + row * p.v_row_stride + (int64_t)(hh - nq - p.kv_heads) * p.v_head_stride + c;
             store8<BF16>(dst, at, a); store8<BF16>(dst, at + half, b);
@@ -284,7 +308,8 @@ int32_t sanic_paged_cache_write(sanic_ctx* ctx, const sanic_paged_write_params* 
     sanic_set_device(ctx);
     const int heads = (p->q ? p->q_heads : 0) + 2 * p->kv_heads, per_token = (heads + HP - 1) / HP * (p->head_dim / 16);
     const int tpb = std::max(1, WT / per_token);
-    const dim3 grid((unsigned)((p->n_tokens + tpb - 1) / tpb)), block(std::min(WT, (tpb * per_token + 31) / 32 * 32));
+    const long long work = (long long)((p->n_tokens + tpb - 1) / tpb) * ((tpb * per_token + WT - 1) / WT);
+    const dim3 grid((unsigned)std::min<long long>(work, (long long)(src == 4 ? write_blocks<float>() : write_blocks<Bf16>()) * ctx->sm_count)), block(WT);
     int shift = -1;
     for (int i = 0; i < 31; ++i) if ((1 << i) == p->page_size) shift = i;
     cudaStream_t st = (cudaStream_t)stream;

@@ -685,6 +685,12 @@ def test_write_forms(dev):
     check_write(dev, 2500, 32, 8, 64, "bf16", "bf16", 16)
 
 
+@pytest.mark.parametrize("src,cache", [("bf16", "bf16"), ("f32", "f16")])
+@pytest.mark.parametrize("t,hq,hkv,d", [(5003, 32, 8, 128), (401, 64, 40, 256), (40001, 1, 1, 16), (9001, 5, 3, 48)])
+def test_write_more_tokens_than_resident_blocks(dev, src, cache, t, hq, hkv, d):
+    check_write(dev, t, hq, hkv, d, src, cache, 16, fused=src == "bf16", in_place=src == "bf16", seed=t)
+
+
 def test_write_out_of_range_is_reported_and_skipped(dev):
     from sanic_b200 import RunError
     td = dev.torch_device
