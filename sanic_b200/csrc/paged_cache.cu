@@ -14,6 +14,7 @@ using namespace sanic::paged;
 // memory, so every block takes the sums itself and then fills its own slice of the token rows, the table entries and the
 // per-request outputs: one launch, no hand-over between blocks, and the time of a decode step is the latency of two
 // dependent loads and a scan. Bytes only start to matter for the slots and positions of whole prompts (12 per token).
+// From a graph: 256 requests of one token 6.3 us, 48 prompts of 124,750 tokens together 8.3 us.
 constexpr int AT = 512;      // threads of a block
 
 struct AppendShared { int warp_pages[AT / 32], warp_tokens[AT / 32]; };
