@@ -535,7 +535,7 @@ int32_t launch_rows(sanic_ctx* ctx, const Params& p, bool tma, int ctas, cudaStr
     }
     CUtensorMap mk, mv;
     RowsArgs a{};
-    a.box_rows = std::min(p.page_size, KT);
+    a.box_rows = box_rows_of(p.page_size, KT);
     bool ki, vi;
     int32_t rc = encode_pool(ctx, &mk, BF16, p, 0, D, a.box_rows, &ki);
     if (rc == SANIC_OK) rc = encode_pool(ctx, &mv, BF16, p, 1, D, a.box_rows, &vi);

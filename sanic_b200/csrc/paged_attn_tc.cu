@@ -623,7 +623,7 @@ int32_t launch(sanic_ctx* ctx, const Params& p, int ctas, cudaStream_t st) {
     using C = Tc<D>;
     TcArgs a{};
     a.tile_tokens = p.block_tokens / 2;
-    a.box_rows = std::min(p.page_size, BN);
+    a.box_rows = box_rows_of(p.page_size, BN);
     CUtensorMap mq, mk, mv;
     {
         const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)p.q_heads, (cuuint64_t)p.n_tokens};

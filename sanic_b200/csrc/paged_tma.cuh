@@ -2,6 +2,7 @@
 // their strides, then pages), whose boxes are 64 columns of one head of a page's rows; 128-byte swizzle.
 #pragma once
 #include <algorithm>
+#include <numeric>
 
 #include "paged.cuh"
 #include "tc_common.cuh"
@@ -67,11 +68,17 @@ static inline int32_t encode_pool(sanic_ctx* ctx, CUtensorMap* map, bool bf16, c
     return encode_map(ctx, map, bf16, kv ? p.v : p.k, 4, dims, strides, box);
 }
 
-// Whether a tile of `tile` keys (64 or 128) is made of whole boxes: pages of 8, 16, 32, 64 .. rows up to a tile, or a multiple of
-// it; strides that nest.
+// Rows of a box: what divides both the page and the tile, so that a tile is made of whole boxes and none crosses a page's end.
+static inline int box_rows_of(int page_size, int tile) { return std::gcd(page_size, tile); }
+
+// Whether the pool can be read in tiles of `tile` keys (64 or 128): pages of a multiple of 8 rows (the swizzle's period, so that every box
+// starts on one); strides that nest.
+// 2048 tokens over 30,000 keys of 128: 970 us in pages of 16, 96 or 128 rows, 1030 of 48, 1410 of 24 and 1330 of 8 (boxes of 8 rows are
+// 1 KB each: their number bounds it), 4410 in pages of 20 (the rows form by 16-byte copies). 64 decodes of 8000 keys in pages of 16,
+// 48, 24, 8 and 20: 348, 355, 443, 417, 451 us.
 static inline bool pool_supported(const sanic_attn_paged_params* p, int tile) {
     const int ps = p->page_size;
-    if (!(ps % tile == 0 || (ps >= 8 && ps < tile && tile % ps == 0))) return false;
+    if (box_rows_of(ps, tile) < 8) return false;
     Pool pool;
     return pool_of(p->k_page_stride, p->k_row_stride, p->k_head_stride, p->n_pages, ps, p->kv_heads, p->head_dim, &pool) &&
            pool_of(p->v_page_stride, p->v_row_stride, p->v_head_stride, p->n_pages, ps, p->kv_heads, p->head_dim, &pool);

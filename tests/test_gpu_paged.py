@@ -157,6 +157,14 @@ def test_attn_long_chunks(dev, d, dtype, page, heads_first):
 
 
 @pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("maxq", [1, 200])
+@pytest.mark.parametrize("page,heads_first", [(8, True), (12, False), (20, True), (40, True), (48, False), (72, True), (96, False), (136, False), (1000, True)])
+def test_attn_odd_page_sizes(dev, d, maxq, page, heads_first):
+    # what the page and a tile have in common decides how much one copy takes: 8 rows up to a tile, or 16 bytes at a time
+    run_case(dev, [1, 75, 200, 3], [700, 513, 0, 1100], 6, 2, d, "bf16", page, heads_first=heads_first, window=333 if page == 72 else 0, seed=page, max_query_len=maxq)
+
+
+@pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("hq,hkv", [(2, 2), (7, 1), (12, 4), (64, 1), (33, 1)])
 @pytest.mark.parametrize("window", [0, 1, 100, 300])
 def test_attn_long_chunks_heads_and_windows(dev, d, hq, hkv, window):
