@@ -429,19 +429,20 @@ paged_rows_tma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     if (tid == 0) p.ws_merge[blockIdx.x] = merge;
 }
 
-// Merge of the items that several CTAs share, for one fold or for two that ran side by side. A block serves the item that starts
-// in one CTA's range (of the tensor-memory form with its up to 256 rows: an eighth of the item's rows): a row's partials are split over 16 / rows warps (at least one) and joined
-// through shared memory in a fixed order. Bound by latency: its start, an item's record, the partials (38 MB at most, in L2), the join;
-// 148 shared items of 256 rows 16-18 us.
+// Merge of the items that several CTAs share, for one fold or for two that ran side by side. The item that starts in one CTA's
+// range is served by a block per 16 rows of the rows form's items (24 drafted chunks of 3-6 tokens: 97.5 us with one block per item,
+// 95.7 so, 99 with a block per 8 rows), by eight blocks of the tensor-memory form's. A row's partials are split over 16 / rows warps
+// (at least one) and joined through shared memory in a fixed order. Bound by latency: its start, an item's record, the partials (38 MB
+// at most, in L2), the join; 148 shared items of 256 rows 16-18 us.
 constexpr int TC_MERGE_SPLIT = 8;      // blocks per item of the tensor-memory form
 struct Merge { const float* ws_o; const float2* ws_ml; const int4* ws_merge; int rows; };      // one fold's partials
 template <int D, bool BF16>
-__global__ void __launch_bounds__(512) paged_merge_kernel(const Merge first, const Merge second, const int n_first, void* out, float* lse, const int q_heads, const int group) {
+__global__ void __launch_bounds__(512) paged_merge_kernel(const Merge first, const Merge second, const int n_first, const int split_first, void* out, float* lse, const int q_heads, const int group) {
     griddep_wait();
     griddep_launch();
     const bool one = blockIdx.x < n_first;
-    const int cta = one ? blockIdx.x : (blockIdx.x - n_first) / TC_MERGE_SPLIT;
-    const int part = one ? 0 : (blockIdx.x - n_first) % TC_MERGE_SPLIT, n_parts = one ? 1 : TC_MERGE_SPLIT;
+    const int n_parts = one ? split_first : TC_MERGE_SPLIT, block = one ? blockIdx.x : blockIdx.x - n_first;
+    const int cta = block / n_parts, part = block - cta * n_parts;
     // field by field: a reference to one of two parameters would be read through memory at every use
     const float* ws_o = one ? first.ws_o : second.ws_o;
     const float2* ws_ml = one ? first.ws_ml : second.ws_ml;
@@ -616,9 +617,10 @@ int32_t validate(sanic_ctx* ctx, const sanic_attn_paged_params* p) {
 
 namespace {
 cudaError_t launch_merge(const Params& a, int n_a, const Params& b, int n_b, int D, int dtype, cudaStream_t st) {
-    const dim3 grid(n_a + n_b * TC_MERGE_SPLIT), block(512);
+    const int split = std::max(1, a.rows / 16);
+    const dim3 grid(n_a * split + n_b * TC_MERGE_SPLIT), block(512);
     const Merge x{a.ws_o, a.ws_ml, a.ws_merge, a.rows}, y{b.ws_o, b.ws_ml, b.ws_merge, b.rows};
-    auto go = [&](auto kernel) { return launch_pdl(kernel, grid, block, 0, st, x, y, n_a, a.out, a.lse, a.q_heads, a.group); };
+    auto go = [&](auto kernel) { return launch_pdl(kernel, grid, block, 0, st, x, y, n_a * split, split, a.out, a.lse, a.q_heads, a.group); };
     if (D == 128) return dtype == SANIC_BF16 ? go(paged_merge_kernel<128, true>) : go(paged_merge_kernel<128, false>);
     return dtype == SANIC_BF16 ? go(paged_merge_kernel<64, true>) : go(paged_merge_kernel<64, false>);
 }
