@@ -431,10 +431,11 @@ paged_rows_tma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 
 // Merge of the items that several CTAs share, for one fold or for two that ran side by side. The item that starts in one CTA's
 // range is served by a block per 16 rows of the rows form's items (24 drafted chunks of 3-6 tokens: 97.5 us with one block per item,
-// 95.7 so, 99 with a block per 8 rows), by eight blocks of the tensor-memory form's. A row's partials are split over 16 / rows warps
+// 95.7 so, 99 with a block per 8 rows), by four blocks of the tensor-memory form's (all resident at once: 16 drafted chunks of 16 tokens 78.3
+// us, 81.2 with eight, 87.8 with 16; two or four rows of a warp at once: 79.5-85). A row's partials are split over 16 / rows warps
 // (at least one) and joined through shared memory in a fixed order. Bound by latency: its start, an item's record, the partials (38 MB
 // at most, in L2), the join; 148 shared items of 256 rows 16-18 us.
-constexpr int TC_MERGE_SPLIT = 8;      // blocks per item of the tensor-memory form
+constexpr int TC_MERGE_SPLIT = 4;      // blocks per item of the tensor-memory form
 struct Merge { const float* ws_o; const float2* ws_ml; const int4* ws_merge; int rows; };      // one fold's partials
 template <int D, bool BF16>
 __global__ void __launch_bounds__(512) paged_merge_kernel(const Merge first, const Merge second, const int n_first, const int split_first, void* out, float* lse, const int q_heads, const int group) {
