@@ -16,6 +16,7 @@ using namespace sanic::paged;
 // dependent loads and a scan. Bytes only start to matter for the slots and positions of whole prompts (12 per token).
 // From a graph: 256 requests of one token 6.3 us, 48 prompts of 124,750 tokens together 8.3 us.
 constexpr int AT = 512;      // threads of a block
+constexpr int append_smem(int n_requests) { return (2 * n_requests + 2) * 4; }
 
 struct AppendShared { int warp_pages[AT / 32], warp_tokens[AT / 32]; };
 
@@ -274,8 +275,14 @@ int32_t sanic_page_table_append(sanic_ctx* ctx, const sanic_page_append_params* 
     for (int i = 0; i < 5; ++i)
         SANIC_REQUIRE(ctx, !overlaps(in[5].ptr, in[5].n, in[i].ptr, in[i].n), "page_table_append: the table overlaps an input");
     sanic_set_device(ctx);
-    const int smem = (2 * p->n_requests + 2) * 4;
-    if (smem > 48 * 1024) SANIC_CUDA_CHECK(ctx, cudaFuncSetAttribute(page_append_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    // The limit is the largest batch's for every call: it is one value per function and device, so a call that set it to its own size
+    // could lower it between another thread's set and launch; and static shared memory counts towards the 48 KB that need none.
+    static thread_local int ready_on = -1;
+    if (ready_on != ctx->device) {
+        SANIC_CUDA_CHECK(ctx, cudaFuncSetAttribute(page_append_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, append_smem(MAX_REQUESTS)));
+        ready_on = ctx->device;
+    }
+    const int smem = append_smem(p->n_requests);
     // a block's slice: about four token rows or requests per thread, at most two blocks per SM
     const long long rows = std::max<long long>(p->n_tokens, p->n_requests);
     const int blocks = (int)std::min<long long>(std::max<long long>(1, (rows + 4 * AT - 1) / (4 * AT)), 2 * ctx->sm_count);

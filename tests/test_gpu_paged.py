@@ -621,6 +621,54 @@ def test_append_refusals(dev):
             dev._check(dev.lib.sanic_page_table_append(dev.h, C.byref(p), dev.stream()), "page_table_append")
 
 
+APPEND_COUNTS = r'''
+import threading
+import torch
+from sanic_b200 import CudaDevice
+
+def step(dev, n, stream=None):
+    """n requests of one new token each, a page each off the end of the free list."""
+    i32 = dict(dtype=torch.int32, device="cuda")
+    seq, new, table = torch.zeros(n, **i32), torch.ones(n, **i32), torch.full((n, 2), -1, **i32)
+    free = torch.arange(n, **i32)
+    got = dev.page_table_append(seq, new, table, free, torch.full((1,), n, **i32), 16, n)
+    dev.sync()
+    assert table[:, 0].tolist() == list(range(n - 1, -1, -1)) and (table[:, 1] == -1).all()
+    assert got.query_start.tolist() == list(range(n + 1)) and got.free_count.item() == 0
+    assert got.slots.tolist() == [16 * (n - 1 - b) for b in range(n)]
+
+dev = CudaDevice(0)
+for n in COUNTS:
+    step(dev, n)
+failed = []
+def many(counts):
+    try:
+        mine = CudaDevice(0)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(15):
+                for n in counts:
+                    step(mine, n)
+    except BaseException as e:
+        failed.append(e)
+threads = [threading.Thread(target=many, args=(c,)) for c in ((6200, 7000), (8000, 6500), (7999, 6144))]
+for t in threads: t.start()
+for t in threads: t.join()
+assert not failed, failed
+print("appended")
+'''
+
+
+@pytest.mark.parametrize("counts", [(6127, 6128), (6135,), (6143, 6144), (8000, 6140)])
+def test_append_counts_around_the_default_shared_memory(counts):
+    # the first calls of a process: no larger call has raised the kernel's limit before; then threads with counts of their own
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", APPEND_COUNTS.replace("COUNTS", repr(counts))], cwd=root, capture_output=True, text=True, timeout=180)
+    assert r.returncode == 0 and "appended" in r.stdout, r.stderr[-2000:]
+
+
 # ───────────────────────── cache writes ─────────────────────────
 def check_write(dev, t, hq, hkv, d, src, cache, page, heads_first=False, fused=False, rope=True, with_q=True, in_place=False, seed=0):
     g = gen(dev, seed)
