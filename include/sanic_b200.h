@@ -571,8 +571,10 @@ int32_t sanic_machine_state(sanic_replay* m, const char* name, sanic_buffer_view
  * (seq + new), pages_out (pages the row holds now), *free_count_out, and per token row of the step its position and slot
  * (page * page_size + row). Token rows behind the last request get slot -1 and position 0.
  * A request that finds the list empty or its table row full keeps what it got: the missing entries are -1 (where the row has
- * room for them), the tokens in them get slot -1, and code 53 is reported; so are a negative length (read as 0) and new
- * tokens beyond n_tokens (query_start stops there). Outputs may not overlap inputs; block_table is updated in place. */
+ * room for them), the tokens in them get slot -1, and code 53 is reported. So are a negative length (read as 0), new tokens beyond
+ * n_tokens (query_start stops there), a held count outside [0, max_pages] or a free count outside [0, free_capacity] (the nearest
+ * value inside is used), a negative page taken off the free list (entry and slots -1; it counts as taken), and a negative entry
+ * in the held part of a row where a new token would stand (slot -1). Outputs may not overlap inputs; block_table is updated in place. */
 typedef struct {
     const int32_t* seq_lens; const int32_t* new_lens; const int32_t* held_pages;     /* [n_requests] */
     const int32_t* free_pages; const int32_t* free_count;                           /* [free_capacity], device scalar */

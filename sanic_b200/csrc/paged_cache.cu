@@ -20,9 +20,16 @@ constexpr int append_smem(int n_requests) { return (2 * n_requests + 2) * 4; }
 
 struct AppendShared { int warp_pages[AT / 32], warp_tokens[AT / 32]; };
 
-__device__ __forceinline__ int held_of(const sanic_page_append_params& p, int b, int seq) {
+// Pages that a row holds, inside the row; `bad` is set where the count given was not.
+__device__ __forceinline__ int held_of(const sanic_page_append_params& p, int b, int seq, bool& bad) {
     const int h = p.held_pages ? p.held_pages[b] : (int)(((long long)seq + p.page_size - 1) / p.page_size);
-    return min(max(h, 0), p.max_pages);
+    const int inside = min(max(h, 0), p.max_pages);
+    bad |= inside != h;
+    return inside;
+}
+__device__ __forceinline__ int held_of(const sanic_page_append_params& p, int b, int seq) {
+    bool reported = false;
+    return held_of(p, b, seq, reported);
 }
 
 __global__ void __launch_bounds__(AT) page_append_kernel(const sanic_page_append_params p, int* err) {
@@ -33,9 +40,9 @@ __global__ void __launch_bounds__(AT) page_append_kernel(const sanic_page_append
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = p.n_requests;
     griddep_wait();
     griddep_launch();
-    const int free_n = min(max(*p.free_count, 0), p.free_capacity);
+    const int free_given = *p.free_count, free_n = min(max(free_given, 0), p.free_capacity);
     long long tok_carry = 0, pg_carry = 0;
-    bool bad = false;
+    bool bad = free_n != free_given;
     if (tid == 0) { s_tok[0] = 0; s_pg[0] = 0; }
     for (int b0 = 0; b0 < n; b0 += AT) {
         const int b = b0 + tid;
@@ -46,7 +53,7 @@ __global__ void __launch_bounds__(AT) page_append_kernel(const sanic_page_append
             tok = min(max(add, 0), p.n_tokens + 1);      // more than the token rows there are: reported below, and the sums stay small
             const long long need = ((long long)max(seq, 0) + max(add, 0) + p.page_size - 1) / p.page_size;
             bad |= need > p.max_pages;
-            pg = max(0, (int)min(need, (long long)p.max_pages) - held_of(p, b, max(seq, 0)));
+            pg = max(0, (int)min(need, (long long)p.max_pages) - held_of(p, b, max(seq, 0), bad));
         }
         int ct = tok, cp = pg;
 #pragma unroll
@@ -83,14 +90,18 @@ __global__ void __launch_bounds__(AT) page_append_kernel(const sanic_page_append
         p.query_start[0] = 0;
         *p.free_count_out = (int)max(0ll, (long long)free_n - pg_carry);
     }
-    if (bad && blockIdx.x == 0 && err) atomicCAS(err, 0, STATUS_POOL);
+    bad &= blockIdx.x == 0;                      // every block found the same so far
+    // the r-th page taken; -1 where the list ends before it or holds no page there
+    auto taken_page = [&](int r) { return r < free_n ? max(p.free_pages[free_n - 1 - r], -1) : -1; };
     // table entries: the taken pages of all requests, in order
     const int taken = s_pg[n];
     for (int r = first; r < taken; r += stride) {
         int lo = 0, hi = n - 1;                  // the last request with s_pg[b] <= r
         while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (s_pg[mid] <= r) lo = mid; else hi = mid - 1; }
         const int col = held_of(p, lo, max(p.seq_lens[lo], 0)) + r - s_pg[lo];
-        p.block_table[(int64_t)lo * p.table_stride + col] = r < free_n ? p.free_pages[free_n - 1 - r] : -1;
+        const int page = taken_page(r);
+        bad |= page < 0;
+        p.block_table[(int64_t)lo * p.table_stride + col] = page;
     }
     // token rows
     const int used = s_tok[n];
@@ -104,15 +115,14 @@ __global__ void __launch_bounds__(AT) page_append_kernel(const sanic_page_append
             const long long idx = pos / p.page_size;
             int page = -1;
             if (idx < held) page = p.block_table[(int64_t)lo * p.table_stride + idx];      // entries of earlier steps: nobody writes them here
-            else if (idx < p.max_pages) {
-                const int r = s_pg[lo] + (int)idx - held;
-                if (r < free_n) page = p.free_pages[free_n - 1 - r];
-            }
+            else if (idx < p.max_pages) page = taken_page(s_pg[lo] + (int)idx - held);
+            bad |= page < 0;
             if (page >= 0) slot = (long long)page * p.page_size + pos - idx * p.page_size;
         }
         p.positions[t] = (int)min(pos, (long long)INT32_MAX);
         p.slots[t] = slot;
     }
+    if (bad && err) atomicCAS(err, 0, STATUS_POOL);
 }
 
 // ── paged_cache_write ──

@@ -602,6 +602,41 @@ def test_append_shortages_are_reported(dev):
     check_append(dev, [5], [2], 16, 4, 8, 2)                                      # and the next call is clean again
 
 
+@pytest.mark.parametrize("n", [2, 700])
+def test_append_counts_and_entries_out_of_range_are_reported(dev, n):
+    # the last two requests are looked at, behind none or more than a block's worth of others that append nothing
+    from sanic_b200 import RunError
+    td = dev.torch_device
+
+    def step(held=(1, 1), count=4, free=(40, 41, 42, 43), entry=7, report=True, seq=(15, 16), new=(3, 2)):
+        pad = n - 2
+        table = torch.full((n, 4), -7, dtype=torch.int32, device=td)
+        table[pad, 0], table[pad + 1, 0] = entry, 9
+        got = dev.page_table_append(ints(dev, [0] * pad + list(seq)), ints(dev, [0] * pad + list(new)), table, ints(dev, list(free)), ints(dev, [count]),
+                                    16, sum(new), held_pages=ints(dev, [0] * pad + list(held)))
+        if report:
+            with pytest.raises(RunError, match="code 53"):
+                dev.sync()
+        dev.sync()
+        assert got.query_start.tolist()[pad:] == [0, new[0], new[0] + new[1]]
+        return table[pad:].tolist(), got.held_pages.tolist()[pad:], got.free_count.item(), got.slots.tolist()
+
+    good = [[7, 43, -7, -7], [9, 42, -7, -7]], [2, 2], 2, [7 * 16 + 15, 43 * 16, 43 * 16 + 1, 42 * 16, 42 * 16 + 1]
+    assert step(report=False) == good
+    # a count of free pages outside the list: nothing is read behind it, none taken in front of it
+    assert step(count=9) == good
+    assert step(count=-1) == ([[7, -1, -7, -7], [9, -1, -7, -7]], [1, 1], 0, [7 * 16 + 15, -1, -1, -1, -1])
+    # counts of held pages outside a table row: the nearest count inside it
+    assert step(held=(-2, 1)) == ([[43, 42, -7, -7], [9, 41, -7, -7]], [2, 2], 1, [43 * 16 + 15, 42 * 16, 42 * 16 + 1, 41 * 16, 41 * 16 + 1])
+    assert step(held=(1, 5))[:3] == ([[7, 43, -7, -7], [9, -7, -7, -7]], [2, 4], 3)
+    # a negative page that a new token would use: no slot; one that no new token uses is not looked at
+    assert step(entry=-1) == ([[-1, 43, -7, -7], [9, 42, -7, -7]], [2, 2], 2, [-1, 43 * 16, 43 * 16 + 1, 42 * 16, 42 * 16 + 1])
+    assert step(entry=-1, seq=(16, 16), new=(2, 2), report=False)[3] == [43 * 16, 43 * 16 + 1, 42 * 16, 42 * 16 + 1]
+    # a negative page on the free list: a missing one
+    assert step(free=(40, 41, 42, -3)) == ([[7, -1, -7, -7], [9, 42, -7, -7]], [2, 2], 2, [7 * 16 + 15, -1, -1, 42 * 16, 42 * 16 + 1])
+    assert step(report=False) == good
+
+
 def test_append_refusals(dev):
     from sanic_b200 import RunError
     z = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev.torch_device)
