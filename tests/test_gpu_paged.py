@@ -637,6 +637,21 @@ def test_append_counts_and_entries_out_of_range_are_reported(dev, n):
     assert step(report=False) == good
 
 
+def test_append_with_an_empty_free_list(dev):
+    # a list without any memory: enough where no request needs a page
+    from sanic_b200 import RunError
+    none = torch.zeros(0, dtype=torch.int32, device=dev.torch_device)
+    for new, want, held in (([1, 0], [7 * 16 + 15], [1, 2]), ([2, 0], [7 * 16 + 15, -1], [1, 2])):
+        table = ints(dev, [[7, -7], [8, 9]])
+        got = dev.page_table_append(ints(dev, [15, 20]), ints(dev, new), table, none, ints(dev, [0]), 16, sum(new))
+        if -1 in want:
+            with pytest.raises(RunError, match="code 53"):
+                dev.sync()
+        dev.sync()
+        assert got.slots.tolist() == want and got.held_pages.tolist() == held and got.free_count.item() == 0
+        assert table.tolist() == [[7, -1 if -1 in want else -7], [8, 9]]
+
+
 def test_append_refusals(dev):
     from sanic_b200 import RunError
     z = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev.torch_device)
