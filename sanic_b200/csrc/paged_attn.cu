@@ -565,9 +565,11 @@ Plan make_plan(const sanic_ctx* ctx, const sanic_attn_paged_params* p) {
     pl.tc = want > TC_ABOVE_ROWS && tc_supported(p);
     if (pl.tc) {
         // A batch may hold single tokens beside its chunks: those are the rows form's, in a launch of their own (28 decodes beside
-        // four chunks of 300-600 tokens: 145 us in one launch of the tensor-memory form)
+        // four chunks of 300-600 tokens: 145 us in one launch of the tensor-memory form). Not where the single tokens of a large
+        // group are all there is: one launch (64 requests of one token, 64 heads of 128 to a kv head, 4000 keys: 45 us; in the
+        // rows form 56, in both 58; head_dim 64: 37, 38, 41)
         pl.tc_ctas = ctx->sm_count;
-        pl.rows = p->n_requests > 1 ? pow2_rows(group) : 0;
+        pl.rows = p->n_requests > 1 && want > pow2_rows(group) ? pow2_rows(group) : 0;
     } else {
         pl.rows = pow2_rows(want);
     }

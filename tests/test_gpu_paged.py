@@ -354,6 +354,25 @@ def test_attn_outputs_and_workspaces_on_16_byte_boundaries(dev, d, maxq):
         dev._check(dev.lib.sanic_attn_paged(dev.h, C.byref(p), dev.stream()), "attn_paged")
 
 
+@pytest.mark.parametrize("hq,hkv", [(64, 1), (40, 1), (66, 2)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attn_single_tokens_of_large_groups_are_one_launch(dev, hq, hkv, d):
+    # every token's rows fit one form: a batch of them has the workspace of that form alone, as a single request has
+    from sanic_b200 import abi
+    x = torch.zeros(16, dtype=torch.int32, device=dev.torch_device).data_ptr()
+
+    def size(n, maxq):      # nothing is launched: the addresses are only looked at
+        p = abi.AttnPagedParams(x, x, None, x, x, x, x, x, None, 0, hq * d, d, 16 * hkv * d, hkv * d, d, 16 * hkv * d, hkv * d, d, 4, abi.BF16, n, n * maxq,
+                                maxq, hq, hkv, d, 16, 4 * n, 4, 0, 1.0)
+        return dev.lib.sanic_attn_paged_workspace_bytes(dev.h, C.byref(p))
+
+    assert size(1, 1) == size(2, 1) == size(1000, 1) > 0
+    assert size(2, 2) > size(1, 2)                        # single tokens beside chunks of two: two launches
+    ctx = [0, 700, 31, 32, 5, 2000]
+    run_case(dev, [1] * 6, ctx, hq, hkv, d, "bf16", 16, seed=hq)
+    run_case(dev, [1, 1, 3, 1, 0, 1], ctx, hq, hkv, d, "f16", 16, seed=hq, max_query_len=1)        # the hint is too small
+
+
 @pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 400, 2 ** 63 - 1])
 @pytest.mark.parametrize("maxq", [1, 300])
 def test_attn_windows_wider_than_the_table(dev, window, maxq):
