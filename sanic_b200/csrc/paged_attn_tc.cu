@@ -57,8 +57,10 @@ struct __align__(16) Work {
     int whole, slot;       // the item's only segment; else the partial slot
 };
 constexpr int END = -1;    // n_tok of the entry behind the last segment
-// Waits for a segment last as long as the segments before it, not as one tile: a limit beyond any (at least 8 s; every other wait is
-// for one tile and ends these too when it runs out)
+// Waits for a segment last as long as the segments before it, not as one tile, and so may a wait for scores: tile 1 passes over
+// segments without rows for it that tile 0 still folds, whatever their length. A limit of their own, then: 16 times that of the
+// other waits (in probes, so no exact time: a sleep asked for 32 ns takes anything from none to 64). Those are for one tile
+// each, and end these too when they run out.
 constexpr uint32_t SEGMENT_SPINS = 1u << 28;
 
 template <int D> struct Shared {
@@ -405,7 +407,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             const bool busy = __any_sync(0xffffffffu, valid);      // a warp without rows only keeps the barriers' count
             for (int j = s.jb; j < s.je && ok; ++j, ++n_it) {
                 const bool first = j == s.jb;
-                if (!scores_ready) ok = mbar_wait(&sh->s_full[t], n_it & 1, abortp, err, 21);
+                if (!scores_ready) ok = mbar_wait(&sh->s_full[t], n_it & 1, abortp, err, 21, SEGMENT_SPINS);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 scores_ready = false;

@@ -171,6 +171,14 @@ def test_attn_long_chunks_heads_and_windows(dev, d, hq, hkv, window):
     run_case(dev, [257, 70, 1, 0, 128], [5, 600, 900, 40, 0], hq, hkv, d, "bf16", 16, window=window, seed=hq + window)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_attn_blocks_of_one_tile_before_blocks_of_two(dev, d):
+    # every head's items are a block of two tiles and one of a single row; an uneven number of them per CTA, so that the second
+    # tile's warps pass over long segments that the first tile still folds and wait for their own behind those
+    run_case(dev, [257], [3000], 222, 222, d, "bf16", 64, seed=d)
+    run_case(dev, [257, 129, 2], [700, 1500, 900], 96, 96, d, "f16", 16, seed=d + 1)
+
+
 @pytest.mark.parametrize("d,dtype", [(64, "bf16"), (128, "f16")])
 def test_attn_splits_a_long_cache(dev, d, dtype):
     # few items over a long key axis: every CTA of the device holds a part, and the parts are merged
