@@ -611,10 +611,10 @@ int32_t sanic_paged_cache_write(sanic_ctx* ctx, const sanic_paged_write_params* 
  * query_start[b], and sees the keys at or before it, at most `window` of them when window > 0. The chunk's own keys are in
  * the pages already. out [n_tokens, q_heads, head_dim] at dtype, dense; lse (optional) [n_tokens, q_heads] f32, the natural
  * log of the sum of exp(scale q.k). A token that sees no key (position < 0) gets zeros and -inf. Rows of q outside every
- * request's range, and their out and lse, are neither read for a result nor written. Keys no token of the request sees
- * (behind kv_lens, before the window) do not count, whatever the pages hold there; a key that some token of the chunk sees is
- * read once for many of them, and a value row of it that is not finite may make NaN of tokens it is hidden from. Scores, maxima, sums and the output
- * accumulator are f32; the weights exp(s - max) are rounded to dtype for the product with v. max_query_len, a bound on the
+ * request's range, and their out and lse, are neither read for a result nor written. Keys that a token does not see (behind it, before
+ * its window, behind kv_lens) do not count for it, whatever the pages hold there, infinities and NaN included. (Where later tokens of
+ * a chunk hold such values, the earlier ones are folded again one by one, which takes some milliseconds.) out and lse overlap no
+ * input. Scores, maxima, sums and the output accumulator are f32; the weights exp(s - max) are rounded to dtype for the product with v. max_query_len, a bound on the
  * chunk lengths (0: n_tokens), only selects a kernel: a longer chunk is still computed. dtype SANIC_BF16 or SANIC_F16,
  * head_dim 64 or 128, at most 64 query heads per kv head. A table entry outside [0, n_pages) reads as zeros; it, and lengths
  * past the table row or n_tokens (clamped), are reported (code 54). Any page size and strides are served; fastest are pages of a

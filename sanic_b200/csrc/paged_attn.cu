@@ -15,6 +15,8 @@
 // softmax out of f16's subnormals), sums and maxima are f32.
 // The work is spread over an exactly resident grid as one contiguous range of (item, key tile) per CTA (paged_sched.h).
 // 64 decodes of 8000 keys on average, 32 + 8 heads of 128, bf16 (2.14 GB): 340 us = 6.3 TB/s, 0.96 of the measured copy rate.
+#include <type_traits>
+
 #include "paged_tma.cuh"
 
 namespace {
@@ -84,8 +86,9 @@ template <int D, int MT, bool BF16> struct Fold {
     int lo_a, lo_c;                      // keys a row sees: [lo, lo + cnt)
     unsigned cnt_a, cnt_c;
     int inner_lo, inner_hi;              // every row of the item sees the whole of a tile between these
+    bool nan_met;                        // a result held a NaN in a segment that hides keys from some of its rows (see repair)
 
-    __device__ __forceinline__ void place(int warp, int lane_) { wr = warp % MT; wk = warp / MT; lane = lane_; g = lane >> 2; t = lane & 3; }
+    __device__ __forceinline__ void place(int warp, int lane_) { wr = warp % MT; wk = warp / MT; lane = lane_; g = lane >> 2; t = lane & 3; nan_met = false; }
     __device__ __forceinline__ int ra() const { return wr * 16 + g; }
 
     // row r of the item is head r % group of token r / group
@@ -206,6 +209,7 @@ template <int D, int MT, bool BF16> struct Fold {
         const bool whole = s.starts && s.finishes;
         const size_t slot = partial_slot(s, blockIdx.x);
         const int rows = n_tok * p.group;
+        const bool hides = min(s.hi, s.je * KT) > inner_hi || max(s.lo, s.jb * KT) < inner_lo;
         for (int idx = tid; idx < rows * (D / 4); idx += 128) {
             const int r = idx / (D / 4), d = (idx % (D / 4)) * 4, c = d ^ ((r & 3) << 3);
             float m = -INFINITY, l = 0.0f;
@@ -220,6 +224,8 @@ template <int D, int MT, bool BF16> struct Fold {
                 l += f * x.y;
                 acc.x += f * v4.x; acc.y += f * v4.y; acc.z += f * v4.z; acc.w += f * v4.w;
             }
+            const float all4 = (acc.x + acc.y) + (acc.z + acc.w);
+            nan_met |= hides && all4 != all4;
             if (whole) {
                 const int tok = r / p.group, head = s.hk * p.group + r - tok * p.group;
                 const int64_t at = (int64_t)(s.r.q0 + block0 + tok) * p.q_heads + head;
@@ -235,8 +241,58 @@ template <int D, int MT, bool BF16> struct Fold {
     }
 };
 
-// Any layout: the four warps copy the tiles themselves, 16 bytes a time (cp.async).
-template <int D, int MT, bool BF16>
+// Writes a row that was folded again: four columns per lane of the first D / 4 lanes.
+template <bool BF16> __device__ __forceinline__ void store4(const Params& p, int64_t at, const float (&acc)[4], float inv) {
+    *(uint2*)((uint16_t*)p.out + at) = make_uint2(pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv));
+}
+template <bool BF16> __device__ __forceinline__ bool holds_nan(const Params& p, int64_t at) {      // the same four columns of the result
+    const uint2 x = __ldcg((const uint2*)((const uint16_t*)p.out + at));
+    float v[4];
+    widen2<BF16>(x.x, v[0], v[1]); widen2<BF16>(x.y, v[2], v[3]);
+    return v[0] != v[0] || v[1] != v[1] || v[2] != v[2] || v[3] != v[3];
+}
+
+// Where the rows form is alone, its CTAs that met a NaN while some key of a segment was hidden from some of its rows go over their
+// segments once more at their end (128 threads that meet at `sync`; `cum`, shared memory, is free again): such rows that hold a
+// NaN are folded again over the keys of the segment that they see (fold_row), a warp per row. 24 drafted chunks 0.5-1.5 us slower for it.
+template <int D, bool BF16, class Sync>
+__device__ __noinline__ void repair(const Params& p, long long* cum, int tid, Sync sync) {
+    const int warp = tid >> 5, lane = tid & 31, col = (lane % (D / 4)) * 4;
+    scan_costs<KT>(p, cum, nullptr, tid, 128, sync);
+    DeviceWalk<KT> walk{LoadReq{&p, nullptr}};
+    walk.init(p, cum, blockIdx.x, gridDim.x);
+    Seg s;
+    while (walk.next(p, s)) {
+        const int block0 = s.rb * p.block_tokens, n_tok = min(p.block_tokens, s.r.qn - block0), pos0 = s.r.kv - s.r.qn + block0;
+        const int first_key = max(s.lo, s.jb * KT), end_key = min(s.hi, s.je * KT);
+        const bool whole = s.starts && s.finishes;
+        for (int r = warp; r < n_tok * p.group; r += 4) {
+            const int tok = r / p.group, head = s.hk * p.group + r - tok * p.group, pos = pos0 + tok;
+            const int k0 = max(first_key, p.window > 0 ? max(0, pos - p.window + 1) : 0), k1 = min(end_key, max(0, pos + 1));
+            if (k0 == first_key && k1 == end_key) continue;
+            const int64_t at = ((int64_t)(s.r.q0 + block0 + tok) * p.q_heads + head) * D + col;
+            const size_t slot_row = (size_t)partial_slot(s, blockIdx.x) * p.rows + r;
+            float4* part = (float4*)(p.ws_o + slot_row * D + col);
+            bool lost;
+            if (whole) lost = holds_nan<BF16>(p, at);
+            else { const float4 x = __ldcg(part); lost = x.x != x.x || x.y != x.y || x.z != x.z || x.w != x.w; }
+            if (!__any_sync(0xffffffffu, lost)) continue;
+            const uint16_t* q = (const uint16_t*)p.q + (int64_t)(s.r.q0 + block0 + tok) * p.q_token_stride + (int64_t)head * p.q_head_stride;
+            float m, l, acc[4];
+            const bool summed = fold_row<D, BF16>(p, s.b, s.hk, q, k0, k1, p_shift<BF16>(), col, m, l, acc);
+            if (lane >= D / 4) continue;
+            if (whole) store4<BF16>(p, at, acc, summed && l > 0.0f ? 1.0f / l : 0.0f);
+            else {
+                *part = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                if (lane == 0 && summed) p.ws_ml[slot_row] = make_float2(m, l);
+            }
+        }
+    }
+}
+
+// Any layout: the four warps copy the tiles themselves, 16 bytes a time (cp.async). ALONE: no tensor-memory form beside (its merge looks at
+// both forms' results, and a longer kernel in front of it costs 3-5 us).
+template <int D, int MT, bool BF16, bool ALONE>
 __global__ void __launch_bounds__(128) paged_rows_kernel(const __grid_constant__ Params p, int* err) {
     constexpr int STAGES = Cfg<D>::STAGES;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -307,6 +363,7 @@ __global__ void __launch_bounds__(128) paged_rows_kernel(const __grid_constant__
         __syncthreads();
     }
     if (tid == 0) p.ws_merge[blockIdx.x] = merge;
+    if (ALONE && __syncthreads_or(f.nan_met)) repair<D, BF16>(p, (long long*)smem, tid, [] { __syncthreads(); });
 }
 
 // Pools that TMA can read (paged_tma.cuh): a fifth warp produces. It walks the same segments ahead of the others, through the ends
@@ -318,7 +375,7 @@ struct RowsArgs { int box_rows, k_heads_inner, v_heads_inner; };
 constexpr int TMA_THREADS = 160;
 template <int D, int MT> constexpr int tma_ctas_per_sm() { return D == 128 ? 2 : (MT == 1 ? 3 : 2); }
 
-template <int D, int MT, bool BF16>
+template <int D, int MT, bool BF16, bool ALONE>
 __global__ void __launch_bounds__(TMA_THREADS, (tma_ctas_per_sm<D, MT>()))
 paged_rows_tma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Params p, const RowsArgs a, int* err) {
     using F = Fold<D, MT, BF16>;
@@ -427,6 +484,93 @@ paged_rows_tma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         if (s.parts > 1) merge = make_int4(s.r.q0 + block0, n_tok, s.hk, s.parts);
     }
     if (tid == 0) p.ws_merge[blockIdx.x] = merge;
+    if (ALONE) {
+        int nan_met;
+        asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.s32 a, %1, 0;\n\tbarrier.cta.red.or.pred b, 1, 128, a;\n\tselp.s32 %0, 1, 0, b;\n\t}"
+                     : "=r"(nan_met) : "r"((int)(f.nan_met && ok)) : "memory");
+        if (nan_met) repair<D, BF16>(p, (long long*)smem, tid, meet);
+    }
+}
+
+struct Merge { const float* ws_o; const float2* ws_ml; const int4* ws_merge; int rows, ctas; };      // one fold's partials
+
+// With the tensor-memory form, whose kernel is left as it is (a look at its sums costs it 2-5 %, one at its tiles 8-16), a few blocks of
+// the merge's launch look at some of the results instead: a value that is hidden from some rows of an item is seen by its last
+// token, or with a window by its first (by some token, where the window is shorter than the item), and a row that sees a value
+// that is not finite is not finite itself (zeros, where each of its few weights was 0). Where they find such a row they go over its item: rows
+// that hold a NaN are folded again over all keys that they see. Items that several CTAs share are written by the merging blocks,
+// which do the same for theirs. A warp's unit is CHECKS such rows of a request and kv head, every `split`-th.
+constexpr int CHECKS = 8;
+struct Look { int blocks, split; long long units; int few, tokens_few, tokens_many; };      // tokens of an item: of requests of up to `few` query rows, of others
+struct Items { int n, r0, r1; int4 item[16 * CHECKS]; };      // to go over: request, first token in its chunk, kv head, first token row; a merging block's one: rows [r0, r1)
+
+template <int D, bool BF16>
+__device__ __forceinline__ void go_over(const Params& p, const int4& it, int r0, int r1) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = (lane % (D / 4)) * 4;
+    const Req r = LoadReq{&p, nullptr}(it.x);
+    if (r.qn < 2) return;                          // a token alone: nothing is hidden from it
+    for (int k = r0 + warp; k < r1; k += 16) {
+        const int i = it.y + k / p.group, head = it.z * p.group + k % p.group, pos = r.kv - r.qn + i, t = r.q0 + i;
+        const int64_t at = ((int64_t)t * p.q_heads + head) * D + col;
+        if (i >= r.qn || pos < 0 || !__any_sync(0xffffffffu, holds_nan<BF16>(p, at))) continue;
+        float m, l, acc[4];
+        const bool summed = fold_row<D, BF16>(p, it.x, it.z, (const uint16_t*)p.q + (int64_t)t * p.q_token_stride + (int64_t)head * p.q_head_stride,
+                                              p.window > 0 ? max(0, pos - p.window + 1) : 0, pos + 1, 0.0f, col, m, l, acc);
+        if (lane < D / 4) store4<BF16>(p, at, acc, summed && l > 0.0f ? 1.0f / l : 0.0f);
+    }
+}
+
+template <int D, bool BF16>
+__device__ __forceinline__ void look_at_results(const Params& p, const Merge& first, const Merge& second, const Look& look, Items& items) {
+    constexpr int LANES = D / 8, ROWS = 32 / LANES;      // lanes of a row, rows of a load
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    long long u = (long long)blockIdx.x * 16 + warp;
+    int c0 = -1;                                   // the unit's next rows; -1: its first
+    if (threadIdx.x == 0) items.n = 0;
+    while (__syncthreads_or(u < look.units)) {     // (the block's turns end together: what one finds is gone over by all of its warps)
+        if (u < look.units) {
+            const long long v = u / look.split;
+            const int hk = (int)(v % p.kv_heads), b = (int)(v / p.kv_heads);
+            const Req r = LoadReq{&p, nullptr}(b);
+            const int bt = (long long)r.qn * p.group <= look.few ? look.tokens_few : look.tokens_many;
+            const int edges = p.window == 0 ? 1 : p.window >= bt ? 2 : bt;      // rows looked at per item
+            if (c0 < 0) c0 = (int)(u - v * look.split) * CHECKS;
+            const int c = c0 + lane % CHECKS, block0 = c / edges * bt, n_tok = min(bt, r.qn - block0);
+            const int i = block0 + (edges == bt ? c % edges : c % edges ? 0 : n_tok - 1);
+            long long off = -1;
+            if (n_tok > 1 && i < block0 + n_tok && r.kv - r.qn + i >= 0) off = ((long long)(r.q0 + i) * p.q_heads + hk * p.group) * D;
+            unsigned odd = 0u, full = 0u;          // not finite; not all zeros
+#pragma unroll
+            for (int k = 0; k < CHECKS; k += ROWS) {
+                const long long o = __shfl_sync(0xffffffffu, off, k + lane / LANES);
+                uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                if (o >= 0) x = __ldcg((const uint4*)((const uint16_t*)p.out + o + (lane % LANES) * 8));
+                constexpr uint32_t one = BF16 ? 0x00800080u : 0x04000400u;      // exponents all ones, in either half of a word
+                const uint32_t y = ((x.x & 0x7fff7fffu) + one) | ((x.y & 0x7fff7fffu) + one) | ((x.z & 0x7fff7fffu) + one) | ((x.w & 0x7fff7fffu) + one);
+                if (y & 0x80008000u) odd |= 1u << (k + lane / LANES);
+                if ((x.x | x.y | x.z | x.w) & 0x7fff7fffu) full |= 1u << (k + lane / LANES);
+            }
+            odd = __reduce_or_sync(0xffffffffu, odd);
+            full = __reduce_or_sync(0xffffffffu, full);
+            if (edges == bt) odd |= __ballot_sync(0xffffffffu, off >= 0 && lane < CHECKS) & ~full;
+            if (((odd >> lane) & 1u) && (__match_any_sync(odd, block0) & ((1u << lane) - 1u)) == 0u)      // one lane per item
+                items.item[atomicAdd(&items.n, 1)] = make_int4(b, block0, hk, r.q0 + block0);
+            c0 += look.split * CHECKS;
+            if (c0 >= (r.qn + bt - 1) / bt * edges) { u += (long long)look.blocks * 16; c0 = -1; }
+        }
+        __syncthreads();
+        for (int x = 0; x < items.n; ++x) {
+            const int4 it = items.item[x];
+            bool shared = false;                   // those are the merging blocks'
+            for (int c = lane; c < first.ctas + second.ctas; c += 32) {
+                const int4 m = c < first.ctas ? first.ws_merge[c] : second.ws_merge[c - first.ctas];
+                shared |= m.w > 1 && m.x == it.w && m.z == it.z;
+            }
+            if (!__any_sync(0xffffffffu, shared)) go_over<D, BF16>(p, it, 0, max(look.tokens_few, look.tokens_many) * p.group);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) items.n = 0;
+    }
 }
 
 // Merge of the items that several CTAs share, for one fold or for two that ran side by side. The item that starts in one CTA's
@@ -436,28 +580,25 @@ paged_rows_tma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 // (at least one) and joined through shared memory in a fixed order. Bound by latency: its start, an item's record, the partials (38 MB
 // at most, in L2), the join; 148 shared items of 256 rows 16-18 us.
 constexpr int TC_MERGE_SPLIT = 4;      // blocks per item of the tensor-memory form
-struct Merge { const float* ws_o; const float2* ws_ml; const int4* ws_merge; int rows; };      // one fold's partials
-template <int D, bool BF16>
-__global__ void __launch_bounds__(512) paged_merge_kernel(const Merge first, const Merge second, const int n_first, const int split_first, void* out, float* lse, const int q_heads, const int group) {
-    griddep_wait();
-    griddep_launch();
-    const bool one = blockIdx.x < n_first;
-    const int n_parts = one ? split_first : TC_MERGE_SPLIT, block = one ? blockIdx.x : blockIdx.x - n_first;
+// One block's part of a shared item; true (NOTE) where one of its rows came out NaN, noted in `items`.
+template <int D, bool BF16, bool NOTE>
+__device__ __forceinline__ bool merge_item(const Params& p, const Merge& first, const Merge& second, int index, int n_first, int split_first, float2 (&s_ml)[16], float (&s_o)[16][D], Items* items) {
+    const bool one = index < n_first;
+    const int n_parts = one ? split_first : TC_MERGE_SPLIT, block = one ? index : index - n_first;
     const int cta = block / n_parts, part = block - cta * n_parts;
     // field by field: a reference to one of two parameters would be read through memory at every use
     const float* ws_o = one ? first.ws_o : second.ws_o;
     const float2* ws_ml = one ? first.ws_ml : second.ws_ml;
     const int slot_rows = one ? first.rows : second.rows;
     const int4 it = (one ? first.ws_merge : second.ws_merge)[cta];
-    if (it.w <= 1) return;
-    __shared__ float2 s_ml[16];
-    __shared__ float s_o[16][D];
+    if (it.w <= 1) return false;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int V = D / 32;                      // floats per lane
-    const int rows = it.y * group, r0 = rows * part / n_parts, r1 = rows * (part + 1) / n_parts;
+    const int rows = it.y * p.group, r0 = rows * part / n_parts, r1 = rows * (part + 1) / n_parts;
     int wpr = 16;                                  // warps per row
     while (wpr > 1 && (r1 - r0) * wpr > 16) wpr >>= 1;
     const int rpp = 16 / wpr, sub = warp % wpr;    // rows at a time, this warp's share of the parts
+    bool met = false;                              // a row that came out NaN
     for (int rr = r0; rr < r1; rr += rpp) {
         const int r = rr + warp / wpr;
         float m = -INFINITY, l = 0.0f, o[V];
@@ -510,29 +651,56 @@ __global__ void __launch_bounds__(512) paged_merge_kernel(const Merge first, con
             __syncthreads();
         }
         if (r < r1 && sub == 0) {
-            const int tok = r / group, head = it.z * group + r - tok * group;
-            const int64_t at = (int64_t)(it.x + tok) * q_heads + head;
+            const int tok = r / p.group, head = it.z * p.group + r - tok * p.group;
+            const int64_t at = (int64_t)(it.x + tok) * p.q_heads + head;
             const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-            uint16_t* dst = (uint16_t*)out + at * D + lane * V;
+            uint16_t* dst = (uint16_t*)p.out + at * D + lane * V;
             *(uint32_t*)dst = pack2<BF16>(o[0] * inv, o[1] * inv);
             if (V == 4) *(uint32_t*)(dst + 2) = pack2<BF16>(o[V - 2] * inv, o[V - 1] * inv);
-            if (lse && lane == 0) lse[at] = (m + log2f(l) - p_shift<BF16>()) * LN2;
+            if (p.lse && lane == 0) p.lse[at] = (m + log2f(l) - p_shift<BF16>()) * LN2;
+            if (NOTE) {
+                float all = o[0] + o[1];
+                if (V == 4) all += o[V - 2] + o[V - 1];
+                met |= all != all;
+            }
         }
     }
+    if (!NOTE || !__syncthreads_or(met)) return false;
+    if (threadIdx.x == 0) {                        // the request: the last that starts at or before the item
+        int b = 0, hi = p.n_requests - 1;
+        while (b < hi) { const int mid = (b + hi + 1) >> 1; if (__ldcg(p.query_start + mid) <= it.x) b = mid; else hi = mid - 1; }
+        items->r0 = r0; items->r1 = r1;
+        items->item[0] = make_int4(b, it.x - LoadReq{&p, nullptr}(b).q0, it.z, it.x);
+    }
+    __syncthreads();
+    return true;
 }
 
-template <int D, int MT, bool BF16>
+// LOOK: with the blocks that look at results in front. p: of all requests, whichever form served them.
+template <int D, bool BF16, bool LOOK>
+__global__ void __launch_bounds__(512) paged_merge_kernel(const __grid_constant__ Params p, const Merge first, const Merge second, const Look look, const int n_first, const int split_first) {
+    griddep_wait();
+    griddep_launch();
+    struct Rows { float2 ml[16]; float o[16][D]; };
+    struct Nothing {};
+    __shared__ union { Rows rows; std::conditional_t<LOOK, Items, Nothing> items; } sh;
+    Items* items = (Items*)&sh;
+    if (LOOK && blockIdx.x < look.blocks) look_at_results<D, BF16>(p, first, second, look, *items);
+    else if (merge_item<D, BF16, LOOK>(p, first, second, blockIdx.x - look.blocks, n_first, split_first, sh.rows.ml, sh.rows.o, items)) go_over<D, BF16>(p, items->item[0], items->r0, items->r1);
+}
+
+template <int D, int MT, bool BF16, bool ALONE>
 int32_t launch_rows(sanic_ctx* ctx, const Params& p, bool tma, int ctas, cudaStream_t st) {
     constexpr int smem = Cfg<D>::RING;
     static_assert(4 * 16 * D * 4 <= Cfg<D>::STAGE_BYTES, "the warps' carriers fit a stage");
     static thread_local int ready_on = -1;       // the attribute is per device
     if (ready_on != ctx->device) {
-        SANIC_CUDA_CHECK(ctx, cudaFuncSetAttribute(paged_rows_kernel<D, MT, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        SANIC_CUDA_CHECK(ctx, cudaFuncSetAttribute(paged_rows_tma_kernel<D, MT, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem + 1024));
+        SANIC_CUDA_CHECK(ctx, cudaFuncSetAttribute(paged_rows_kernel<D, MT, BF16, ALONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        SANIC_CUDA_CHECK(ctx, cudaFuncSetAttribute(paged_rows_tma_kernel<D, MT, BF16, ALONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem + 1024));
         ready_on = ctx->device;
     }
     if (!tma) {
-        SANIC_CUDA_CHECK(ctx, launch_pdl(paged_rows_kernel<D, MT, BF16>, dim3(ctas), dim3(128), smem, st, p, ctx->status_dev));
+        SANIC_CUDA_CHECK(ctx, launch_pdl(paged_rows_kernel<D, MT, BF16, ALONE>, dim3(ctas), dim3(128), smem, st, p, ctx->status_dev));
         return SANIC_OK;
     }
     CUtensorMap mk, mv;
@@ -543,13 +711,13 @@ int32_t launch_rows(sanic_ctx* ctx, const Params& p, bool tma, int ctas, cudaStr
     if (rc == SANIC_OK) rc = encode_pool(ctx, &mv, BF16, p, 1, D, a.box_rows, &vi);
     if (rc != SANIC_OK) return rc;
     a.k_heads_inner = ki; a.v_heads_inner = vi;
-    SANIC_CUDA_CHECK(ctx, launch_pdl(paged_rows_tma_kernel<D, MT, BF16>, dim3(ctas), dim3(TMA_THREADS), smem + 1024, st, mk, mv, p, a, ctx->status_dev));
+    SANIC_CUDA_CHECK(ctx, launch_pdl(paged_rows_tma_kernel<D, MT, BF16, ALONE>, dim3(ctas), dim3(TMA_THREADS), smem + 1024, st, mk, mv, p, a, ctx->status_dev));
     return SANIC_OK;
 }
-template <int MT>
+template <int MT, bool ALONE>
 int32_t launch_rows_any(sanic_ctx* ctx, const Params& p, int D, int dtype, bool tma, int ctas, cudaStream_t st) {
-    if (D == 128) return dtype == SANIC_BF16 ? launch_rows<128, MT, true>(ctx, p, tma, ctas, st) : launch_rows<128, MT, false>(ctx, p, tma, ctas, st);
-    return dtype == SANIC_BF16 ? launch_rows<64, MT, true>(ctx, p, tma, ctas, st) : launch_rows<64, MT, false>(ctx, p, tma, ctas, st);
+    if (D == 128) return dtype == SANIC_BF16 ? launch_rows<128, MT, true, ALONE>(ctx, p, tma, ctas, st) : launch_rows<128, MT, false, ALONE>(ctx, p, tma, ctas, st);
+    return dtype == SANIC_BF16 ? launch_rows<64, MT, true, ALONE>(ctx, p, tma, ctas, st) : launch_rows<64, MT, false, ALONE>(ctx, p, tma, ctas, st);
 }
 
 // Resident CTAs of the rows form: what its shared memory (96 or 64 KB) and registers leave.
@@ -619,13 +787,26 @@ int32_t validate(sanic_ctx* ctx, const sanic_attn_paged_params* p) {
 }  // namespace
 
 namespace {
-cudaError_t launch_merge(const Params& a, int n_a, const Params& b, int n_b, int D, int dtype, cudaStream_t st) {
-    const int split = std::max(1, a.rows / 16);
-    const dim3 grid(n_a * split + n_b * TC_MERGE_SPLIT), block(512);
-    const Merge x{a.ws_o, a.ws_ml, a.ws_merge, a.rows}, y{b.ws_o, b.ws_ml, b.ws_merge, b.rows};
-    auto go = [&](auto kernel) { return launch_pdl(kernel, grid, block, 0, st, x, y, n_a * split, split, a.out, a.lse, a.q_heads, a.group); };
-    if (D == 128) return dtype == SANIC_BF16 ? go(paged_merge_kernel<128, true>) : go(paged_merge_kernel<128, false>);
-    return dtype == SANIC_BF16 ? go(paged_merge_kernel<64, true>) : go(paged_merge_kernel<64, false>);
+// a: the rows form's launch with n_a CTAs, b: the tensor-memory form's; 0 CTAs: not launched
+cudaError_t launch_merge(int sm_count, const Params& a, int n_a, const Params& b, int n_b, int max_query_len, int D, int dtype, cudaStream_t st) {
+    const int split = std::max(1, a.rows / 16), n_first = n_a * split;
+    Look look{};
+    if (n_b && b.n_tokens > 1) {       // (a token alone hides nothing)
+        const int longest = std::min(max_query_len ? max_query_len : INT32_MAX, b.n_tokens), items = (longest + b.block_tokens - 1) / b.block_tokens;
+        look.split = std::max(1, (b.window == 0 ? items : b.window >= b.block_tokens ? 2 * items : longest) / CHECKS);
+        look.units = (long long)b.n_requests * b.kv_heads * look.split;
+        look.blocks = (int)std::min<long long>((look.units + 15) / 16, 2 * sm_count);
+        look.few = n_a ? a.rows_upto : 0; look.tokens_few = n_a ? a.block_tokens : 1; look.tokens_many = b.block_tokens;
+    }
+    Params p = b;
+    p.rows_above = 0; p.rows_upto = INT32_MAX;
+    const dim3 grid(look.blocks + n_first + n_b * TC_MERGE_SPLIT), block(512);
+    const Merge x{a.ws_o, a.ws_ml, a.ws_merge, a.rows, n_a}, y{b.ws_o, b.ws_ml, b.ws_merge, b.rows, n_b};
+    auto go = [&](auto kernel) { return launch_pdl(kernel, grid, block, 0, st, p, x, y, look, n_first, split); };
+    auto of = [&](auto d, auto bf16) { return look.blocks ? go(paged_merge_kernel<d.value, bf16.value, true>) : go(paged_merge_kernel<d.value, bf16.value, false>); };
+    using std::integral_constant;
+    if (D == 128) return dtype == SANIC_BF16 ? of(integral_constant<int, 128>{}, std::true_type{}) : of(integral_constant<int, 128>{}, std::false_type{});
+    return dtype == SANIC_BF16 ? of(integral_constant<int, 64>{}, std::true_type{}) : of(integral_constant<int, 64>{}, std::false_type{});
 }
 }  // namespace
 
@@ -665,9 +846,14 @@ int32_t sanic_attn_paged(sanic_ctx* ctx, const sanic_attn_paged_params* p, void*
         ws = place(q, ws, pl.rows_ctas, pl.rows, p->head_dim);
         q.block_tokens = pl.rows / q.group;
         if (pl.tc) { q.rows_upto = t.rows_above = pl.rows; t.beside = 1; }
-        rc = pl.rows == 16   ? launch_rows_any<1>(ctx, q, p->head_dim, p->dtype, pool_supported(p, KT), pl.rows_ctas, st)
-             : pl.rows == 32 ? launch_rows_any<2>(ctx, q, p->head_dim, p->dtype, pool_supported(p, KT), pl.rows_ctas, st)
-                             : launch_rows_any<4>(ctx, q, p->head_dim, p->dtype, pool_supported(p, KT), pl.rows_ctas, st);
+        const bool tma = pool_supported(p, KT);
+        auto launch = [&](auto mt) {
+            return pl.tc ? launch_rows_any<mt.value, false>(ctx, q, p->head_dim, p->dtype, tma, pl.rows_ctas, st)
+                         : launch_rows_any<mt.value, true>(ctx, q, p->head_dim, p->dtype, tma, pl.rows_ctas, st);
+        };
+        rc = pl.rows == 16   ? launch(std::integral_constant<int, 1>{})
+             : pl.rows == 32 ? launch(std::integral_constant<int, 2>{})
+                             : launch(std::integral_constant<int, 4>{});
         if (rc != SANIC_OK) return rc;
     }
     if (pl.tc) {
@@ -676,7 +862,7 @@ int32_t sanic_attn_paged(sanic_ctx* ctx, const sanic_attn_paged_params* p, void*
         rc = tc_launch(ctx, t, p->head_dim, p->dtype, pl.tc_ctas, st);
         if (rc != SANIC_OK) return rc;
     }
-    SANIC_CUDA_CHECK(ctx, launch_merge(q, pl.rows ? pl.rows_ctas : 0, t, pl.tc ? pl.tc_ctas : 0, p->head_dim, p->dtype, st));
+    SANIC_CUDA_CHECK(ctx, launch_merge(ctx->sm_count, q, pl.rows ? pl.rows_ctas : 0, t, pl.tc ? pl.tc_ctas : 0, p->max_query_len, p->head_dim, p->dtype, st));
     return SANIC_OK;
 }
 

@@ -172,6 +172,74 @@ def test_attn_long_chunks_heads_and_windows(dev, d, hq, hkv, window):
 
 
 @pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("page", [16, 20])
+@pytest.mark.parametrize("maxq", [1, 5, 200])
+@pytest.mark.parametrize("window", [0, 40])
+def test_attn_hidden_keys_and_values_of_any_kind(dev, d, dtype, page, maxq, window):
+    """Keys and values of the chunk's own tokens that are infinite or NaN: tokens that see them have what the formula gives, tokens
+    that do not (before them, or past the window) their finite result. Long caches, whose items several CTAs share, among them."""
+    new, ctx, hq, hkv = [70, 9, 1, 3, 300], [300, 20000, 64, 0, 1100], 8, 2
+    args, keys, values = make_problem(dev, new, ctx, hq, hkv, d, dtype, page, window=window, seed=page + maxq)
+    inf, nan = math.inf, math.nan
+
+    def put(pool, mine, b, pos, col, x):       # into a request's row and the page that holds it
+        mine[b][pos, :, col] = x
+        args[pool][args["block_table"][b, pos // page].long(), pos % page, :, col] = x
+
+    for pos, col, x in ((305, slice(None), nan), (310, 3, inf), (311, 5, -inf), (330, 3, -inf), (369, slice(0, 8), nan)):
+        put("v_pages", values, 0, pos, col, x)
+    for pos, col, x in ((20004, slice(1, 60, 2), inf), (20007, slice(None), nan)):
+        put("v_pages", values, 1, pos, col, x)
+    put("k_pages", keys, 1, 20006, 9, nan)
+    put("v_pages", values, 3, 2, slice(None), -inf)
+    if window:
+        put("v_pages", values, 4, 1075, slice(0, 32), nan)        # the first 15 tokens see it, the others no longer
+    put("v_pages", values, 4, 1290, slice(16, None), nan)
+    put("k_pages", keys, 4, 1340, slice(None), nan)
+    kv = [c + n for c, n in zip(ctx, new)]
+    got, lse = dev.attn_paged(**args, max_query_len=maxq, window=window, return_lse=True)
+    dev.sync()
+    want, amp, wl = plain_attention(args["q"], keys, values, new, kv, window, d ** -0.5)
+    fine = torch.isfinite(want)
+    assert fine.sum() > want.numel() // 2 and not fine.all()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), (torch.isnan(got) != torch.isnan(want)).nonzero()[:4].tolist()
+    assert torch.equal(got.double()[torch.isinf(want)], want[torch.isinf(want)])
+    u = torch.finfo(got.dtype).eps / 2
+    assert ((got.double() - want).abs()[fine] <= (u * want.abs() + (u + 2.5e-4) * amp)[fine]).all()
+    fine = torch.isfinite(wl)
+    assert torch.equal(torch.isfinite(lse), fine) and ((lse.double() - wl).abs()[fine] <= 1.5e-4).all()
+
+
+@pytest.mark.parametrize("maxq", [33, 100])
+def test_attn_hidden_values_in_more_blocks_than_are_noted(dev, maxq):
+    # 100 tokens of 400 requests over 32 kv heads: a NaN value in both blocks of every one of them, at tokens 40 and 90
+    n, t, hkv, group, d, page, td = 400, 100, 32, 4, 64, 16, dev.torch_device
+    g = gen(dev, 41)
+    per = -(-t // page)
+    k, v = (torch.randn(n * per, page, hkv, d, generator=g, device=td).to(torch.bfloat16) for _ in range(2))
+    table = torch.randperm(n * per, generator=g, device=td).to(torch.int32).view(n, per)
+    for i, cols in ((40, slice(3, 20)), (90, slice(17, 40))):
+        v[table[:, i // page].long(), i % page, :, cols] = math.nan
+    q = torch.randn(n * t, hkv * group, d, generator=g, device=td).to(torch.bfloat16)
+    got = dev.attn_paged(q, k, v, table, ints(dev, list(range(0, n * t + 1, t))), ints(dev, [t] * n), max_query_len=maxq)
+    dev.sync()
+    hidden = torch.ones(t, t, dtype=torch.bool, device=td).triu(1)
+    for b in range(0, n, 20):
+        rows = table[b:b + 20].long()
+        kk, vv = (x[rows].flatten(1, 2)[:, :t].double().transpose(1, 2).repeat_interleave(group, 1) for x in (k, v))
+        s = q[b * t:(b + 20) * t].view(20, t, hkv * group, d).double().transpose(1, 2) @ kk.transpose(2, 3) * 0.125
+        w = torch.softmax(s.masked_fill(hidden, -math.inf), -1)
+        want, amp = w @ torch.nan_to_num(vv), w @ torch.nan_to_num(vv).abs()
+        want[:, :, 40:, 3:20] = math.nan
+        want[:, :, 90:, 17:40] = math.nan
+        have = got[b * t:(b + 20) * t].view(20, t, hkv * group, d).double().transpose(1, 2)
+        nan = torch.isnan(want)
+        assert torch.equal(torch.isnan(have), nan)
+        assert ((have - want).abs()[~nan] <= (2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.5e-4) * amp)[~nan]).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
 def test_attn_blocks_of_one_tile_before_blocks_of_two(dev, d):
     # every head's items are a block of two tiles and one of a single row; an uneven number of them per CTA, so that the second
     # tile's warps pass over long segments that the first tile still folds and wait for their own behind those
