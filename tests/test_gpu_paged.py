@@ -211,6 +211,39 @@ def test_attn_hidden_keys_and_values_of_any_kind(dev, d, dtype, page, maxq, wind
     assert torch.equal(torch.isfinite(lse), fine) and ((lse.double() - wl).abs()[fine] <= 1.5e-4).all()
 
 
+@pytest.mark.parametrize("hq,hkv", [(2, 2), (7, 1), (40, 1), (64, 1)])
+@pytest.mark.parametrize("window", [1, 3, 64, 100, 300])
+@pytest.mark.parametrize("maxq", [1, 300])
+def test_attn_values_that_leave_the_window_and_a_replay_over_others(dev, hq, hkv, window, maxq):
+    """Values that are not finite below and inside the window's edges, in blocks of every size a form makes of a chunk; then the
+    same graph over finite values."""
+    new, ctx, d, page = [300, 40, 2], [700, 5, 130], 64, 16
+    args, keys, values = make_problem(dev, new, ctx, hq, hkv, d, "bf16", page, window=window, seed=window + hq)
+    dev.attn_paged(**args, max_query_len=maxq, window=window)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got, lse = dev.attn_paged(**args, max_query_len=maxq, window=window, return_lse=True)
+    spots = [(b, p, c, x) for b, p, c, x in ((0, 700 - window + 1, 3, math.nan), (0, 700 - window // 2, 60, -math.inf), (0, 801, 7, math.inf),
+                                             (0, 999, slice(None), math.nan), (1, 6, 1, math.nan), (1, 44, 2, math.inf), (2, 131, 5, math.nan)) if p >= 0]
+    kv = [c + n for c, n in zip(ctx, new)]
+    for poisoned in (True, False):
+        for b, pos, col, x in spots:
+            if not poisoned:
+                x = 0.25
+            values[b][pos, :, col] = x
+            args["v_pages"][args["block_table"][b, pos // page].long(), pos % page, :, col] = x
+        graph.replay()
+        dev.sync()
+        want, amp, wl = plain_attention(args["q"], keys, values, new, kv, window, d ** -0.5)
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), (torch.isnan(got) != torch.isnan(want)).nonzero()[:4].tolist()
+        assert torch.equal(got.double()[torch.isinf(want)], want[torch.isinf(want)])
+        fine = torch.isfinite(want)
+        assert fine.all() != poisoned
+        assert ((got.double() - want).abs()[fine] <= (2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.5e-4) * amp)[fine]).all()
+        assert ((lse.double() - wl).abs() <= 1.5e-4).all()
+
+
 @pytest.mark.parametrize("maxq", [33, 100])
 def test_attn_hidden_values_in_more_blocks_than_are_noted(dev, maxq):
     # 100 tokens of 400 requests over 32 kv heads: a NaN value in both blocks of every one of them, at tokens 40 and 90
