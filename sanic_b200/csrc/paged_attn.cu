@@ -527,6 +527,9 @@ __device__ __forceinline__ void look_at_results(const Params& p, const Merge& fi
     long long u = (long long)blockIdx.x * 16 + warp;
     int c0 = -1;                                   // the unit's next rows; -1: its first
     if (threadIdx.x == 0) items.n = 0;
+    // The first turn is taken twice: while the folds still run, for the instructions and lengths that it fetches (their latencies are
+    // most of it), and for its result once they have ended.
+    bool ahead = true;
     while (__syncthreads_or(u < look.units)) {     // (the block's turns end together: what one finds is gone over by all of its warps)
         if (u < look.units) {
             const long long v = u / look.split;
@@ -553,11 +556,15 @@ __device__ __forceinline__ void look_at_results(const Params& p, const Merge& fi
             odd = __reduce_or_sync(0xffffffffu, odd);
             full = __reduce_or_sync(0xffffffffu, full);
             if (edges == bt) odd |= __ballot_sync(0xffffffffu, off >= 0 && lane < CHECKS) & ~full;
+            if (ahead) odd = 0u;
             if (((odd >> lane) & 1u) && (__match_any_sync(odd, block0) & ((1u << lane) - 1u)) == 0u)      // one lane per item
                 items.item[atomicAdd(&items.n, 1)] = make_int4(b, block0, hk, r.q0 + block0);
-            c0 += look.split * CHECKS;
-            if (c0 >= (r.qn + bt - 1) / bt * edges) { u += (long long)look.blocks * 16; c0 = -1; }
+            if (!ahead) {
+                c0 += look.split * CHECKS;
+                if (c0 >= (r.qn + bt - 1) / bt * edges) { u += (long long)look.blocks * 16; c0 = -1; }
+            }
         }
+        if (ahead) { griddep_wait(); ahead = false; }
         __syncthreads();
         for (int x = 0; x < items.n; ++x) {
             const int4 it = items.item[x];
@@ -679,7 +686,7 @@ __device__ __forceinline__ bool merge_item(const Params& p, const Merge& first, 
 // LOOK: with the blocks that look at results in front. p: of all requests, whichever form served them.
 template <int D, bool BF16, bool LOOK>
 __global__ void __launch_bounds__(512) paged_merge_kernel(const __grid_constant__ Params p, const Merge first, const Merge second, const Look look, const int n_first, const int split_first) {
-    griddep_wait();
+    if (!LOOK || blockIdx.x >= look.blocks) griddep_wait();
     griddep_launch();
     struct Rows { float2 ml[16]; float o[16][D]; };
     struct Nothing {};
