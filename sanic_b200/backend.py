@@ -45,6 +45,7 @@ class PageStep(NamedTuple):
 
 
 _HALF = {torch.bfloat16: abi.BF16, torch.float16: abi.F16}
+_MOST = 0x7fffffff     # of a 32-bit count of the C side
 
 
 class CudaDevice:
@@ -441,6 +442,9 @@ class CudaDevice:
         n_tokens = int(n_tokens)
         if n_tokens < 0:
             raise RunError("n_tokens must not be negative")
+        if max(n_tokens, page_size, block_table.shape[1], free_pages.numel()) > _MOST or page_size < -_MOST:      # what the C side would not see
+            raise RunError(f"n_tokens, page_size, the table's width and the free list's length must fit 32 bits, got {n_tokens}, {page_size}, "
+                           f"{block_table.shape[1]}, {free_pages.numel()}")
         # one allocation for all outputs: an allocation or a view costs more host time than the kernel takes
         block = seq_lens.new_empty(3 * n_tokens + 3 * n + 2, dtype=i32)
         slots, start, kv, held, count, pos = block.unsafe_split_with_sizes((2 * n_tokens, n + 1, n, n, 1, n_tokens))
@@ -528,6 +532,8 @@ class CudaDevice:
         T, hq, d = q.shape
         n_pages, page_size, hkv, dk = k_pages.shape
         n, max_pages = block_table.shape
+        if min(window, max_query_len) < 0:
+            raise RunError(f"window and max_query_len must not be negative, got {window} and {max_query_len}")
         if dk != d or q.dtype != k_pages.dtype:
             raise RunError(f"attention shapes disagree: q {tuple(q.shape)} {q.dtype}, pages {tuple(k_pages.shape)} {k_pages.dtype}")
         if out is None:
@@ -539,8 +545,8 @@ class CudaDevice:
         p = abi.AttnPagedParams(
             q.data_ptr(), out_ptr, lse.data_ptr() if return_lse else None, k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
             self._flat("query_start", query_start, torch.int32, n + 1), self._flat("kv_lens", kv_lens, torch.int32, n), None, 0,
-            qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], ts[0], _HALF[q.dtype], n, T, min(int(max_query_len), 0x7fffffff), hq, hkv, d, page_size,
-            n_pages, max_pages, min(int(window), 0x7fffffff), float(scale) if scale is not None else 1.0 / math.sqrt(d))
+            qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], ts[0], _HALF[q.dtype], n, T, min(int(max_query_len), _MOST), hq, hkv, d, page_size,
+            n_pages, max_pages, min(int(window), _MOST), float(scale) if scale is not None else 1.0 / math.sqrt(d))
         # a workspace per call: calls on other streams, and graphs that replay side by side, never share one
         nbytes = self.lib.sanic_attn_paged_workspace_bytes(self.h, C.byref(p))
         ws = kv_lens.new_empty(nbytes // 4)

@@ -174,6 +174,24 @@ def test_host_refusals():
     refuses("requests, drafts", ve, draft_tokens=z(6))
 
 
+def test_host_refuses_numbers_that_would_wrap():
+    # the C side counts in 32 bits: 2^32 + 16 would be a page of 16 rows, a window of -2^32 none
+    d = HostDevice()
+    i32, bf = torch.int32, torch.bfloat16
+    z = lambda *s, t=i32: torch.zeros(*s, dtype=t)
+    good = dict(seq_lens=z(3), new_lens=z(3), block_table=z(3, 4), free_pages=z(9), free_count=z(1), page_size=16, n_tokens=5)
+    ap = lambda **kw: d.page_table_append(**dict(good, **kw))
+    refuses("32 bits", ap, page_size=2 ** 32 + 16)
+    refuses("32 bits", ap, page_size=16 - 2 ** 32)
+    refuses("32 bits", ap, n_tokens=2 ** 32 + 5)
+    refuses("32 bits", ap, block_table=torch.zeros(3, 2 ** 32 + 4, dtype=i32, device="meta"))       # (no memory behind them)
+    refuses("32 bits", ap, free_pages=torch.zeros(2 ** 32 + 9, dtype=i32, device="meta"))
+    good = dict(q=z(5, 4, 64, t=bf), k_pages=z(3, 16, 2, 64, t=bf), v_pages=z(3, 16, 2, 64, t=bf), block_table=z(2, 3), query_start=z(3), kv_lens=z(2))
+    at = lambda **kw: d.attn_paged(**dict(good, **kw))
+    refuses("window", at, window=-2 ** 32)
+    refuses("max_query_len", at, max_query_len=-2 ** 32)
+
+
 def test_entry_points_refuse_a_null_context():
     lib = abi.load()
     assert lib.sanic_page_table_append(None, C.byref(abi.PageAppendParams()), None) == abi.ERR_INVALID
