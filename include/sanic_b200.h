@@ -615,7 +615,7 @@ int32_t sanic_paged_cache_write(sanic_ctx* ctx, const sanic_paged_write_params* 
  * its window, behind kv_lens) do not count for it, whatever the pages hold there, infinities and NaN included. (Where later tokens of
  * a chunk hold such values, the earlier ones are folded again one by one, which takes some milliseconds.) out and lse overlap no
  * input. Scores, maxima, sums and the output accumulator are f32; the weights exp(s - max) are rounded to dtype for the product with v. max_query_len, a bound on the
- * chunk lengths (0: n_tokens), only selects a kernel: a longer chunk is still computed. dtype SANIC_BF16 or SANIC_F16,
+ * chunk lengths (0: n_tokens), only selects kernels: a longer chunk is still computed, but short ones are served faster where it is given. dtype SANIC_BF16 or SANIC_F16,
  * head_dim 64 or 128, at most 64 query heads per kv head. A table entry outside [0, n_pages) reads as zeros; it, and lengths
  * past the table row or n_tokens (clamped), are reported (code 54). Any page size and strides are served; fastest are pages of a
  * multiple of 16 rows whose strides nest (rows and heads of a page in either order), slowest (about 4x for long chunks, 1.3x
@@ -642,7 +642,8 @@ size_t sanic_attn_paged_workspace_bytes(sanic_ctx* ctx, const sanic_attn_paged_p
  * u_sample[b] times their total, in index order, sums in f64; weights that are NaN, infinite or not positive count as 0. tokens_out
  * [n, max_draft + 1]: accepted drafts, the drawn token (-1 if no weight is positive), -1 behind it; accepted [n]: the count of drafts
  * accepted. A draft token outside the vocabulary is rejected, draft lengths are clamped to [0, max_draft], a target row outside
- * [0, target_rows) ends the request with -1; each is reported (code 55). */
+ * [0, target_rows) ends the request with -1; each is reported (code 55). Every request of the call is given a token: one that pauses (no
+ * target row of its own) is left out of the call, since the row that its target_start names is another request's. */
 typedef struct {
     const float* target_probs; int64_t target_stride; int32_t target_rows; const int32_t* target_start;
     const float* draft_probs; int64_t draft_request_stride, draft_stride;     /* [n, max_draft, vocab] or NULL; requests may share rows (stride 0) */

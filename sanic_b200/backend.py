@@ -525,7 +525,8 @@ class CudaDevice:
         query_start[b] .. query_start[b + 1], its last token standing at key kv_lens[b] - 1 (the chunk's own keys are in the pages
         already). k_pages, v_pages [n_pages, page_size, Hkv, D] (any strides), block_table [n, max_pages], query_start [n + 1] and
         kv_lens [n] int32. -> out [n_tokens, Hq, D] (or into `out`), and with return_lse the log-sum-exp [n_tokens, Hq] f32.
-        max_query_len, a bound on the chunks known on the host, selects the kernel. Rows outside every chunk stay unwritten."""
+        max_query_len, a bound on the chunks known on the host, selects the kernel (left out: slower for short chunks). Rows outside
+        every chunk stay unwritten; `out` overlaps no input."""
         qs = self._paged("q", q, (torch.bfloat16, torch.float16), 3)
         ks, vs = self._pages(k_pages, v_pages)
         ts = self._paged("block_table", block_table, (torch.int32,), 2)
@@ -558,7 +559,8 @@ class CudaDevice:
         """Rejection sampling of drafted tokens (see sanic_draft_verify). target_probs [rows, vocab] f32: request b's rows start at
         target_start[b] (default b * (K + 1)), one per draft and one more; draft_tokens [n, K] int32, draft_probs [n, K, vocab] f32
         (None: drafts made without probabilities), draft_lens [n] int32 (None: all K); u_accept [n, K] and u_sample [n] f32 in [0, 1).
-        -> tokens [n, K + 1] int32 (kept drafts, the drawn token, then -1) and the number of drafts kept [n] int32."""
+        -> tokens [n, K + 1] int32 (kept drafts, the drawn token, then -1) and the number of drafts kept [n] int32. A request without
+        a target row of its own (one that pauses) is left out of the call."""
         ts = self._paged("target_probs", target_probs, (torch.float32,), 2)
         rows, vocab = target_probs.shape
         if draft_tokens.dim() != 2:

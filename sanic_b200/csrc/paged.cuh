@@ -23,7 +23,9 @@ struct Params : Shape {
     float scale;
     int rows;              // rows of a partial slot (at least block_tokens * group)
     int rows_above, rows_upto;   // requests of this launch: those whose chunk has more and at most this many query rows
-    int beside;            // 1: this launch runs beside the one before it (the other class of requests) and waits for it at its end
+    int beside;            // 1: this launch may start before the one before it (the other class of requests) has ended, and waits for it at
+                           // its end. Each needs most of an SM (196 KB of shared memory for the rows form's CTAs, 226 for the other's), so
+                           // the two follow one another on every SM; what is saved is the gap between launches.
     // workspace: float [2 * ctas][rows][head_dim], float2 (max in log2 units, sum) [2 * ctas][rows], one int4 per CTA: the item
     // that starts in its range and is shared with the next CTAs (first token row, tokens, kv head, CTAs that hold a part; 0: none)
     float* ws_o; float2* ws_ml; int4* ws_merge;

@@ -11,7 +11,7 @@
 // per SM instead of three: 77 instead of 67 us for 64 decodes of 2000 keys.) The rows of an item are 16 MT rows of m16n8k16
 // MMAs: with MT = 1 each warp takes 16 of the tile's keys, with MT = 2 a warp takes 16 rows and half of the keys, with MT = 4 a
 // warp takes 16 rows and all keys. Carriers stay in registers; the warps that share rows merge once per segment. P goes to the tensor core rounded
-// to the storage type (bf16: 2^-9 per weight; f16 likewise after a shift by 2^8, which keeps the weights of a long flat
+// to the storage type (off by at most 2^-8 of a weight in bf16, 2^-11 in f16, there after a shift by 2^8, which keeps the weights of a long flat
 // softmax out of f16's subnormals), sums and maxima are f32.
 // The work is spread over an exactly resident grid as one contiguous range of (item, key tile) per CTA (paged_sched.h).
 // 64 decodes of 8000 keys on average, 32 + 8 heads of 128, bf16 (2.14 GB): 340 us = 6.3 TB/s, 0.96 of the measured copy rate.
@@ -26,7 +26,10 @@ using namespace sanic::paged;
 constexpr int KT = 64;
 // Chunks of more query rows than this (tokens * heads of a group) go to the tensor-memory form where its loads suit the layout.
 // Groups of 4 heads of 128 over 4000 keys, rows form against tensor-memory form: 20 rows of 32 requests 104 / 125 us, 32 rows
-// 107 / 126 us, 64 rows of 16 requests 92 / 80 us, of 2 requests 53 / 28 us.
+// 107 / 126 us, 64 rows of 16 requests 92 / 80 us, of 2 requests 53 / 28 us. That is the border where no request may have more (by
+// max_query_len, or by n_tokens where it is left out). Where one may, two launches share the requests and the border is what a
+// single token of the group needs, 16 rows for groups up to 16 (make_plan): a rows form of 32 rows would fold single tokens, the most
+// of such a batch, in items of twice the rows. Drafts beside a prompt, or without max_query_len, are served slower for it.
 constexpr int TC_ABOVE_ROWS = 32;
 
 template <int D> struct Cfg {
@@ -372,6 +375,7 @@ __global__ void __launch_bounds__(128) paged_rows_kernel(const __grid_constant__
 // back, each for itself: no barrier between tiles. (With the copies issued by the folding warps: 434 us by cp.async, 363 us
 // by TMA from warp 0, for 64 requests of 8000 keys on average.)
 struct RowsArgs { int box_rows, k_heads_inner, v_heads_inner; };
+// Registers: at head_dim 128 two CTAs per SM leave a thread 168; 32, 56 and 132 bytes spill for 16, 32 and 64 rows.
 constexpr int TMA_THREADS = 160;
 template <int D, int MT> constexpr int tma_ctas_per_sm() { return D == 128 ? 2 : (MT == 1 ? 3 : 2); }
 
@@ -584,8 +588,8 @@ __device__ __forceinline__ void look_at_results(const Params& p, const Merge& fi
 // range is served by a block per 16 rows of the rows form's items (24 drafted chunks of 3-6 tokens: 97.5 us with one block per item,
 // 95.7 so, 99 with a block per 8 rows), by four blocks of the tensor-memory form's (all resident at once: 16 drafted chunks of 16 tokens 78.3
 // us, 81.2 with eight, 87.8 with 16; two or four rows of a warp at once: 79.5-85). A row's partials are split over 16 / rows warps
-// (at least one) and joined through shared memory in a fixed order. Bound by latency: its start, an item's record, the partials (38 MB
-// at most, in L2), the join; 148 shared items of 256 rows 16-18 us.
+// (at least one) and joined through shared memory in a fixed order. Bound by latency: its start, an item's record, the partials (39 MB
+// at most of the tensor-memory form and 20 MB of the rows form, in L2), the join; 148 shared items of 256 rows 16-18 us.
 constexpr int TC_MERGE_SPLIT = 4;      // blocks per item of the tensor-memory form
 // One block's part of a shared item; true (NOTE) where one of its rows came out NaN, noted in `items`.
 template <int D, bool BF16, bool NOTE>
