@@ -577,7 +577,7 @@ __device__ __forceinline__ void look_at_results(const Params& p, const Merge& fi
                 const int4 m = c < first.ctas ? first.ws_merge[c] : second.ws_merge[c - first.ctas];
                 shared |= m.w > 1 && m.x == it.w && m.z == it.z;
             }
-            if (!__any_sync(0xffffffffu, shared)) go_over<D, BF16>(p, it, 0, max(look.tokens_few, look.tokens_many) * p.group);
+            if (!__any_sync(0xffffffffu, shared)) go_over<D, BF16>(p, it, 0, look.tokens_many * p.group);      // (a chunk of the other form is one item, and smaller)
         }
         __syncthreads();
         if (threadIdx.x == 0) items.n = 0;

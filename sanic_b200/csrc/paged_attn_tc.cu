@@ -21,9 +21,8 @@
 //
 // Bound: 4 rows keys head_dim flop on the tensor pipe (8192 per clock and SM) against one exponential per score on the SFU (16
 // per clock and SM): equal at head_dim 128, SFU-bound at 64. Measured, 32 + 8 heads, bf16, replayed from a graph: 2048 tokens over
-// 30,000 keys of 128 960 us = 1085 TFLOP/s, 0.65 of the measured matrix-product rate (at the power cap, back to back for seconds, 1130
-// us); 8 prompts of 4096 of 128 1185 us = 928 TFLOP/s, of 64 1002 us = 549
-// TFLOP/s. A 256 x 128 block of scores takes 3840 clocks
+// 30,000 keys of 128 950-960 us = 1090 TFLOP/s, 0.65 of the measured matrix-product rate (at the power cap, back to back for seconds,
+// 1140); 8 prompts of 4096 of 128 1185 us = 928 TFLOP/s, of 64 1002 us = 549 TFLOP/s. A 256 x 128 block of scores takes 3840 clocks
 // where either pipe needs 2048: a tile's exponentials (2000) and its products with four barrier hops (1800) follow one another, and only
 // the other tile's lie over them. (Tile 0 leaving out a last key tile that only tile 1 sees: 4 % slower at head_dim 128 even so, since
 // the tiles fall out of the order below; descriptors and ring places computed ahead of the issuer's waits: the same 4 %.)
